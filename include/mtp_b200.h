@@ -264,6 +264,119 @@ MTP_API int mtp_w4a16_moe_prefill_tables(int32_t num_tokens, int32_t num_experts
                                          MtpPrefillTables* out);
 
 
+/* ---- tokens sorted by expert and back --------------------------------------- */
+enum MtpDtype {
+  MTP_DTYPE_BF16 = 0,
+  MTP_DTYPE_FP16 = 1,
+  MTP_DTYPE_FP32 = 2,
+  MTP_DTYPE_INT8 = 3
+};
+
+/* rows [M*k, H] = the rows of x in expert order: pair (t, j) has the key
+ * topk_ids[t, j] (through expert_map [global_num_experts] when given), or
+ * num_experts where that is no expert in [0, num_experts); its row is the
+ * number of pairs of a smaller key plus the earlier pairs of the same key, a
+ * stable order. Pairs without an expert come last and their rows are zero.
+ * positions [M, k] = the pair's row, or ~row (negative) without an expert;
+ * offsets [num_experts + 1] = first row of each expert, then the routed rows.
+ * x: any MtpDtype, rows x_stride elements apart; x and rows both NULL: positions
+ * and offsets only. row_scales [M] (with sorted_scales [M*k]): one fp32 per
+ * row, sorted along (0 for a pair without an expert). num_experts <= 1024,
+ * k <= 32, M * k < 2^31. The gradient of x is mtp_unsort_tokens of the rows'
+ * gradient without weights. Same pair order as mtp_moe_align.              */
+MTP_API int mtp_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t H,
+                            const int32_t* topk_ids, int32_t k, int32_t num_experts, const int32_t* expert_map,
+                            int32_t global_num_experts, const float* row_scales, void* rows, float* sorted_scales,
+                            int32_t* positions, int32_t* offsets, void* stream);
+
+/* out [M, H] = sum over j with positions[t, j] >= 0, ascending, of
+ * weights[t, j] * rows[positions[t, j]] in fp32, rounded once to the rows'
+ * type (bf16, fp16 or fp32). weights [M, k] fp32, NULL = 1. A token without
+ * routed pairs gets zeros. A position outside [0, num_rows) counts as none.  */
+MTP_API int mtp_unsort_tokens(const void* rows, int64_t num_rows, int32_t dtype, const int32_t* positions,
+                              const float* weights, int32_t M, int32_t k, int32_t H, void* out, void* stream);
+
+/* Its gradient for grad [M, H]: grad_rows[positions[t, j]] = weights[t, j] *
+ * grad[t] (rows of unrouted pairs: zero), grad_weights[t, j] = <grad[t],
+ * rows[positions[t, j]]> summed in fp32 in a fixed order (unrouted: 0). Either
+ * output may be NULL; rows may be NULL without grad_weights. positions as
+ * mtp_sort_tokens writes them: every row belongs to exactly one pair.       */
+MTP_API int mtp_unsort_tokens_backward(const void* grad, const void* rows, int64_t num_rows, int32_t dtype,
+                                       const int32_t* positions, const float* weights, int32_t M, int32_t k,
+                                       int32_t H, void* grad_rows, float* grad_weights, void* stream);
+
+/* ---- int8 (W8A8) ------------------------------------------------------------- */
+/* One scale per row: scale = max|x| / 127, q = round(x * (127 / max|x|)), half
+ * to even, in fp32. A row of zeros has scale 0; a row with an infinity or a NaN
+ * has that scale and codes 0, so its products are NaN. x: bf16, fp16 or fp32,
+ * rows x_stride elements apart; q rows q_stride bytes apart.                */
+MTP_API int mtp_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t K, int8_t* q,
+                              int64_t q_stride, float* scale, void* stream);
+
+enum MtpActivation {
+  MTP_ACT_NONE = 0,
+  MTP_ACT_SILU_MUL = 1   /* out[:, i] = silu(z[:, i]) * z[:, n/2 + i]        */
+};
+
+/* z = (a . b^T) * a_scale[row] * b_scale[channel] (+ bias[channel]), the sum
+ * exact in int32, scales in fp32, rounded once to out_dtype.
+ * offsets NULL: one product, b [n, k]. With offsets [num_groups + 1]: rows
+ * offsets[g] .. offsets[g + 1] use b[g] of [num_groups, n, k] and b_scale[g];
+ * rows from offsets[num_groups] on are written as zeros (offsets[0] = 0, as
+ * mtp_sort_tokens gives them).
+ * a_dtype int8: a [rows, k] with a_scale [rows]. Else a is bf16, fp16 or fp32
+ * and is quantised as mtp_quantize_int8 does, in the workspace; a_scale NULL.
+ * k < 131072; num_groups <= 1024. Rows of a (int8) or b that are not 16-byte
+ * aligned with a stride of a multiple of 16 are first copied into the workspace;
+ * k a multiple of 16 needs no copy.                                         */
+typedef struct MtpInt8MatmulArgs {
+  int32_t rows, n, k, num_groups;
+  int32_t a_dtype, out_dtype, activation, reserved;
+  const void* a;
+  int64_t a_stride;            /* elements between rows of a                  */
+  const float* a_scale;
+  const int8_t* b;             /* contiguous                                  */
+  const float* b_scale;        /* [num_groups, n]                             */
+  const float* bias;           /* [n] or NULL (not with silu_mul)             */
+  const int32_t* offsets;
+  void* out;                   /* [rows, n], silu_mul: [rows, n / 2]          */
+  int32_t* status;             /* optional [1]: bit 0 is set when a bounded
+                                  wait ran out (the output is wrong then); the
+                                  caller zeroes it                           */
+  void* workspace;             /* 256-byte aligned; no zero fill needed       */
+  int64_t workspace_bytes;
+} MtpInt8MatmulArgs;
+MTP_API int mtp_int8_matmul_workspace_size(const MtpInt8MatmulArgs* args, int64_t* bytes);
+MTP_API int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream);
+
+/* The W8A8 mixture-of-experts layer: router (softmax, top-k, renormalise) or
+ * given topk_weights / topk_ids (with expert_map: global ids), rows of
+ * hidden_states quantised and sorted by expert, h = silu(gate) * up of the
+ * gate_up product kept in fp32, quantised per row, the down product rounded to
+ * dtype per pair, and the weighted sum of each token's pairs in fp32 rounded
+ * to dtype. w13 [E, 2I, H] (gate rows, then up rows), w2 [E, H, I] int8 with
+ * scales [E, 2I] and [E, H].                                                */
+typedef struct MtpW8A8LayerArgs {
+  int32_t num_tokens, hidden, inter, num_experts, top_k, renormalize;
+  int32_t dtype;                   /* hidden_states and out: bf16, fp16, fp32 */
+  int32_t global_num_experts;      /* entries of expert_map                   */
+  const void* hidden_states;       /* [M, H]                                  */
+  const float* router_logits;      /* [M, E] or NULL                          */
+  const float* topk_weights;       /* [M, k] when router_logits NULL          */
+  const int32_t* topk_ids;         /* [M, k] when router_logits NULL          */
+  const int32_t* expert_map;       /* optional, only with given ids           */
+  const int8_t* w13;
+  const float* w13_scale;
+  const int8_t* w2;
+  const float* w2_scale;
+  void* out;                       /* [M, H]                                  */
+  int32_t* status;                 /* as MtpInt8MatmulArgs                    */
+  void* workspace;
+  int64_t workspace_bytes;
+} MtpW8A8LayerArgs;
+MTP_API int mtp_w8a8_moe_layer_workspace_size(const MtpW8A8LayerArgs* args, int64_t* bytes);
+MTP_API int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream);
+
 /* ---- MTP expert-demand predictor (prefetch driver) --------------------------
  * logits = W2 . silu(W1 . h + b1) + b2 for each hidden state h [M, hidden]
  * bf16: hidden -> width -> future x experts, then the top_k experts of every

@@ -24,6 +24,16 @@ from .ops import (  # noqa: F401
     topk_softmax,
     vllm_wna16_to_gptq,
 )
+from .w8a8 import (  # noqa: F401
+    SortedTokens,
+    int8_grouped_matmul,
+    int8_linear,
+    int8_matmul,
+    moe_layer_w8a8,
+    quantize_int8,
+    sort_tokens,
+    unsort_tokens,
+)
 
 __all__ = [
     "ExpertParallelMoE",
@@ -33,16 +43,24 @@ __all__ = [
     "PrefetchSession",
     "load_library",
     "SharedExpert",
+    "SortedTokens",
     "W4A16Experts",
     "dequantize_gptq_projection",
     "experts_from_vllm_wna16",
     "fused_experts",
+    "int8_grouped_matmul",
+    "int8_linear",
+    "int8_matmul",
     "layer_path",
     "layer_workspace",
     "moe_align_block_size",
     "moe_layer_w4a16",
+    "moe_layer_w8a8",
     "plan_dispatch",
     "prefill_workspace",
+    "quantize_int8",
+    "sort_tokens",
     "topk_softmax",
+    "unsort_tokens",
     "vllm_wna16_to_gptq",
 ]

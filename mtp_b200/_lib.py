@@ -31,6 +31,14 @@ EXPORTS = (
     "mtp_w4a16_moe_prefill_workspace_size",
     "mtp_w4a16_moe_prefill",
     "mtp_w4a16_moe_prefill_tables",
+    "mtp_sort_tokens",
+    "mtp_unsort_tokens",
+    "mtp_unsort_tokens_backward",
+    "mtp_quantize_int8",
+    "mtp_int8_matmul_workspace_size",
+    "mtp_int8_matmul",
+    "mtp_w8a8_moe_layer_workspace_size",
+    "mtp_w8a8_moe_layer",
     "mtp_predictor_pack",
     "mtp_predictor_workspace_size",
     "mtp_predict_topk",
@@ -78,6 +86,21 @@ class MtpPrefillTables(C.Structure):
                 ("pairs_per_token", i32), ("block_size", i32)]
 
 
+class MtpInt8MatmulArgs(C.Structure):
+    _fields_ = [("rows", i32), ("n", i32), ("k", i32), ("num_groups", i32),
+                ("a_dtype", i32), ("out_dtype", i32), ("activation", i32), ("reserved", i32),
+                ("a", vp), ("a_stride", i64), ("a_scale", vp), ("b", vp), ("b_scale", vp), ("bias", vp),
+                ("offsets", vp), ("out", vp), ("status", vp), ("workspace", vp), ("workspace_bytes", i64)]
+
+
+class MtpW8A8LayerArgs(C.Structure):
+    _fields_ = [("num_tokens", i32), ("hidden", i32), ("inter", i32), ("num_experts", i32), ("top_k", i32),
+                ("renormalize", i32), ("dtype", i32), ("global_num_experts", i32),
+                ("hidden_states", vp), ("router_logits", vp), ("topk_weights", vp), ("topk_ids", vp),
+                ("expert_map", vp), ("w13", vp), ("w13_scale", vp), ("w2", vp), ("w2_scale", vp), ("out", vp),
+                ("status", vp), ("workspace", vp), ("workspace_bytes", i64)]
+
+
 class MtpPrefetchConfig(C.Structure):
     _fields_ = [("device", i32), ("num_layers", i32), ("num_experts", i32), ("slots_per_layer", i32),
                 ("expert_bytes", i64), ("host_store", vp), ("cache_base", vp), ("slot_tables", vp),
@@ -110,6 +133,14 @@ _SIGS = {
     "mtp_w4a16_moe_prefill_tables": (C.c_int, [i32, i32, i32, i32, i32, i32, C.POINTER(MtpPrefillTables)]),
     "mtp_w4a16_moe_prefill_workspace_size": (C.c_int, [i32, i32, i32, i32, i32, C.POINTER(i64)]),
     "mtp_w4a16_moe_prefill": (C.c_int, [C.POINTER(MtpMoeLayerArgs), vp]),
+    "mtp_sort_tokens": (C.c_int, [vp, i64, i32, i32, i32, vp, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]),
+    "mtp_unsort_tokens": (C.c_int, [vp, i64, i32, vp, vp, i32, i32, i32, vp, vp]),
+    "mtp_unsort_tokens_backward": (C.c_int, [vp, vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp]),
+    "mtp_quantize_int8": (C.c_int, [vp, i64, i32, i32, i32, vp, i64, vp, vp]),
+    "mtp_int8_matmul_workspace_size": (C.c_int, [C.POINTER(MtpInt8MatmulArgs), C.POINTER(i64)]),
+    "mtp_int8_matmul": (C.c_int, [C.POINTER(MtpInt8MatmulArgs), vp]),
+    "mtp_w8a8_moe_layer_workspace_size": (C.c_int, [C.POINTER(MtpW8A8LayerArgs), C.POINTER(i64)]),
+    "mtp_w8a8_moe_layer": (C.c_int, [C.POINTER(MtpW8A8LayerArgs), vp]),
     "mtp_predictor_pack": (C.c_int, [vp, i32, i32, vp, vp]),
     "mtp_predictor_workspace_size": (C.c_int, [i32, i32, i32, i32, C.POINTER(i64)]),
     "mtp_predict_topk": (C.c_int, [vp, i32, i32, vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, vp, i64, vp]),

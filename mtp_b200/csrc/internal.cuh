@@ -133,4 +133,52 @@ struct PrefillWs {
 PrefillWs prefill_ws(int M, int E, int k, int H, int I, int has_shared);
 int launch_moe_prefill(PrefillArgs& a, int renorm, const float* logits, cudaStream_t st);
 
+// Token sort and unsort (token_sort.cu). Strides and row sizes in bytes.
+struct SortArgs {
+  int M, k, E, E_map, numel;
+  int64_t x_stride, row_bytes;  // row_bytes 0: positions and offsets only
+  const uint8_t* x;
+  const int32_t* ids;          // [M, k]
+  const int32_t* emap;         // [E_map] or NULL
+  const float* row_scales;     // [M] or NULL
+  uint8_t* rows;               // [M * k] rows
+  float* sorted_scales;        // [M * k] with row_scales
+  int32_t* positions;          // [M, k]
+  int32_t* offsets;            // [E + 1]
+};
+struct UnsortArgs {
+  int M, k, H;
+  int64_t num_rows;
+  const void* rows;            // [num_rows, H]
+  const int32_t* positions;    // [M, k]
+  const float* weights;        // [M, k] or NULL (= 1)
+  void* out;                   // forward: [M, H]
+  const void* grad;            // backward: [M, H]
+  void* grad_rows;             // [num_rows, H] or NULL
+  float* grad_weights;         // [M, k] or NULL
+};
+int launch_sort_tokens(const SortArgs& a, cudaStream_t st);
+int launch_unsort_tokens(const UnsortArgs& a, int dtype, bool backward, cudaStream_t st);
+
+// Rows to int8 (quantize.cu); strides in elements.
+int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
+                         float* scale, cudaStream_t st);
+
+// int8 products (int8_matmul.cu).
+struct Int8Args {
+  int P, N, K, E;              // rows, rows of b per group, K, groups
+  int ctiles;                  // channel tiles (set by the launcher)
+  const float* a_scale;        // [P]
+  const float* b_scale;        // [E, N]
+  const float* bias;           // [N] or NULL
+  const int32_t* offsets;      // [E + 1] or NULL (one group of all rows)
+  void* out;                   // [P, N] or, gated, [P, N / 2]
+  int32_t* status;             // [1] or NULL: bit 0 set when a wait ran out
+};
+bool tma_rows_ok(const void* base, int64_t stride);
+int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* dst, int64_t dst_stride,
+                    cudaStream_t st);
+int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, const void* bp,
+                       int64_t b_stride, cudaStream_t st);
+
 }  // namespace mtp

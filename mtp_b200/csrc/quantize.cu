@@ -1,0 +1,181 @@
+// Rows quantised to int8 with one scale each:
+//   scale = max|x| / 127,  q = round(x * (127 / max|x|)), half to even.
+// The codes are exactly what these fp32 operations give (one division per
+// row, one product per element). A row of zeros has scale 0 and codes 0. A
+// row with an infinity or a NaN has that as its scale and codes 0, so every
+// product with it is NaN rather than a number. Rows below 2^-64 are scaled by
+// 2^64 first, where 127 / max|x| would overflow.
+//
+// HBM-bound: a row is read once into registers (up to kUnits units of 8
+// elements per thread), its maximum is a warp or CTA reduction, and the codes
+// are written 8 bytes at a time. Longer rows read the rest a second time.
+#include "internal.cuh"
+
+#include <algorithm>
+
+namespace mtp {
+namespace {
+
+constexpr int kUnits = 8;
+
+__device__ __forceinline__ void unpack(const __nv_bfloat16* p, float* v) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const __half* p, float* v) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const float* p, float* v) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float one(const float* p) { return *p; }
+
+// Elements c .. c + 7 of a row of K (zeros past it).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_unit(const T* row, int c, int K, float* v) {
+  if (WIDE) {
+    unpack(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? one(row + c + i) : 0.f;
+  }
+}
+
+// |x| as an integer orders like |x|, infinities above all numbers and NaNs
+// above them.
+__device__ __forceinline__ uint32_t magnitude(const float* v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+struct RowScale {
+  float factor;  // 127 / max, 0 for a row of zeros or with an infinity or NaN
+  float pre;     // 2^64 for tiny rows
+};
+
+__device__ __forceinline__ RowScale row_scale(uint32_t most) {
+  RowScale r;
+  const float m = __uint_as_float(most);
+  r.pre = m < 0x1p-64f ? 0x1p64f : 1.f;
+  r.factor = most == 0 || most >= 0x7f800000u ? 0.f : __fdiv_rn(127.f, m * r.pre);
+  return r;
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void store_unit(int8_t* q, int c, int K, const float* v, RowScale r) {
+  uint32_t w[2] = {0, 0};
+  if (r.factor != 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = r.pre == 1.f ? v[i] : v[i] * r.pre;
+      const int code = __float2int_rn(__fmul_rn(x, r.factor));
+      w[i >> 2] |= (static_cast<uint32_t>(code) & 0xffu) << (8 * (i & 3));
+    }
+  }
+  if (WIDE) {
+    *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
+  } else {
+    for (int i = 0; i < 8 && c + i < K; ++i) q[c + i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// A row per warp (CTA false) or per CTA of 256 threads.
+template <typename T, bool WIDE, bool CTA>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t x_stride, int M, int K,
+                                                       int8_t* __restrict__ q, int64_t q_stride,
+                                                       float* __restrict__ scale) {
+  __shared__ uint32_t red[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t m = CTA ? static_cast<int64_t>(blockIdx.x) : static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  if (m >= M) return;
+  const int first = (CTA ? threadIdx.x : lane) * 8;
+  constexpr int kStep = (CTA ? 256 : 32) * 8;
+  const T* row = x + m * x_stride;
+  int8_t* out = q + m * q_stride;
+  float v[kUnits][8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u)
+    if (first + u * kStep < K) load_unit<T, WIDE>(row, first + u * kStep, K, v[u]);
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u)
+    if (first + u * kStep < K) most = max(most, magnitude(v[u]));
+  for (int c = first + kUnits * kStep; c < K; c += kStep) {
+    float t[8];
+    load_unit<T, WIDE>(row, c, K, t);
+    most = max(most, magnitude(t));
+  }
+  most = __reduce_max_sync(kFullMask, most);
+  if (CTA) {
+    if (lane == 0) red[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) most = max(most, red[w]);
+  }
+  const RowScale r = row_scale(most);
+  if (first == 0) scale[m] = __fdiv_rn(__uint_as_float(most), 127.f);
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u)
+    if (first + u * kStep < K) store_unit<WIDE>(out, first + u * kStep, K, v[u], r);
+  for (int c = first + kUnits * kStep; c < K; c += kStep) {
+    float t[8];
+    load_unit<T, WIDE>(row, c, K, t);
+    store_unit<WIDE>(out, c, K, t, r);
+  }
+}
+
+template <typename T>
+int run(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale, cudaStream_t st) {
+  const bool wide = aligned(x, 16) && x_stride * sizeof(T) % 16 == 0 && K % 8 == 0 && aligned(q, 8) && q_stride % 8 == 0;
+  // A warp per row where the row fits its registers and there are rows for
+  // every warp; a CTA per row where rows are long or few.
+  const bool cta = K > kUnits * 32 * 8 || M < 148 * 8;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cta ? M : (M + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto* kernel = wide ? (cta ? quantize_kernel<T, true, true> : quantize_kernel<T, true, false>)
+                      : (cta ? quantize_kernel<T, false, true> : quantize_kernel<T, false, false>);
+  if (cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(x), x_stride, M, K, q, q_stride, scale) != cudaSuccess) {
+    cudaGetLastError();
+    return MTP_ERR_LAUNCH;
+  }
+  return MTP_OK;
+}
+
+}  // namespace
+
+int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
+                         float* scale, cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return run<__nv_bfloat16>(x, x_stride, M, K, q, q_stride, scale, st);
+    case MTP_DTYPE_FP16: return run<__half>(x, x_stride, M, K, q, q_stride, scale, st);
+    default: return run<float>(x, x_stride, M, K, q, q_stride, scale, st);
+  }
+}
+
+}  // namespace mtp

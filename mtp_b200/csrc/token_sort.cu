@@ -1,0 +1,436 @@
+// Tokens sorted by expert, and back with the routing weights applied.
+//
+// sort:    the pairs (t, j) of a token and its j-th choice get the key
+//          expert_map[topk_ids[t, j]] (or the id itself), E where that is no
+//          expert of this rank. Row p(t, j) = #{pairs of a smaller key} +
+//          #{earlier pairs of the same key}: a stable sort, so the result
+//          does not depend on scheduling. rows[p(t, j)] = x[t]; pairs without
+//          an expert come last and their rows are zero. positions holds p,
+//          or ~p (negative) for a pair without an expert, so every pair knows
+//          the one row that is its own. offsets[e] = #{pairs of a key < e}.
+// unsort:  out[t] = sum over the routed j, ascending, of w[t, j] * rows[p(t, j)]
+//          (w = 1 without weights: the gradient of the sort), in fp32, rounded
+//          once.
+// its gradient: grad_rows[p(t, j)] = w[t, j] * g[t], zero rows for unrouted
+//          pairs, grad_w[t, j] = <g[t], rows[p(t, j)]> in fp32.
+//
+// All three move rows and are bound by HBM; the ranking is integer counting.
+#include "internal.cuh"
+#include "route.cuh"
+
+#include <algorithm>
+
+namespace mtp {
+namespace {
+
+constexpr int kRankCtas = 8;        // one cluster ranks all pairs of a large call
+constexpr int kRankThreads = 1024;
+constexpr int kRankWarps = kRankThreads / 32;
+// Up to this many pairs every CTA of the copy ranks its own token's pairs by
+// counting over all keys in shared memory (one launch); above, a cluster ranks
+// all pairs first.
+constexpr int kSmallPairs = 4096;
+constexpr int kSmallThreads = 256;
+
+__device__ __forceinline__ int sort_key(const SortArgs& a, int i) {
+  int id = a.ids[i];
+  if (a.emap) id = id >= 0 && id < a.E_map ? a.emap[id] : -1;
+  return id >= 0 && id < a.E ? id : a.E;
+}
+
+template <typename V>
+__device__ __forceinline__ V zero_of() {
+  V v;
+  memset(&v, 0, sizeof(V));
+  return v;
+}
+
+// Row t of x to its k rows (zeros where the position is negative). `lane` of
+// `lanes` threads take the row's vectors in turn.
+template <typename V>
+__device__ __forceinline__ void copy_row(const SortArgs& a, int t, const int* pos, int lane, int lanes) {
+  const V* src = reinterpret_cast<const V*>(a.x + static_cast<int64_t>(t) * a.x_stride);
+  const int n = static_cast<int>(a.row_bytes / sizeof(V));
+  for (int c = lane; c < n; c += lanes) {
+    const V v = src[c];
+    for (int j = 0; j < a.k; ++j) {
+      const int p = pos[j];
+      V* dst = reinterpret_cast<V*>(a.rows + static_cast<int64_t>(p >= 0 ? p : ~p) * a.row_bytes);
+      dst[c] = p >= 0 ? v : zero_of<V>();
+    }
+  }
+  if (a.row_scales)
+    for (int j = lane; j < a.k; j += lanes) {
+      const int p = pos[j];
+      a.sorted_scales[p >= 0 ? p : ~p] = p >= 0 ? a.row_scales[t] : 0.f;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// one launch: CTA t ranks the pairs of token t and copies its row
+// ---------------------------------------------------------------------------
+template <typename V>
+__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArgs a) {
+  extern __shared__ int keys[];  // [numel], then the token's k positions
+  int* pos = keys + a.numel;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int i = tid; i < a.numel; i += blockDim.x) keys[i] = sort_key(a, i);
+  __syncthreads();
+  const int t = blockIdx.x;
+  if (t < a.M) {
+    for (int j = warp; j < a.k; j += warps) {
+      const int i = t * a.k + j, key = keys[i];
+      int before = 0;
+      for (int q = lane; q < a.numel; q += 32) {
+        const int kq = keys[q];
+        before += kq < key || (kq == key && q < i) ? 1 : 0;
+      }
+      before = __reduce_add_sync(kFullMask, before);
+      if (lane == 0) {
+        const int p = key < a.E ? before : ~before;
+        pos[j] = p;
+        a.positions[i] = p;
+      }
+    }
+  }
+  // offsets: entry e belongs to CTA e % gridDim; a thread each where the CTA
+  // has many, a warp each where it has few
+  const int mine = (a.E + 1 - t + gridDim.x - 1) / static_cast<int>(gridDim.x);
+  if (mine > 2 * warps || a.numel <= 64) {
+    for (int e = t + tid * gridDim.x; e <= a.E; e += blockDim.x * gridDim.x) {
+      int before = 0;
+      for (int q = 0; q < a.numel; ++q) before += keys[q] < e ? 1 : 0;
+      a.offsets[e] = before;
+    }
+  } else {
+    for (int e = t + warp * gridDim.x; e <= a.E; e += warps * gridDim.x) {
+      int before = 0;
+      for (int q = lane; q < a.numel; q += 32) before += keys[q] < e ? 1 : 0;
+      before = __reduce_add_sync(kFullMask, before);
+      if (lane == 0) a.offsets[e] = before;
+    }
+  }
+  __syncthreads();
+  if (t < a.M) copy_row<V>(a, t, pos, tid, blockDim.x);
+}
+
+// ---------------------------------------------------------------------------
+// large calls: ranks from one cluster, then the copy
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t local, int cta) {
+  uint32_t remote;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(cta));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+inline size_t rank_smem(int E) { return static_cast<size_t>(kRankWarps + 2) * (E + 1) * sizeof(int); }
+
+// Every warp of the cluster takes one contiguous range of the pairs and walks
+// it twice: first it counts its pairs of every key, then, with the counts of
+// the ranges before its own summed (over the warps of the CTA in shared memory,
+// over the CTAs through distributed shared memory), it numbers them.
+__global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads, 1) sort_rank_kernel(const SortArgs a) {
+  extern __shared__ int sm[];
+  __shared__ int scan_tmp[32];
+  const int bins = a.E + 1;
+  int* wcnt = sm;                       // [warps][bins]
+  int* tot = sm + kRankWarps * bins;    // [bins] this CTA's pairs of every key
+  int* base = tot + bins;               // [bins] first row of this CTA's pairs of a key
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
+  for (int x = tid; x < kRankWarps * bins; x += kRankThreads) wcnt[x] = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  const int64_t parts = kRankCtas * kRankWarps;
+  const int64_t span = (a.numel + parts * 32 - 1) / (parts * 32) * 32;
+  const int64_t begin = (static_cast<int64_t>(cta) * kRankWarps + warp) * span;
+  const int64_t end = min(begin + span, static_cast<int64_t>(a.numel));
+  int* mine = wcnt + warp * bins;
+  for (int64_t c = begin; c < end; c += 32) {
+    const int64_t i = c + lane;
+    const int key = i < end ? sort_key(a, static_cast<int>(i)) : -1;
+    const unsigned same = __match_any_sync(kFullMask, key);
+    if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int b = tid; b < bins; b += kRankThreads) {
+    int run = 0;
+    for (int w = 0; w < kRankWarps; ++w) {
+      const int v = wcnt[w * bins + b];
+      wcnt[w * bins + b] = run;
+      run += v;
+    }
+    tot[b] = run;
+  }
+  cluster_sync_all();
+  int all = 0, before = 0;
+  if (tid < a.E)
+    for (int r = 0; r < kRankCtas; ++r) {
+      const int v = ld_cluster(smem_u32(tot + tid), r);
+      before += r < cta ? v : 0;
+      all += v;
+    }
+  int routed;
+  const int off = block_exclusive_scan(all, &routed, scan_tmp);
+  if (tid < a.E) {
+    base[tid] = off + before;
+    if (cta == 0) a.offsets[tid] = off;
+  }
+  if (tid == 0) {
+    if (cta == 0) a.offsets[a.E] = routed;
+    int unrouted = 0;
+    for (int r = 0; r < cta; ++r) unrouted += ld_cluster(smem_u32(tot + a.E), r);
+    base[a.E] = routed + unrouted;
+  }
+  cluster_sync_all();  // also: no CTA leaves while another reads its counts
+  for (int64_t c = begin; c < end; c += 32) {
+    const int64_t i = c + lane;
+    const int key = i < end ? sort_key(a, static_cast<int>(i)) : -1;
+    const unsigned same = __match_any_sync(kFullMask, key);
+    int p = 0;
+    if (key >= 0) p = base[key] + mine[key] + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (key >= 0) {
+      a.positions[i] = key < a.E ? p : ~p;
+      if (lane == __ffs(same) - 1) mine[key] += __popc(same);
+    }
+    __syncwarp();
+  }
+}
+
+// blockDim (lanes of a row, tokens of a CTA)
+template <typename V>
+__global__ void __launch_bounds__(256) sort_copy_kernel(const SortArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= a.M) return;
+  copy_row<V>(a, static_cast<int>(t), a.positions + t * a.k, threadIdx.x, blockDim.x);
+}
+
+// ---------------------------------------------------------------------------
+// unsort
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+constexpr int kSlots = 8;  // slots whose rows a thread has in flight together
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
+  using V = Vec<T, N>;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= a.M) return;
+  const int32_t* pos = a.positions + t * a.k;
+  const float* wt = a.weights ? a.weights + t * a.k : nullptr;
+  const T* rows = static_cast<const T*>(a.rows);
+  T* out = static_cast<T*>(a.out) + t * a.H;
+  for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
+    float acc[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] = 0.f;
+    for (int j0 = 0; j0 < a.k; j0 += kSlots) {
+      V v[kSlots];
+      float w[kSlots];
+      bool here[kSlots];
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        const int p = j0 + j < a.k ? pos[j0 + j] : -1;
+        here[j] = p >= 0 && p < a.num_rows;
+        w[j] = here[j] && wt ? wt[j0 + j] : 1.f;
+        if (here[j]) v[j] = *reinterpret_cast<const V*>(rows + static_cast<int64_t>(p) * a.H + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j)
+        if (here[j])
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[n] = fmaf(w[j], to_f<T>(v[j].v[n]), acc[n]);
+    }
+    V o;
+#pragma unroll
+    for (int n = 0; n < N; ++n) o.v[n] = from_f<T>(acc[n]);
+    *reinterpret_cast<V*>(out + c) = o;
+  }
+}
+
+// blockDim.x is a multiple of 32: the lanes of a token are whole warps.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) unsort_backward_kernel(const UnsortArgs a) {
+  using V = Vec<T, N>;
+  __shared__ float red[8][kSlots];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const bool in = t < a.M;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t* pos = a.positions + t * a.k;
+  const float* wt = a.weights ? a.weights + t * a.k : nullptr;
+  const T* g = static_cast<const T*>(a.grad) + t * a.H;
+  const T* rows = static_cast<const T*>(a.rows);
+  T* grows = static_cast<T*>(a.grad_rows);
+  for (int j0 = 0; j0 < a.k; j0 += kSlots) {
+    float dot[kSlots], w[kSlots];
+    int p[kSlots];
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      dot[j] = 0.f;
+      const bool slot = in && j0 + j < a.k;
+      p[j] = slot ? pos[j0 + j] : INT_MIN;  // ~INT_MIN is past every row
+      w[j] = slot && wt && p[j] >= 0 ? wt[j0 + j] : 1.f;
+    }
+    if (in)
+      for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
+        const V gv = *reinterpret_cast<const V*>(g + c);
+        V v[kSlots];
+        if (a.grad_weights) {
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j)
+            if (p[j] >= 0 && p[j] < a.num_rows)
+              v[j] = *reinterpret_cast<const V*>(rows + static_cast<int64_t>(p[j]) * a.H + c);
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j)
+            if (p[j] >= 0 && p[j] < a.num_rows)
+#pragma unroll
+              for (int n = 0; n < N; ++n) dot[j] = fmaf(to_f<T>(gv.v[n]), to_f<T>(v[j].v[n]), dot[j]);
+        }
+        if (grows)
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            const int r = p[j] >= 0 ? p[j] : ~p[j];
+            if (r >= a.num_rows) continue;
+            V o;
+#pragma unroll
+            for (int n = 0; n < N; ++n) o.v[n] = from_f<T>(p[j] >= 0 ? w[j] * to_f<T>(gv.v[n]) : 0.f);
+            *reinterpret_cast<V*>(grows + static_cast<int64_t>(r) * a.H + c) = o;
+          }
+      }
+    if (a.grad_weights) {
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) dot[j] = warp_sum(dot[j]);
+      if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) red[threadIdx.y * warps + warp][j] = dot[j];
+      __syncthreads();
+      if (in && threadIdx.x < kSlots && j0 + static_cast<int>(threadIdx.x) < a.k) {
+        float s = 0.f;
+        for (int x = 0; x < warps; ++x) s += red[threadIdx.y * warps + x][threadIdx.x];
+        a.grad_weights[t * a.k + j0 + threadIdx.x] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Threads of a row (a power of two in [least, 256]) and rows of a CTA.
+dim3 row_block(int64_t vectors, int least) {
+  int x = least;
+  while (x < vectors && x < 256) x *= 2;
+  return dim3(x, 256 / x);
+}
+
+template <typename F, typename... A>
+int launch(F* kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return MTP_ERR_LAUNCH;
+  }
+  return MTP_OK;
+}
+
+template <typename V>
+int sort_run(const SortArgs& a, cudaStream_t st) {
+  if (a.numel <= kSmallPairs)
+    return launch(sort_small_kernel<V>, dim3(std::max(a.M, 1)), dim3(kSmallThreads),
+                  static_cast<size_t>(a.numel + a.k) * sizeof(int), st, a);
+  static int configured_device = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
+  if (configured_device != dev) {
+    if (cudaFuncSetAttribute(sort_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(rank_smem(1024))) != cudaSuccess)
+      return MTP_ERR_CUDA;
+    configured_device = dev;
+  }
+  const int rc = launch(sort_rank_kernel, dim3(kRankCtas), dim3(kRankThreads), rank_smem(a.E), st, a);
+  if (rc != MTP_OK) return rc;
+  const dim3 block = row_block(a.row_bytes / static_cast<int64_t>(sizeof(V)), 8);
+  return launch(sort_copy_kernel<V>, dim3((a.M + block.y - 1) / block.y), block, 0, st, a);
+}
+
+template <typename T>
+int unsort_run(const UnsortArgs& a, bool backward, cudaStream_t st) {
+  // the widest vector that every row start and length allows
+  constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.out) |
+                         reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.grad_rows) |
+                         static_cast<uintptr_t>(static_cast<int64_t>(a.H) * sizeof(T));
+  const int n = (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
+  const dim3 block = row_block((a.H + n - 1) / n, backward ? 32 : 8);
+  const dim3 grid((a.M + block.y - 1) / block.y);
+  auto pick = [&](auto* wide, auto* pair, auto* one) { return n == kWide ? wide : n == kPair ? pair : one; };
+  if (backward)
+    return launch(pick(unsort_backward_kernel<T, kWide>, unsort_backward_kernel<T, kPair>, unsort_backward_kernel<T, 1>),
+                  grid, block, 0, st, a);
+  return launch(pick(unsort_kernel<T, kWide>, unsort_kernel<T, kPair>, unsort_kernel<T, 1>), grid, block, 0, st, a);
+}
+
+}  // namespace
+
+int launch_sort_tokens(const SortArgs& a, cudaStream_t st) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.rows) |
+                         static_cast<uintptr_t>(a.row_bytes) | static_cast<uintptr_t>(a.x_stride);
+  if ((bits & 15) == 0) return sort_run<uint4>(a, st);
+  if ((bits & 7) == 0) return sort_run<uint2>(a, st);
+  if ((bits & 3) == 0) return sort_run<uint32_t>(a, st);
+  if ((bits & 1) == 0) return sort_run<uint16_t>(a, st);
+  return sort_run<uint8_t>(a, st);
+}
+
+int launch_unsort_tokens(const UnsortArgs& a, int dtype, bool backward, cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return unsort_run<__nv_bfloat16>(a, backward, st);
+    case MTP_DTYPE_FP16: return unsort_run<__half>(a, backward, st);
+    default: return unsort_run<float>(a, backward, st);
+  }
+}
+
+}  // namespace mtp

@@ -1,0 +1,433 @@
+"""The int8 (W8A8) expert path and the token sort around it: torch tensors in,
+C-ABI calls out.
+
+* :func:`sort_tokens` / :func:`unsort_tokens` - token rows into expert order and
+  back with the routing weights applied; both have gradients
+  (``torch.autograd``);
+* :func:`quantize_int8` - rows to int8 codes with one scale each;
+* :func:`int8_matmul` / :func:`int8_linear` - int8 rows (or rows quantised on the
+  way in) times int8 weights with one scale per output channel;
+* :func:`int8_grouped_matmul` - the same with one weight matrix per group of
+  sorted rows, optionally with SiLU(gate) * up;
+* :func:`moe_layer_w8a8` - router, sort, both expert products and the way back.
+
+Pair order, ``-1`` ids and ``expert_map`` follow :func:`mtp_b200.moe_align_block_size`
+and :func:`mtp_b200.moe_layer_w4a16`. Shape, dtype and device errors raise
+``ValueError`` before any launch; a non-zero C status raises
+:class:`mtp_b200.MtpError`. Every call is asynchronous on the current torch
+CUDA stream. There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from functools import lru_cache
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MtpDtype
+_INT8 = 3
+MAX_K = 131071  # 128 * 128 * K stays below 2^31
+_SILU_MUL = 1
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None, contiguous: bool = True):
+    """``t`` is a CUDA tensor of one of ``dtypes`` and ``ndim`` dimensions on ``device``."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor, got device {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"{name} must be {ndim}-D, got shape {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
+_I8 = (torch.int8,)
+_ROWS = (torch.bfloat16, torch.float16, torch.float32, torch.int8)
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _row_stride(name: str, t: torch.Tensor) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are contiguous and do not overlap."""
+    if t.shape[0] <= 1:
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"the rows of {name} must be contiguous")
+        return t.shape[1]
+    if (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
+        raise ValueError(f"the rows of {name} must be contiguous and must not overlap, got strides {t.stride()}")
+    return t.stride(0)
+
+
+# ---------------------------------------------------------------------------
+# sort and unsort
+# ---------------------------------------------------------------------------
+class SortedTokens(NamedTuple):
+    """What :func:`sort_tokens` returns.
+
+    ``rows`` [M*k, H] in expert order (pairs without an expert last, as zeros),
+    ``positions`` [M, k] int32 (the pair's row, or ``~row`` < 0 without an
+    expert), ``offsets`` [E + 1] int32 (first row of each expert, then the
+    number of routed rows), ``row_scales`` [M*k] fp32 if scales were given."""
+
+    rows: torch.Tensor
+    positions: torch.Tensor
+    offsets: torch.Tensor
+    row_scales: torch.Tensor | None
+
+
+def _sort(x, ids, num_experts, expert_map, row_scales):
+    m, k = ids.shape
+    dev, h = x.device, x.shape[1]
+    rows = torch.empty((m * k, h), dtype=x.dtype, device=dev)
+    positions = torch.empty((m, k), dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    scales = None if row_scales is None else torch.empty(m * k, dtype=torch.float32, device=dev)
+    _lib.call("mtp_sort_tokens", x.data_ptr() or None, _row_stride("hidden_states", x), DTYPES.get(x.dtype, _INT8), m, h,
+              ids.data_ptr(), k, num_experts, None if expert_map is None else expert_map.data_ptr(),
+              0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
+              rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(),
+              offsets.data_ptr(), _stream(dev))
+    return rows, positions, offsets, scales
+
+
+def _unsort(rows, positions, weights):
+    m, k = positions.shape
+    out = torch.empty((m, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    _lib.call("mtp_unsort_tokens", rows.data_ptr(), rows.shape[0], DTYPES[rows.dtype], positions.data_ptr(),
+              None if weights is None else weights.data_ptr(), m, k, rows.shape[1], out.data_ptr(),
+              _stream(rows.device))
+    return out
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ids, num_experts, expert_map, row_scales):
+        rows, positions, offsets, scales = _sort(x, ids, num_experts, expert_map, row_scales)
+        ctx.save_for_backward(positions)
+        ctx.mark_non_differentiable(positions, offsets, *([] if scales is None else [scales]))
+        return rows, positions, offsets, scales
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_rows, *_):
+        (positions,) = ctx.saved_tensors
+        return _unsort(grad_rows.contiguous(), positions, None), None, None, None, None
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, positions, weights):
+        ctx.save_for_backward(rows if weights is not None and weights.requires_grad else None, positions, weights)
+        ctx.num_rows = rows.shape[0]
+        return _unsort(rows, positions, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        rows, positions, weights = ctx.saved_tensors
+        grad = grad.contiguous()
+        (m, k), h = positions.shape, grad.shape[1]
+        need_rows, _, need_weights = ctx.needs_input_grad
+        grad_rows = torch.empty((ctx.num_rows, h), dtype=grad.dtype, device=grad.device) if need_rows else None
+        grad_weights = torch.empty_like(weights) if need_weights else None
+        _lib.call("mtp_unsort_tokens_backward", grad.data_ptr(), None if rows is None else rows.data_ptr(),
+                  ctx.num_rows, DTYPES[grad.dtype], positions.data_ptr(),
+                  None if weights is None else weights.data_ptr(), m, k, h,
+                  None if grad_rows is None else grad_rows.data_ptr(),
+                  None if grad_weights is None else grad_weights.data_ptr(), _stream(grad.device))
+        return grad_rows, None, grad_weights
+
+
+def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *,
+                expert_map: torch.Tensor | None = None, row_scales: torch.Tensor | None = None) -> SortedTokens:
+    """The rows of ``hidden_states`` [M, H] (bf16, fp16, fp32 or int8) in expert
+    order, one per pair of a token and one of its ``topk_ids`` [M, k] int32.
+
+    The order is stable (experts ascending, ``t*k + j`` ascending inside an
+    expert). Ids outside [0, ``num_experts``) - after ``expert_map`` [global E]
+    int32, if given - have no expert here: their rows come last, as zeros.
+    ``row_scales`` [M] fp32 (the scales of int8 rows) are sorted along. The
+    gradient of ``hidden_states`` sums the gradients of a token's routed rows
+    in fp32."""
+    _tensor("hidden_states", hidden_states, 2, _ROWS, contiguous=False)
+    dev = hidden_states.device
+    _tensor("topk_ids", topk_ids, 2, _I32, dev)
+    m, k = topk_ids.shape
+    if m != hidden_states.shape[0]:
+        raise ValueError(f"topk_ids has {m} rows, hidden_states has {hidden_states.shape[0]}")
+    if not 1 <= k <= 32:
+        raise ValueError(f"topk_ids must have 1 to 32 columns, got {k}")
+    if not 1 <= num_experts <= 1024:
+        raise ValueError(f"num_experts must be in [1, 1024], got {num_experts}")
+    if m * k >= 2 ** 31 - 1:
+        raise ValueError(f"at most 2^31 - 2 pairs are supported, got {m * k}")
+    if expert_map is not None:
+        _tensor("expert_map", expert_map, 1, _I32, dev)
+        if not expert_map.numel():
+            raise ValueError("expert_map is empty")
+    if row_scales is not None:
+        _tensor("row_scales", row_scales, 1, _F32, dev)
+        if row_scales.numel() != m:
+            raise ValueError(f"row_scales must have {m} entries")
+    if hidden_states.requires_grad and torch.is_grad_enabled():
+        return SortedTokens(*_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales))
+    return SortedTokens(*_sort(hidden_states, topk_ids, num_experts, expert_map, row_scales))
+
+
+def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
+                  topk_weights: torch.Tensor | None = None) -> torch.Tensor:
+    """out [M, H] = the weighted sum of each token's routed ``rows`` [R, H] (bf16,
+    fp16 or fp32), in fp32 and rounded once. ``positions`` [M, k] int32 as
+    :func:`sort_tokens` gives them; ``topk_weights`` [M, k] fp32 (None: 1). A
+    token without routed pairs gets zeros. Gradients go to ``rows`` (zero for
+    rows of unrouted pairs) and ``topk_weights``."""
+    _tensor("rows", rows, 2, _FLOATS)
+    _tensor("positions", positions, 2, _I32, rows.device)
+    m, k = positions.shape
+    if not 1 <= k <= 32:
+        raise ValueError(f"positions must have 1 to 32 columns, got {k}")
+    if rows.shape[0] != m * k:
+        raise ValueError(f"rows must have one row per pair, {m * k}, got {rows.shape[0]}")
+    if topk_weights is not None:
+        _tensor("topk_weights", topk_weights, 2, _F32, rows.device)
+        if topk_weights.shape != positions.shape:
+            raise ValueError(f"topk_weights must be {(m, k)}, got {tuple(topk_weights.shape)}")
+    if torch.is_grad_enabled() and (rows.requires_grad or (topk_weights is not None and topk_weights.requires_grad)):
+        return _UnsortTokens.apply(rows, positions, topk_weights)
+    return _unsort(rows, positions, topk_weights)
+
+
+# ---------------------------------------------------------------------------
+# int8 products
+# ---------------------------------------------------------------------------
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes int8 [M, K], scales fp32 [M])`` of the rows of ``x`` [M, K] (bf16,
+    fp16 or fp32): scale = max|x| / 127, code = round(x * (127 / max|x|)), half
+    to even. A row of zeros has scale 0; a row with an infinity or a NaN has
+    that as its scale and codes 0. The codes' rows are a multiple of 16 bytes
+    apart, as the products read them best."""
+    _tensor("x", x, 2, _FLOATS, contiguous=False)
+    m, k = x.shape
+    if k < 1:
+        raise ValueError("x must have at least one column")
+    codes = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _lib.call("mtp_quantize_int8", x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(),
+              codes.shape[1], scale.data_ptr(), _stream(x.device))
+    return codes[:, :k], scale
+
+
+@lru_cache(maxsize=4096)
+def _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, a_off, b_off) -> int:
+    """Workspace bytes; a_off and b_off are the operands' addresses modulo 256 (their alignment)."""
+    args = _lib.MtpInt8MatmulArgs(rows, n, k, groups, a_dtype, 0, 0, 0, 256 + a_off, a_stride, None, 256 + b_off, None,
+                                  None, 256 if groups > 1 else None, None, None, None, 0)
+    out = _lib.i64()
+    _lib.call("mtp_int8_matmul_workspace_size", C.byref(args), C.byref(out))
+    return out.value
+
+
+def _product(a, a_scale, b, b_scale, bias, offsets, out_dtype, activation, status):
+    dev = a.device
+    rows, k = a.shape
+    n, groups = b.shape[-2], b.shape[0] if b.dim() == 3 else 1
+    out = torch.empty((rows, n // 2 if activation else n), dtype=out_dtype, device=dev)
+    a_dtype, a_stride = DTYPES.get(a.dtype, _INT8), _row_stride("a", a)
+    ap, bp = a.data_ptr(), b.data_ptr()
+    size = _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, ap & 255, bp & 255)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    args = _lib.MtpInt8MatmulArgs(rows, n, k, groups, a_dtype, DTYPES[out_dtype], activation, 0, ap, a_stride,
+                                  None if a_scale is None else a_scale.data_ptr(), bp, b_scale.data_ptr(),
+                                  None if bias is None else bias.data_ptr(),
+                                  None if offsets is None else offsets.data_ptr(), out.data_ptr(),
+                                  None if status is None else status.data_ptr(),
+                                  None if ws is None else ws.data_ptr(), size)
+    _lib.call("mtp_int8_matmul", C.byref(args), _stream(dev))
+    return out
+
+
+def _check_weight(name, b, scale, ndim, device, k):
+    _tensor(name, b, ndim, _I8, device)
+    _tensor(name + "_scale", scale, ndim - 1, _F32, device)
+    if b.shape[-1] != k:
+        raise ValueError(f"{name} must have {k} columns, got shape {tuple(b.shape)}")
+    if scale.shape != b.shape[:-1]:
+        raise ValueError(f"{name}_scale must be {tuple(b.shape[:-1])}, got {tuple(scale.shape)}")
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"1 to {MAX_K} columns are supported, got {k}")
+    if not b.shape[-2] or (ndim == 3 and not b.shape[0]):
+        raise ValueError(f"{name} must not be empty, got shape {tuple(b.shape)}")
+    if b.numel() // k >= 2 ** 31:
+        raise ValueError(f"{name} has 2^31 or more rows")
+
+
+def _check_bias(bias, n, device):
+    if bias is not None:
+        _tensor("bias", bias, 1, _F32, device)
+        if bias.numel() != n:
+            raise ValueError(f"bias must have {n} entries")
+
+
+def _check_out(out_dtype, status, device):
+    if out_dtype not in DTYPES:
+        raise ValueError(f"out_dtype must be one of {[str(d) for d in DTYPES]}, got {out_dtype}")
+    if status is not None:
+        _tensor("status", status, 1, _I32, device)
+        if not status.numel():
+            raise ValueError("status must have an entry")
+
+
+def _check_rows(a, a_scale):
+    _tensor("a", a, 2, _I8, contiguous=False)
+    _tensor("a_scale", a_scale, 1, _F32, a.device)
+    if a_scale.numel() != a.shape[0]:
+        raise ValueError(f"a_scale must have {a.shape[0]} entries, got {a_scale.numel()}")
+
+
+def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                status: torch.Tensor | None = None) -> torch.Tensor:
+    """``(a @ b.T) * a_scale[:, None] * b_scale (+ bias)`` for int8 ``a`` [M, K] and
+    ``b`` [N, K], fp32 scales per row and per output channel and fp32 ``bias``
+    [N]. The sum is exact in int32; the result is rounded once to ``out_dtype``.
+    ``status`` [1] int32 (zeroed by the caller) gets bit 0 if a bounded wait of
+    the kernel ran out, in which case the output is wrong."""
+    _check_rows(a, a_scale)
+    _check_weight("b", b, b_scale, 2, a.device, a.shape[1])
+    _check_bias(bias, b.shape[0], a.device)
+    _check_out(out_dtype, status, a.device)
+    return _product(a, a_scale, b, b_scale, bias, None, out_dtype, 0, status)
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, *, out_dtype: torch.dtype | None = None,
+                status: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`int8_matmul` of the rows of ``x`` [M, K] (bf16, fp16 or fp32)
+    quantised as :func:`quantize_int8` does, in one call; the result has the
+    type of ``x`` unless ``out_dtype`` is given."""
+    _tensor("x", x, 2, _FLOATS, contiguous=False)
+    _check_weight("weight", weight, weight_scale, 2, x.device, x.shape[1])
+    _check_bias(bias, weight.shape[0], x.device)
+    out_dtype = out_dtype or x.dtype
+    _check_out(out_dtype, status, x.device)
+    return _product(x, None, weight, weight_scale, bias, None, out_dtype, 0, status)
+
+
+def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                        offsets: torch.Tensor, *, out_dtype: torch.dtype = torch.bfloat16,
+                        activation: str | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows ``offsets[g] .. offsets[g + 1]`` of int8 ``a`` [P, K] times ``b[g]`` of
+    [G, N, K], scaled as in :func:`int8_matmul` by ``a_scale`` [P] and ``b_scale``
+    [G, N]. ``offsets`` [G + 1] int32 ascend from 0 (those of
+    :func:`sort_tokens`); rows behind ``offsets[G]`` are zeros.
+    ``activation="silu_mul"``: the first N / 2 channels are gates, and the
+    result [P, N / 2] is silu(gate) * up."""
+    _check_rows(a, a_scale)
+    _check_weight("b", b, b_scale, 3, a.device, a.shape[1])
+    _tensor("offsets", offsets, 1, _I32, a.device)
+    groups, n = b.shape[0], b.shape[1]
+    if groups > 1024:
+        raise ValueError(f"at most 1024 groups are supported, got {groups}")
+    if offsets.numel() != groups + 1:
+        raise ValueError(f"offsets must have {groups + 1} entries, got {offsets.numel()}")
+    if activation not in (None, "silu_mul"):
+        raise ValueError(f'activation must be None or "silu_mul", got {activation!r}')
+    if activation and n % 2:
+        raise ValueError(f"silu_mul needs an even number of channels, got {n}")
+    _check_out(out_dtype, status, a.device)
+    return _product(a, a_scale, b, b_scale, None, offsets, out_dtype, _SILU_MUL if activation else 0, status)
+
+
+# ---------------------------------------------------------------------------
+# the layer
+# ---------------------------------------------------------------------------
+@lru_cache(maxsize=4096)
+def _layer_workspace(m, h, i, e, k, dtype, logits, w13_off, w2_off) -> int:
+    args = _lib.MtpW8A8LayerArgs(m, h, i, e, k, 0, dtype, 0, None, 256 if logits else None, None, None, None,
+                                 256 + w13_off, None, 256 + w2_off, None, None, None, None, 0)
+    out = _lib.i64()
+    _lib.call("mtp_w8a8_moe_layer_workspace_size", C.byref(args), C.byref(out))
+    return out.value
+
+
+def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | None, w13: torch.Tensor,
+                   w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor, top_k: int,
+                   renormalize: bool = True, *, topk_weights: torch.Tensor | None = None,
+                   topk_ids: torch.Tensor | None = None, expert_map: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """One W8A8 MoE layer forward: router (when ``router_logits`` [M, E] fp32 is
+    given, else the given ``topk_weights`` fp32 / ``topk_ids`` int32 [M, k]),
+    rows quantised and sorted by expert, ``silu(gate) * up`` of the w13 product
+    in fp32, quantised per row, the w2 product, and the weighted sum per token.
+
+    ``hidden_states`` [M, H] bf16, fp16 or fp32; ``w13`` [E, 2I, H] int8 (gate
+    rows, then up rows) with ``w13_scale`` [E, 2I]; ``w2`` [E, H, I] int8 with
+    ``w2_scale`` [E, H]. Ids outside [0, E) - after ``expert_map``, which takes
+    global ids to local ones - contribute nothing. Returns ``out`` [M, H] in
+    the type of ``hidden_states``. ``status`` as in :func:`int8_matmul`."""
+    _tensor("hidden_states", hidden_states, 2, _FLOATS)
+    dev = hidden_states.device
+    m, h = hidden_states.shape
+    _check_weight("w13", w13, w13_scale, 3, dev, h)
+    e, i = w13.shape[0], w13.shape[1] // 2
+    if w13.shape[1] != 2 * i:
+        raise ValueError(f"w13 must have gate and up rows, got {w13.shape[1]}")
+    _check_weight("w2", w2, w2_scale, 3, dev, i)
+    if w2.shape != (e, h, i):
+        raise ValueError(f"w2 must be {(e, h, i)}, got {tuple(w2.shape)}")
+    if e > 1024:
+        raise ValueError(f"at most 1024 experts are supported, got {e}")
+    if not 1 <= top_k <= 32:
+        raise ValueError(f"top_k must be in [1, 32], got {top_k}")
+    if router_logits is not None:
+        _tensor("router_logits", router_logits, 2, _F32, dev)
+        if router_logits.shape != (m, e):
+            raise ValueError(f"router_logits must be {(m, e)}, got {tuple(router_logits.shape)}")
+        if top_k > e:
+            raise ValueError(f"top_k {top_k} exceeds the {e} experts")
+        if expert_map is not None:
+            raise ValueError("expert_map needs given topk_ids (global ids), not router_logits")
+    else:
+        if topk_weights is None or topk_ids is None:
+            raise ValueError("give router_logits or topk_weights and topk_ids")
+        _tensor("topk_weights", topk_weights, 2, _F32, dev)
+        _tensor("topk_ids", topk_ids, 2, _I32, dev)
+        if topk_weights.shape != (m, top_k) or topk_ids.shape != (m, top_k):
+            raise ValueError(f"topk_weights/topk_ids must be {(m, top_k)}")
+    if expert_map is not None:
+        _tensor("expert_map", expert_map, 1, _I32, dev)
+        if not expert_map.numel():
+            raise ValueError("expert_map is empty")
+    if out is None:
+        out = torch.empty_like(hidden_states)
+    else:
+        _tensor("out", out, 2, (hidden_states.dtype,), dev)
+        if out.shape != (m, h):
+            raise ValueError(f"out must be {(m, h)}, got {tuple(out.shape)}")
+    _check_out(hidden_states.dtype, status, dev)
+    given = router_logits is None
+    dtype, p13, p2 = DTYPES[hidden_states.dtype], w13.data_ptr(), w2.data_ptr()
+    size = _layer_workspace(m, h, i, e, top_k, dtype, not given, p13 & 255, p2 & 255)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    args = _lib.MtpW8A8LayerArgs(m, h, i, e, top_k, 1 if renormalize else 0, dtype,
+                                 0 if expert_map is None else expert_map.numel(), hidden_states.data_ptr(),
+                                 None if given else router_logits.data_ptr(),
+                                 topk_weights.data_ptr() if given else None, topk_ids.data_ptr() if given else None,
+                                 None if expert_map is None else expert_map.data_ptr(), p13, w13_scale.data_ptr(), p2,
+                                 w2_scale.data_ptr(), out.data_ptr(), None if status is None else status.data_ptr(),
+                                 ws.data_ptr(), size)
+    _lib.call("mtp_w8a8_moe_layer", C.byref(args), _stream(dev))
+    return out
