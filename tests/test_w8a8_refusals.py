@@ -111,7 +111,7 @@ class TestOnTheGpu:
     pytestmark = pytest.mark.gpu
 
     def test_shapes_types_and_layouts(self, cuda_device):
-        z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device=cuda_device)
+        z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=cuda_device)
         x, ids = z(4, 8), z(4, 2, dtype=I32)
         bad = [
             ("sort_tokens", (x, ids[:3], 4), {}), ("sort_tokens", (x, ids.long(), 4), {}), ("sort_tokens", (x, ids, 0), {}),
