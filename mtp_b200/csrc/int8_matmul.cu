@@ -5,18 +5,23 @@
 // The sum is exact in int32 (K < 2^17); the scales are applied in fp32 and the
 // result is rounded once.
 //
-// tile_kernel: persistent, warp-specialised, one CTA per SM. A tile is 128
-// output channels (the MMA's M) x up to NT rows of one group (its N, rounded
-// up to 16 for a group's last tile, so a ragged group costs what it has).
+// tile_kernel: persistent, warp-specialised, one CTA per SM. A CTA's tile is
+// 128 output channels (the MMA's M) x up to NT rows of one group (its N, rounded
+// up to 16 or 32 for a group's last tile, so a ragged group costs what it has).
 //   warp 8    producer: per stage (128 of K) one TMA box of weights and the
 //             boxes of rows that the tile has, 128-byte swizzle; columns past
 //             K and rows past the end arrive as zeros;
 //   warp 9    one thread issues tcgen05.mma kind::i8 (K = 32) into one of two
 //             accumulators of NT columns in tensor memory;
-//   warps 0-7 epilogue: tensor memory -> scales -> output, while the next
+//   warps 0-7 epilogue in two halves of 128 threads that take chunks of rows in
+//             turn: tensor memory -> scales -> shared memory, row by row, and
+//             from there 16 bytes a thread to the output, while the next
 //             tile's products run.
-// Gated tiles hold 16 gate channels, then their 16 up channels, four times,
-// so that a gate and its up value lie 16 lanes apart in one warp.
+// PAIR: two CTAs of a cluster take 256 channels together (cta_group::2): each
+// holds its 128 channels and half of the rows, so per product a CTA loads 2/3
+// of what it loads alone. Gated tiles hold 16 gate channels, then their 16 up
+// channels, four times, so that a gate and its up value lie 16 lanes apart in
+// one warp.
 #include "internal.cuh"
 
 #include <cuda.h>
@@ -27,55 +32,149 @@ namespace mtp {
 namespace {
 
 constexpr int kTK = 128;            // K of a stage: one 128-byte swizzle row of int8
-constexpr int kTM = 128;            // channels of a tile
+constexpr int kTM = 128;            // channels of a CTA's tile
 constexpr int kTEpiWarps = 8;
 constexpr int kTThreads = (kTEpiWarps + 2) * 32;
 constexpr int kTMaxGroups = 1024;
+constexpr int kTBox = 32;           // rows of one TMA box
 constexpr uint32_t kTWBytes = kTM * kTK;
+constexpr uint32_t kTStagingBytes = 8192;  // one chunk of output rows; two per epilogue half
 constexpr uint64_t kTTimeoutNs = 2000000000ull;
-constexpr uint32_t kTIdesc = (2u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // D s32, A and B s8, M = 128
+constexpr uint32_t kTIdesc = (2u << 4) | (1u << 7) | (1u << 10);  // D s32, A and B s8
 
-// Ring of a tile of NT rows.
-template <int NT>
+// Ring of a tile of NT rows; a CTA of a pair holds half of them.
+template <int NT, bool PAIR>
 struct Ring {
-  static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-  static constexpr int kBox = NT < 64 ? NT : 64;  // rows of one TMA box
-  static constexpr uint32_t kBytes = kTWBytes + NT * kTK;
+  static constexpr int kRows = PAIR ? NT / 2 : NT;
+  static constexpr int kStages = kRows >= 128 ? 5 : kRows == 64 ? 6 : 8;
+  static constexpr uint32_t kBytes = kTWBytes + kRows * kTK;
 };
 
-struct alignas(8) TileCtrl {
-  uint64_t full[8], empty[8];  // stage landed / consumed
-  uint64_t dfull[2], dempty[2];  // accumulator complete / read
+struct alignas(16) TileCtrl {
+  uint64_t full[8], empty[8];     // stage landed / consumed
+  uint64_t dfull[2], dempty[2];   // accumulator complete / read
   uint32_t tmem;
-  int routed;                  // rows before offsets[E]
-  int pre[kTMaxGroups + 1];    // row tiles before each group
+  int routed;                     // rows before offsets[E]
+  int pre[kTMaxGroups + 1];       // row tiles before each group
+  int first[kTMaxGroups + 1];     // first row of each group
+  alignas(16) float sa[2][256];   // row scales of the tile, per epilogue half
 };
-constexpr uint32_t kTCtrl = 6144;  // control block at the end of the stages
+constexpr uint32_t kTCtrl = 11264;
 static_assert(sizeof(TileCtrl) <= kTCtrl, "control block");
 
-template <int NT>
+template <int NT, bool PAIR>
 constexpr size_t tile_smem() {
-  return 1024 + static_cast<size_t>(Ring<NT>::kStages) * Ring<NT>::kBytes + kTCtrl;
+  return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + 4 * kTStagingBytes + kTCtrl;
 }
-static_assert(tile_smem<256>() <= 227 * 1024 && tile_smem<128>() <= 227 * 1024 && tile_smem<64>() <= 227 * 1024,
+static_assert(tile_smem<256, true>() <= 227 * 1024 && tile_smem<128, false>() <= 227 * 1024 &&
+                  tile_smem<64, false>() <= 227 * 1024 && tile_smem<32, false>() <= 227 * 1024,
               "shared memory");
 
+template <bool PAIR>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
 }
 
 // D[tmem] (+)= A[smem] x B[smem]^T, kind::i8
+template <bool PAIR>
 __device__ __forceinline__ void umma_i8_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// Arrive on this barrier (of both CTAs of a pair) when the products issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void tile_commit(uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    umma_commit(bar);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tile_tmem_alloc(uint32_t dst, uint32_t cols) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, cols);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tile_tmem_free(uint32_t addr, uint32_t cols) {
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else
+    tmem_dealloc(addr, cols);
+}
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared-memory address in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, "
+      "p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// 32 consecutive 32-bit columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
 
 // K-major operand in the 128-byte swizzle: 8-row groups of 1024 bytes.
 __device__ __forceinline__ uint64_t desc_swizzle128(uint32_t addr) {
@@ -91,45 +190,53 @@ struct Waits {
   bool out = false;
   __device__ __forceinline__ explicit Waits(const Int8Args& a) : status(a.status) {}
   __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity) || out) return;
-    if (!mbar_wait(bar, parity, global_timer_ns() + kTTimeoutNs)) {
-      out = true;
-      if (status) atomicOr(status, 1);
-    }
+    if (mbar_try_wait_cluster(bar, parity) || out) return;
+    const uint64_t deadline = global_timer_ns() + kTTimeoutNs;
+    do {
+      if (mbar_try_wait_cluster(bar, parity)) return;
+    } while (global_timer_ns() < deadline);
+    out = true;
+    if (status) atomicOr(status, 1);
   }
 };
 
-// One tile of the walk: group, first row, rows, channel tile.
+// One tile of the walk: group, first row, rows, channel tile of this CTA.
 struct Tile {
   int e, row, n, ct;
 };
 
-template <int NT>
-__device__ __forceinline__ Tile tile_at(const Int8Args& a, const TileCtrl& cb, int t, int& e) {
-  Tile r;
-  const int blk = t / a.ctiles;
-  r.ct = t - blk * a.ctiles;
-  // first group whose tiles end past blk; tiles ascend, so the last one's
-  // group is a lower bound
-  int lo = e, hi = a.E - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cb.pre[mid + 1] > blk)
-      hi = mid;
-    else
-      lo = mid + 1;
+template <int NT, bool PAIR>
+struct Walk {
+  const TileCtrl& cb;
+  int groups, ctiles, ntiles, t, step, rank, e = 0;
+  __device__ __forceinline__ Walk(const Int8Args& a, const TileCtrl& c)
+      : cb(c), groups(a.E), ctiles(a.ctiles), ntiles(c.pre[a.E] * a.ctiles) {
+    rank = PAIR ? static_cast<int>(cta_rank()) : 0;
+    t = PAIR ? blockIdx.x / 2 : blockIdx.x;
+    step = PAIR ? gridDim.x / 2 : gridDim.x;
   }
-  e = lo;
-  r.e = lo;
-  int first = 0, last = a.P;
-  if (a.offsets) {
-    first = min(max(a.offsets[lo], 0), a.P);
-    last = min(max(a.offsets[lo + 1], 0), a.P);
+  __device__ __forceinline__ bool next(Tile& r) {
+    if (t >= ntiles) return false;
+    const int blk = t / ctiles;
+    r.ct = t - blk * ctiles;
+    if (PAIR) r.ct = 2 * r.ct + rank;
+    // first group whose tiles end past blk; tiles ascend, so the last one's
+    // group is a lower bound
+    int hi = groups - 1;
+    while (e < hi) {
+      const int mid = (e + hi) >> 1;
+      if (cb.pre[mid + 1] > blk)
+        hi = mid;
+      else
+        e = mid + 1;
+    }
+    r.e = e;
+    r.row = cb.first[e] + (blk - cb.pre[e]) * NT;
+    r.n = min(NT, cb.first[e + 1] - r.row);
+    t += step;
+    return true;
   }
-  r.row = first + (blk - cb.pre[lo]) * NT;
-  r.n = min(NT, last - r.row);
-  return r;
-}
+};
 
 template <typename T>
 __device__ __forceinline__ T out_cast(float v);
@@ -140,73 +247,89 @@ __device__ __forceinline__ __half out_cast(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ __nv_bfloat16 out_cast(float v) { return __float2bfloat16_rn(v); }
 
-template <int NT, bool GATED>
+template <int NT, bool PAIR, bool GATED>
 __device__ void tile_producer(const CUtensorMap* ta, const CUtensorMap* tb, const Int8Args& a, TileCtrl& cb,
-                              uint32_t stages, int ntiles) {
-  constexpr int S = Ring<NT>::kStages, BOX = Ring<NT>::kBox;
+                              uint32_t stages) {
+  using R = Ring<NT, PAIR>;
   const int nk = (a.K + kTK - 1) / kTK;
   Waits wait(a);
-  int st = 0, e = 0;
+  Walk<NT, PAIR> walk(a, cb);
+  int st = 0;
   uint32_t ph = 0;
   int64_t issued = 0;
-  for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
-    const Tile w = tile_at<NT>(a, cb, t, e);
-    const int boxes = (w.n + BOX - 1) / BOX;
+  Tile w;
+  while (walk.next(w)) {
+    // rows of this CTA: all of the tile's, or this rank's half of the MMA's N
+    const int rows = PAIR ? (w.n + 31) / 32 * 16 : w.n;
+    const int boxes = (rows + kTBox - 1) / kTBox;
+    const int row = w.row + (PAIR ? walk.rank * rows : 0);
+    const uint32_t bytes = kTWBytes + boxes * (kTBox * kTK);
+    const int ch = GATED ? w.e * a.N + w.ct * 64 : w.e * a.N + w.ct * kTM;
     for (int s = 0; s < nk; ++s) {
       wait(smem_u32(&cb.empty[st]), ph ^ 1u);
-      const uint32_t sb = stages + st * Ring<NT>::kBytes, bar = smem_u32(&cb.full[st]);
-      mbar_arrive_expect_tx(bar, kTWBytes + boxes * (BOX * kTK));
+      const uint32_t sb = stages + st * R::kBytes;
+      uint32_t bar = smem_u32(&cb.full[st]);
+      if (PAIR) {
+        // both CTAs' bytes arrive on the first one's barrier
+        if (walk.rank == 0) mbar_arrive_expect_tx(bar, 2 * bytes);
+        bar = in_leader(bar);
+      } else {
+        mbar_arrive_expect_tx(bar, bytes);
+      }
       if (GATED) {
-        const int g0 = w.e * a.N + w.ct * 64, u0 = g0 + a.N / 2;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tma_2d(sb + q * 4096, tb, s * kTK, g0 + 16 * q, bar);
-          tma_2d(sb + q * 4096 + 2048, tb, s * kTK, u0 + 16 * q, bar);
+          tma_2d<PAIR>(sb + q * 4096, tb, s * kTK, ch + 16 * q, bar);
+          tma_2d<PAIR>(sb + q * 4096 + 2048, tb, s * kTK, ch + a.N / 2 + 16 * q, bar);
         }
       } else {
-        tma_2d(sb, tb, s * kTK, w.e * a.N + w.ct * kTM, bar);
+        tma_2d<PAIR>(sb, tb, s * kTK, ch, bar);
       }
-      for (int q = 0; q < boxes; ++q) tma_2d(sb + kTWBytes + q * (BOX * kTK), ta, s * kTK, w.row + q * BOX, bar);
+      for (int q = 0; q < boxes; ++q)
+        tma_2d<PAIR>(sb + kTWBytes + q * (kTBox * kTK), ta, s * kTK, row + q * kTBox, bar);
       ++issued;
-      if (++st == S) {
+      if (++st == R::kStages) {
         st = 0;
         ph ^= 1u;
       }
     }
   }
-  // no copy may still be writing shared memory when the CTA exits
+  // No copy may still be writing shared memory when the CTA exits: stage j's
+  // products (whose completion both CTAs of a pair see) came after its bytes.
   wait.out = false;
-  for (int64_t j = issued - 1; j >= 0 && j >= issued - S; --j)
-    wait(smem_u32(&cb.full[j % S]), static_cast<uint32_t>((j / S) & 1));
+  for (int64_t j = issued - 1; j >= 0 && j >= issued - R::kStages; --j)
+    wait(smem_u32(&cb.empty[j % R::kStages]), static_cast<uint32_t>((j / R::kStages) & 1));
 }
 
-template <int NT>
-__device__ void tile_mma(const Int8Args& a, TileCtrl& cb, uint32_t stages, uint32_t tmem, int ntiles) {
-  constexpr int S = Ring<NT>::kStages;
+template <int NT, bool PAIR>
+__device__ void tile_mma(const Int8Args& a, TileCtrl& cb, uint32_t stages, uint32_t tmem) {
+  using R = Ring<NT, PAIR>;
   const int nk = (a.K + kTK - 1) / kTK;
   Waits wait(a);
-  int st = 0, db = 0, e = 0;
+  Walk<NT, PAIR> walk(a, cb);
+  int st = 0, db = 0;
   uint32_t ph = 0, dph = 0;
-  for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
-    const Tile w = tile_at<NT>(a, cb, t, e);
-    const uint32_t idesc = kTIdesc | (static_cast<uint32_t>((w.n + 15) >> 4) << 18);
+  Tile w;
+  while (walk.next(w)) {
+    const uint32_t n = PAIR ? (w.n + 31) / 32 * 32 : (w.n + 15) / 16 * 16;
+    const uint32_t idesc = kTIdesc | (n >> 3 << 17) | ((PAIR ? 16u : 8u) << 24);
     wait(smem_u32(&cb.dempty[db]), dph ^ 1u);
     tc_fence_after();
     const uint32_t d = tmem + db * NT;
     for (int s = 0; s < nk; ++s) {
       wait(smem_u32(&cb.full[st]), ph);
       tc_fence_after();
-      const uint64_t wd = desc_swizzle128(stages + st * Ring<NT>::kBytes);
-      const uint64_t xd = desc_swizzle128(stages + st * Ring<NT>::kBytes + kTWBytes);
+      const uint64_t wd = desc_swizzle128(stages + st * R::kBytes);
+      const uint64_t xd = desc_swizzle128(stages + st * R::kBytes + kTWBytes);
 #pragma unroll
-      for (int j = 0; j < kTK / 32; ++j) umma_i8_ss(d, wd + 2 * j, xd + 2 * j, idesc, (s | j) != 0);
-      umma_commit(smem_u32(&cb.empty[st]));
-      if (++st == S) {
+      for (int j = 0; j < kTK / 32; ++j) umma_i8_ss<PAIR>(d, wd + 2 * j, xd + 2 * j, idesc, (s | j) != 0);
+      tile_commit<PAIR>(smem_u32(&cb.empty[st]));
+      if (++st == R::kStages) {
         st = 0;
         ph ^= 1u;
       }
     }
-    umma_commit(smem_u32(&cb.dfull[db]));
+    tile_commit<PAIR>(smem_u32(&cb.dfull[db]));
     if (++db == 2) {
       db = 0;
       dph ^= 1u;
@@ -230,58 +353,107 @@ __device__ __forceinline__ void zero_tail(uint8_t* from, uint8_t* to) {
   if (tid < to - hi) hi[tid] = 0;
 }
 
-template <int NT, bool GATED, typename T>
-__device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint32_t tmem, int ntiles) {
+template <int NT, bool PAIR, bool GATED, typename T>
+__device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging, uint32_t tmem) {
+  constexpr int kChannels = GATED ? 64 : kTM;                 // output channels of a tile
+  constexpr int kRow = kChannels * sizeof(T);                 // bytes of a staged row,
+  constexpr int kPitch = kRow + (GATED ? kRow / 4 : 0);       // apart: the two rows of a gated store on other banks
+  constexpr int kChunk = 64 / sizeof(T);                      // rows of a chunk
+  constexpr int kPieces = kRow / 16;
+  static_assert(kChunk * kPitch <= static_cast<int>(kTStagingBytes), "staging");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = warp & 3, half = warp >> 2;
+  const int quad = warp & 3, half = warp >> 2, htid = threadIdx.x & 127;
   const int width = GATED ? a.N / 2 : a.N;  // columns of the output
   T* out = static_cast<T*>(a.out);
   if (cb.routed < a.P)
     zero_tail(reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.routed) * width),
               reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width));
+  const int64_t pitch = static_cast<int64_t>(width) * sizeof(T);
+  const bool wide = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  uint8_t* stg = staging + half * 2 * kTStagingBytes;
+  float* sa = cb.sa[half];
+  const uint32_t dbar = PAIR ? in_leader(smem_u32(&cb.dempty[0])) : smem_u32(&cb.dempty[0]);
   Waits wait(a);
-  int db = 0, e = 0;
+  Walk<NT, PAIR> walk(a, cb);
+  int db = 0, buf = 0;
   uint32_t dph = 0;
-  for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
-    const Tile w = tile_at<NT>(a, cb, t, e);
+  Tile w;
+  while (walk.next(w)) {
     // this lane's output channel and the row of b behind its accumulator lane
-    const int ch = GATED ? w.ct * 64 + 16 * quad + (lane & 15) : w.ct * kTM + 32 * quad + lane;
-    const bool valid = ch < width;
-    const int brow = GATED && lane >= 16 ? a.N / 2 + ch : ch;
+    const int ch0 = w.ct * kChannels;
+    const int local = GATED ? 16 * quad + (lane & 15) : 32 * quad + lane;
+    const bool valid = ch0 + local < width;
+    const int brow = ch0 + local + (GATED && lane >= 16 ? a.N / 2 : 0);
     const float sb = valid ? a.b_scale[static_cast<int64_t>(w.e) * a.N + brow] : 0.f;
-    const float bias = valid && a.bias ? a.bias[ch] : 0.f;
+    const float bias = valid && a.bias ? a.bias[ch0 + local] : 0.f;
+    // (the last tile's were read before the last chunk's barrier)
+    for (int i = htid; i < NT; i += 128) sa[i] = i < w.n ? a.a_scale[w.row + i] : 0.f;
+    named_bar_sync(1 + half, 128);
     wait(smem_u32(&cb.dfull[db]), dph);
     tc_fence_after();
     const uint32_t dt = tmem + (static_cast<uint32_t>(32 * quad) << 16) + db * NT;
-    for (int c = 16 * half; c < w.n; c += 32) {
-      const int mine = c + (lane & 15);
-      const float sa = mine < w.n ? a.a_scale[w.row + mine] : 0.f;
-      uint32_t v[16];
-      tmem_ld16(dt + c, v);
+    const int row_bytes = min(kChannels, width - ch0) * static_cast<int>(sizeof(T));
+    for (int c = kChunk * half; c < w.n; c += 2 * kChunk) {
+      uint32_t v[kChunk];
+      tmem_ld_chunk(dt + c, v);
       tmem_wait_ld();
-      T* o = out + static_cast<int64_t>(w.row + c) * width + ch;
+      uint8_t* sw = stg + buf * kTStagingBytes;
       if (GATED) {
         // two rows at a time: the low lanes take the first, the high lanes the second
+        uint8_t* at = sw + local * sizeof(T) + (lane >> 4) * kPitch;
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float z0 = __int2float_rn(static_cast<int>(v[j])) * __shfl_sync(kFullMask, sa, j) * sb;
-          const float z1 = __int2float_rn(static_cast<int>(v[j + 1])) * __shfl_sync(kFullMask, sa, j + 1) * sb;
-          const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
-          const float h = lane < 16 ? silu_fast(z0) * got : silu_fast(got) * z1;
-          const int r = j + (lane >> 4);
-          if (valid && c + r < w.n) o[static_cast<int64_t>(r) * width] = out_cast<T>(h);
+        for (int j = 0; j < kChunk; j += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(sa + c + j);
+          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            const float z0 = __int2float_rn(static_cast<int>(v[j + q])) * s[q] * sb;
+            const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sb;
+            const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
+            const float gate = lane < 16 ? z0 : got, up = lane < 16 ? got : z1;
+            *reinterpret_cast<T*>(at + (j + q) * kPitch) = out_cast<T>(silu_fast(gate) * up);
+          }
         }
       } else {
+        uint8_t* at = sw + local * sizeof(T);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float z = __int2float_rn(static_cast<int>(v[j])) * __shfl_sync(kFullMask, sa, j) * sb + bias;
-          if (valid && c + j < w.n) o[static_cast<int64_t>(j) * width] = out_cast<T>(z);
+        for (int j = 0; j < kChunk; j += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(sa + c + j);
+          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<T*>(at + (j + q) * kPitch) =
+                out_cast<T>(fmaf(__int2float_rn(static_cast<int>(v[j + q])) * s[q], sb, bias));
         }
       }
+      // The other buffer's readers are past the last barrier, so one per chunk is enough.
+      named_bar_sync(1 + half, 128);
+      const int rows = min(kChunk, w.n - c);
+      uint8_t* o = reinterpret_cast<uint8_t*>(out) + (w.row + c) * pitch + static_cast<int64_t>(ch0) * sizeof(T);
+      if (wide) {
+#pragma unroll
+        for (int i = 0; i < kChunk * kPieces / 128; ++i) {
+          const int x = htid + 128 * i, r = x / kPieces, piece = x % kPieces;
+          if (r < rows && piece * 16 < row_bytes)
+            *reinterpret_cast<uint4*>(o + r * pitch + piece * 16) = lds128(smem_u32(sw + r * kPitch + piece * 16));
+        }
+      } else {
+        for (int x = htid; x < kChunk * kChannels; x += 128) {
+          const int r = x / kChannels, q = x % kChannels * static_cast<int>(sizeof(T));
+          if (r < rows && q < row_bytes)
+            *reinterpret_cast<T*>(o + r * pitch + q) = *reinterpret_cast<const T*>(sw + r * kPitch + q);
+        }
+      }
+      buf ^= 1;
     }
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&cb.dempty[db]));
+    if (lane == 0) {
+      if (PAIR)
+        mbar_arrive_cluster(dbar + 8 * db);
+      else
+        mbar_arrive(dbar + 8 * db);
+    }
     if (++db == 2) {
       db = 0;
       dph ^= 1u;
@@ -289,37 +461,40 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint32_t tmem, in
   }
 }
 
-template <int NT, bool GATED, typename T>
+template <int NT, bool PAIR, bool GATED, typename T>
 __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap ta,
                                                             const __grid_constant__ CUtensorMap tb, const Int8Args a) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr int S = Ring<NT>::kStages;
+  using R = Ring<NT, PAIR>;
   const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (stages - smem_u32(smem_raw));
-  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(aligned + S * Ring<NT>::kBytes);
+  uint8_t* staging = aligned + R::kStages * R::kBytes;
+  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(staging + 4 * kTStagingBytes);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < R::kStages; ++i) {
       mbar_init(smem_u32(&cb.full[i]), 1);
       mbar_init(smem_u32(&cb.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&cb.dfull[i]), 1);
-      mbar_init(smem_u32(&cb.dempty[i]), kTEpiWarps);
+      mbar_init(smem_u32(&cb.dempty[i]), PAIR ? 2 * kTEpiWarps : kTEpiWarps);
     }
     fence_mbar_init();
   }
-  if (warp == kTEpiWarps + 1) {
-    tmem_alloc(smem_u32(&cb.tmem), 2 * NT);
-    tmem_relinquish();
-  }
+  if (warp == kTEpiWarps + 1) tile_tmem_alloc<PAIR>(smem_u32(&cb.tmem), 2 * NT);
   pdl_launch_dependents();
   pdl_wait();
-  // row tiles of every group, then their running sum
-  for (int e = threadIdx.x; e < a.E; e += kTThreads) {
-    int n = a.P;
-    if (a.offsets) n = min(max(a.offsets[e + 1], 0), a.P) - min(max(a.offsets[e], 0), a.P);
-    cb.pre[e + 1] = (max(n, 0) + NT - 1) / NT;
+  // first row and row tiles of every group, then the tiles' running sum
+  for (int e = threadIdx.x; e <= a.E; e += kTThreads) {
+    const int lo = a.offsets ? min(max(a.offsets[e], 0), a.P) : e * a.P;
+    if (e < a.E) {
+      const int hi = a.offsets ? min(max(a.offsets[e + 1], 0), a.P) : a.P;
+      cb.pre[e + 1] = (max(hi - lo, 0) + NT - 1) / NT;
+    } else {
+      cb.routed = lo;
+    }
+    cb.first[e] = lo;
   }
   __syncthreads();
   if (warp == 0) {
@@ -335,29 +510,27 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
       if (e0 + lane < a.E) cb.pre[e0 + lane + 1] = run + x;
       run += __shfl_sync(kFullMask, x, 31);
     }
-    if (lane == 0) {
-      cb.pre[0] = 0;
-      cb.routed = a.offsets ? min(max(a.offsets[a.E], 0), a.P) : a.P;
-    }
+    if (lane == 0) cb.pre[0] = 0;
   }
   tc_fence_before();
+  if (PAIR) cluster_sync();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = cb.tmem;
-  const int ntiles = cb.pre[a.E] * a.ctiles;
   if (warp == kTEpiWarps) {
-    if ((threadIdx.x & 31) == 0) tile_producer<NT, GATED>(&ta, &tb, a, cb, stages, ntiles);
+    if ((threadIdx.x & 31) == 0) tile_producer<NT, PAIR, GATED>(&ta, &tb, a, cb, stages);
   } else if (warp == kTEpiWarps + 1) {
-    if ((threadIdx.x & 31) == 0) tile_mma<NT>(a, cb, stages, tmem, ntiles);
+    if ((threadIdx.x & 31) == 0 && (!PAIR || cta_rank() == 0)) tile_mma<NT, PAIR>(a, cb, stages, tmem);
   } else {
-    tile_epilogue<NT, GATED, T>(a, cb, tmem, ntiles);
+    tile_epilogue<NT, PAIR, GATED, T>(a, cb, staging, tmem);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers and tensor memory are in use until here
   if (warp == kTEpiWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * NT);
+    tile_tmem_free<PAIR>(tmem, 2 * NT);
   }
 }
 
@@ -443,48 +616,89 @@ int device_sms() {
   return sms[dev];
 }
 
-template <int NT, bool GATED, typename T>
+// Clusters of two CTAs that the device holds at once.
+template <typename F>
+int pair_slots(F* kernel, size_t smem, int sms) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms / 2 * 2);
+  cfg.blockDim = dim3(kTThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+template <int NT, bool PAIR, bool GATED, typename T>
 int run_tiles(Int8Args& a, const void* ap, int64_t a_stride, const void* bp, int64_t b_stride, int sms,
               cudaStream_t st) {
-  auto* kernel = tile_kernel<NT, GATED, T>;
-  constexpr size_t smem = tile_smem<NT>();
-  static int configured_device = -1;
+  auto* kernel = tile_kernel<NT, PAIR, GATED, T>;
+  constexpr size_t smem = tile_smem<NT, PAIR>();
+  static int configured_device = -1, slots = 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
   if (configured_device != dev) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) !=
         cudaSuccess)
       return MTP_ERR_CUDA;
+    slots = PAIR ? pair_slots(kernel, smem, sms) : sms;
+    if (slots < 1) return MTP_ERR_CUDA;
     configured_device = dev;
   }
   CUtensorMap ta, tb;
-  int rc = encode_rows(&ta, ap, a.P, a.K, a_stride, Ring<NT>::kBox);
+  int rc = encode_rows(&ta, ap, a.P, a.K, a_stride, kTBox);
   if (rc == MTP_OK) rc = encode_rows(&tb, bp, static_cast<int64_t>(a.E) * a.N, a.K, b_stride, GATED ? 16 : kTM);
   if (rc != MTP_OK) return rc;
-  a.ctiles = GATED ? (a.N / 2 + 63) / 64 : (a.N + kTM - 1) / kTM;
+  const int channels = (GATED ? 64 : kTM) * (PAIR ? 2 : 1), width = GATED ? a.N / 2 : a.N;
+  a.ctiles = (width + channels - 1) / channels;
   // row tiles: at most one partial one per group that has rows
   const int64_t blocks = a.P / NT + std::min(a.P, a.E);
-  const int64_t grid = std::min<int64_t>(sms, std::max<int64_t>(blocks * a.ctiles, 1));
-  return launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(kTThreads), smem, st, ta, tb, a);
+  const int64_t grid = std::min<int64_t>(slots, std::max<int64_t>(blocks * a.ctiles, 1)) * (PAIR ? 2 : 1);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kTThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, a) != cudaSuccess) {
+    cudaGetLastError();
+    return MTP_ERR_LAUNCH;
+  }
+  return MTP_OK;
 }
 
-template <int NT, bool GATED>
+template <int NT, bool PAIR, bool GATED>
 int by_out(Int8Args& a, int out_dtype, const void* ap, int64_t as, const void* bp, int64_t bs, int sms,
            cudaStream_t st) {
   switch (out_dtype) {
-    case MTP_DTYPE_BF16: return run_tiles<NT, GATED, __nv_bfloat16>(a, ap, as, bp, bs, sms, st);
-    case MTP_DTYPE_FP16: return run_tiles<NT, GATED, __half>(a, ap, as, bp, bs, sms, st);
-    default: return run_tiles<NT, GATED, float>(a, ap, as, bp, bs, sms, st);
+    case MTP_DTYPE_BF16: return run_tiles<NT, PAIR, GATED, __nv_bfloat16>(a, ap, as, bp, bs, sms, st);
+    case MTP_DTYPE_FP16: return run_tiles<NT, PAIR, GATED, __half>(a, ap, as, bp, bs, sms, st);
+    default: return run_tiles<NT, PAIR, GATED, float>(a, ap, as, bp, bs, sms, st);
   }
 }
 
 template <bool GATED>
 int by_rows(Int8Args& a, int nt, int out_dtype, const void* ap, int64_t as, const void* bp, int64_t bs, int sms,
             cudaStream_t st) {
-  if (nt == 256) return by_out<256, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
-  if (nt == 128) return by_out<128, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
-  if (nt == 64) return by_out<64, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
-  return by_out<32, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
+  if (nt == 256) return by_out<256, true, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
+  if (nt == 128) return by_out<128, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
+  if (nt == 64) return by_out<64, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
+  return by_out<32, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
 }
 
 }  // namespace
@@ -504,10 +718,14 @@ int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, in
   if (!sms) return MTP_ERR_CUDA;
   // Rows of a tile: enough for the average group, fewer while the tiles do not
   // fill the SMs.
-  const int per_group = (a.P + a.E - 1) / a.E;
+  const int per_group = (a.P + a.E - 1) / a.E, width = gated ? a.N / 2 : a.N;
+  auto ctas = [&](int nt) {
+    const int channels = (gated ? 64 : kTM) * (nt == 256 ? 2 : 1);
+    return static_cast<int64_t>((width + channels - 1) / channels) * ((per_group + nt - 1) / nt) *
+           std::min(a.P, a.E) * (nt == 256 ? 2 : 1);
+  };
   int nt = per_group <= 24 ? 32 : per_group <= 48 ? 64 : per_group <= 96 ? 128 : 256;
-  const int64_t ct = gated ? (a.N / 2 + 63) / 64 : (a.N + kTM - 1) / kTM;
-  while (nt > 32 && ct * ((per_group + nt - 1) / nt) * std::min(a.P, a.E) < sms) nt /= 2;
+  while (nt > 32 && ctas(nt) < sms) nt /= 2;
   return gated ? by_rows<true>(a, nt, out_dtype, ap, a_stride, bp, b_stride, sms, st)
                : by_rows<false>(a, nt, out_dtype, ap, a_stride, bp, b_stride, sms, st);
 }
