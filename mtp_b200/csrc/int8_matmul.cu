@@ -8,18 +8,21 @@
 // tile_kernel: persistent, warp-specialised, one CTA per SM. A CTA's tile is
 // 128 output channels (the MMA's M) x up to NT rows of one group (its N, rounded
 // up to 16 or 32 for a group's last tile, so a ragged group costs what it has).
-//   warp 8    producer: per stage (128 of K) one TMA box of weights and the
-//             boxes of rows that the tile has, 128-byte swizzle; columns past
-//             K and rows past the end arrive as zeros;
+//   warp 8    producer: per stage (128 of K) one TMA box of weights and one of
+//             rows (a few of 32 where the tile has few), 128-byte swizzle;
+//             columns past K and rows past the end arrive as zeros. Few large
+//             boxes: with boxes of 32 rows throughout, 8192^2 x 2048 took 113 us
+//             against 98;
 //   warp 9    one thread issues tcgen05.mma kind::i8 (K = 32) into one of two
 //             accumulators of NT columns in tensor memory;
-//   warps 0-7 epilogue in two halves of 128 threads that take chunks of rows in
-//             turn: tensor memory -> scales -> shared memory, row by row, and
-//             from there 16 bytes a thread to the output, while the next
-//             tile's products run.
+//   warps 0-7 epilogue: each warp takes its 32 channels of every other chunk of
+//             rows on its own: tensor memory -> scales -> its own staging rows
+//             in shared memory -> 16 bytes a thread to the output, while the
+//             next tile's products run and the next scales are on their way.
 // PAIR: two CTAs of a cluster take 256 channels together (cta_group::2): each
 // holds its 128 channels and half of the rows, so per product a CTA loads 2/3
-// of what it loads alone. Gated tiles hold 16 gate channels, then their 16 up
+// of what it loads alone. A group's rows are shared out evenly over its tiles.
+// Gated tiles hold 16 gate channels, then their 16 up
 // channels, four times, so that a gate and its up value lie 16 lanes apart in
 // one warp.
 #include "internal.cuh"
@@ -36,9 +39,9 @@ constexpr int kTM = 128;            // channels of a CTA's tile
 constexpr int kTEpiWarps = 8;
 constexpr int kTThreads = (kTEpiWarps + 2) * 32;
 constexpr int kTMaxGroups = 1024;
-constexpr int kTBox = 32;           // rows of one TMA box
+constexpr int kTBox = 32;           // rows of a small TMA box
 constexpr uint32_t kTWBytes = kTM * kTK;
-constexpr uint32_t kTStagingBytes = 8192;  // one chunk of output rows; two per epilogue half
+constexpr uint32_t kTStagingBytes = 2048;  // one chunk of output rows of an epilogue warp; two per warp
 constexpr uint64_t kTTimeoutNs = 2000000000ull;
 constexpr uint32_t kTIdesc = (2u << 4) | (1u << 7) | (1u << 10);  // D s32, A and B s8
 
@@ -57,14 +60,15 @@ struct alignas(16) TileCtrl {
   int routed;                     // rows before offsets[E]
   int pre[kTMaxGroups + 1];       // row tiles before each group
   int first[kTMaxGroups + 1];     // first row of each group
-  alignas(16) float sa[2][256];   // row scales of the tile, per epilogue half
+  uint16_t rows[kTMaxGroups];     // rows of a tile of each group
+  alignas(16) float sa[kTEpiWarps][32];  // row scales of a warp's chunk
 };
-constexpr uint32_t kTCtrl = 11264;
+constexpr uint32_t kTCtrl = 11776;
 static_assert(sizeof(TileCtrl) <= kTCtrl, "control block");
 
 template <int NT, bool PAIR>
 constexpr size_t tile_smem() {
-  return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + 4 * kTStagingBytes + kTCtrl;
+  return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + 2 * kTEpiWarps * kTStagingBytes + kTCtrl;
 }
 static_assert(tile_smem<256, true>() <= 227 * 1024 && tile_smem<128, false>() <= 227 * 1024 &&
                   tile_smem<64, false>() <= 227 * 1024 && tile_smem<32, false>() <= 227 * 1024,
@@ -83,6 +87,22 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
             dst),
         "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int x, int block, int group, uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(0), "r"(block), "r"(group), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, "
+        "%5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(0), "r"(block), "r"(group), "r"(bar)
         : "memory");
 }
 
@@ -189,11 +209,13 @@ struct Waits {
   int32_t* status;
   bool out = false;
   __device__ __forceinline__ explicit Waits(const Int8Args& a) : status(a.status) {}
-  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
-    if (mbar_try_wait_cluster(bar, parity) || out) return;
+  template <bool CLUSTER = false>  // CLUSTER: arrivals of the other CTA of the pair
+  __device__ __forceinline__ void on(uint32_t bar, uint32_t parity) {
+    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+    if (done() || out) return;
     const uint64_t deadline = global_timer_ns() + kTTimeoutNs;
     do {
-      if (mbar_try_wait_cluster(bar, parity)) return;
+      if (done()) return;
     } while (global_timer_ns() < deadline);
     out = true;
     if (status) atomicOr(status, 1);
@@ -231,8 +253,9 @@ struct Walk {
         e = mid + 1;
     }
     r.e = e;
-    r.row = cb.first[e] + (blk - cb.pre[e]) * NT;
-    r.n = min(NT, cb.first[e + 1] - r.row);
+    const int rows = cb.rows[e];
+    r.row = cb.first[e] + (blk - cb.pre[e]) * rows;
+    r.n = min(rows, cb.first[e + 1] - r.row);
     t += step;
     return true;
   }
@@ -247,9 +270,14 @@ __device__ __forceinline__ __half out_cast(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ __nv_bfloat16 out_cast(float v) { return __float2bfloat16_rn(v); }
 
+// Tensor maps: rows of a in boxes of a ring's rows and of kTBox, weights.
+struct Maps {
+  CUtensorMap rows, few, weights;
+  int blocks;  // gated: 16-channel blocks of gate and up in one box of the weights' map
+};
+
 template <int NT, bool PAIR, bool GATED>
-__device__ void tile_producer(const CUtensorMap* ta, const CUtensorMap* tb, const Int8Args& a, TileCtrl& cb,
-                              uint32_t stages) {
+__device__ void tile_producer(const Maps& m, const Int8Args& a, TileCtrl& cb, uint32_t stages) {
   using R = Ring<NT, PAIR>;
   const int nk = (a.K + kTK - 1) / kTK;
   Waits wait(a);
@@ -261,12 +289,12 @@ __device__ void tile_producer(const CUtensorMap* ta, const CUtensorMap* tb, cons
   while (walk.next(w)) {
     // rows of this CTA: all of the tile's, or this rank's half of the MMA's N
     const int rows = PAIR ? (w.n + 31) / 32 * 16 : w.n;
-    const int boxes = (rows + kTBox - 1) / kTBox;
     const int row = w.row + (PAIR ? walk.rank * rows : 0);
-    const uint32_t bytes = kTWBytes + boxes * (kTBox * kTK);
+    const int boxes = 2 * rows > R::kRows ? 0 : (rows + kTBox - 1) / kTBox;  // 0: one large box
+    const uint32_t bytes = kTWBytes + (boxes ? boxes * kTBox : R::kRows) * kTK;
     const int ch = GATED ? w.e * a.N + w.ct * 64 : w.e * a.N + w.ct * kTM;
     for (int s = 0; s < nk; ++s) {
-      wait(smem_u32(&cb.empty[st]), ph ^ 1u);
+      wait.on(smem_u32(&cb.empty[st]), ph ^ 1u);
       const uint32_t sb = stages + st * R::kBytes;
       uint32_t bar = smem_u32(&cb.full[st]);
       if (PAIR) {
@@ -276,17 +304,20 @@ __device__ void tile_producer(const CUtensorMap* ta, const CUtensorMap* tb, cons
       } else {
         mbar_arrive_expect_tx(bar, bytes);
       }
-      if (GATED) {
+      if (!GATED) {
+        tma_2d<PAIR>(sb, &m.weights, s * kTK, ch, bar);
+      } else if (m.blocks) {
+        tma_5d<PAIR>(sb, &m.weights, s * kTK, w.ct * 4, w.e, bar);
+      } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tma_2d<PAIR>(sb + q * 4096, tb, s * kTK, ch + 16 * q, bar);
-          tma_2d<PAIR>(sb + q * 4096 + 2048, tb, s * kTK, ch + a.N / 2 + 16 * q, bar);
+          tma_2d<PAIR>(sb + q * 4096, &m.weights, s * kTK, ch + 16 * q, bar);
+          tma_2d<PAIR>(sb + q * 4096 + 2048, &m.weights, s * kTK, ch + a.N / 2 + 16 * q, bar);
         }
-      } else {
-        tma_2d<PAIR>(sb, tb, s * kTK, ch, bar);
       }
+      if (!boxes) tma_2d<PAIR>(sb + kTWBytes, &m.rows, s * kTK, row, bar);
       for (int q = 0; q < boxes; ++q)
-        tma_2d<PAIR>(sb + kTWBytes + q * (kTBox * kTK), ta, s * kTK, row + q * kTBox, bar);
+        tma_2d<PAIR>(sb + kTWBytes + q * (kTBox * kTK), &m.few, s * kTK, row + q * kTBox, bar);
       ++issued;
       if (++st == R::kStages) {
         st = 0;
@@ -298,7 +329,7 @@ __device__ void tile_producer(const CUtensorMap* ta, const CUtensorMap* tb, cons
   // products (whose completion both CTAs of a pair see) came after its bytes.
   wait.out = false;
   for (int64_t j = issued - 1; j >= 0 && j >= issued - R::kStages; --j)
-    wait(smem_u32(&cb.empty[j % R::kStages]), static_cast<uint32_t>((j / R::kStages) & 1));
+    wait.on(smem_u32(&cb.empty[j % R::kStages]), static_cast<uint32_t>((j / R::kStages) & 1));
 }
 
 template <int NT, bool PAIR>
@@ -313,11 +344,11 @@ __device__ void tile_mma(const Int8Args& a, TileCtrl& cb, uint32_t stages, uint3
   while (walk.next(w)) {
     const uint32_t n = PAIR ? (w.n + 31) / 32 * 32 : (w.n + 15) / 16 * 16;
     const uint32_t idesc = kTIdesc | (n >> 3 << 17) | ((PAIR ? 16u : 8u) << 24);
-    wait(smem_u32(&cb.dempty[db]), dph ^ 1u);
+    wait.template on<PAIR>(smem_u32(&cb.dempty[db]), dph ^ 1u);
     tc_fence_after();
     const uint32_t d = tmem + db * NT;
     for (int s = 0; s < nk; ++s) {
-      wait(smem_u32(&cb.full[st]), ph);
+      wait.on(smem_u32(&cb.full[st]), ph);
       tc_fence_after();
       const uint64_t wd = desc_swizzle128(stages + st * R::kBytes);
       const uint64_t xd = desc_swizzle128(stages + st * R::kBytes + kTWBytes);
@@ -355,14 +386,13 @@ __device__ __forceinline__ void zero_tail(uint8_t* from, uint8_t* to) {
 
 template <int NT, bool PAIR, bool GATED, typename T>
 __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging, uint32_t tmem) {
-  constexpr int kChannels = GATED ? 64 : kTM;                 // output channels of a tile
-  constexpr int kRow = kChannels * sizeof(T);                 // bytes of a staged row,
-  constexpr int kPitch = kRow + (GATED ? kRow / 4 : 0);       // apart: the two rows of a gated store on other banks
-  constexpr int kChunk = 64 / sizeof(T);                      // rows of a chunk
+  constexpr int kChannels = GATED ? 16 : 32;                // output channels of a warp
+  constexpr int kRow = kChannels * sizeof(T);               // bytes of a staged row
+  constexpr int kChunk = 64 / sizeof(T);                    // rows of a chunk
   constexpr int kPieces = kRow / 16;
-  static_assert(kChunk * kPitch <= static_cast<int>(kTStagingBytes), "staging");
+  static_assert(kChunk * kRow <= static_cast<int>(kTStagingBytes), "staging");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = warp & 3, half = warp >> 2, htid = threadIdx.x & 127;
+  const int quad = warp & 3, half = warp >> 2;
   const int width = GATED ? a.N / 2 : a.N;  // columns of the output
   T* out = static_cast<T*>(a.out);
   if (cb.routed < a.P)
@@ -370,78 +400,96 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
               reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width));
   const int64_t pitch = static_cast<int64_t>(width) * sizeof(T);
   const bool wide = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  uint8_t* stg = staging + half * 2 * kTStagingBytes;
-  float* sa = cb.sa[half];
+  uint8_t* stg = staging + warp * 2 * kTStagingBytes;
+  float* sas = cb.sa[warp];
   const uint32_t dbar = PAIR ? in_leader(smem_u32(&cb.dempty[0])) : smem_u32(&cb.dempty[0]);
+  const int local = GATED ? lane & 15 : lane;  // channel of the warp's
+  // scales of a tile: this lane's channel (gated: of its gate or up row), its row of the warp's first chunk
+  struct Scales {
+    float sb, bias, sa;
+  };
+  auto first_channel = [&](const Tile& w) { return w.ct * 4 * kChannels + quad * kChannels; };
+  auto row_scale = [&](const Tile& w, int c) {
+    return lane < kChunk && c + lane < w.n ? a.a_scale[w.row + c + lane] : 0.f;
+  };
+  auto load = [&](const Tile& w) {
+    const int ch = first_channel(w) + local;
+    const bool in = ch < width;
+    Scales r;
+    r.sb = in ? a.b_scale[static_cast<int64_t>(w.e) * a.N + ch + (GATED && lane >= 16 ? a.N / 2 : 0)] : 0.f;
+    r.bias = in && a.bias ? a.bias[ch] : 0.f;
+    r.sa = row_scale(w, kChunk * half);
+    return r;
+  };
   Waits wait(a);
   Walk<NT, PAIR> walk(a, cb);
   int db = 0, buf = 0;
   uint32_t dph = 0;
-  Tile w;
-  while (walk.next(w)) {
-    // this lane's output channel and the row of b behind its accumulator lane
-    const int ch0 = w.ct * kChannels;
-    const int local = GATED ? 16 * quad + (lane & 15) : 32 * quad + lane;
-    const bool valid = ch0 + local < width;
-    const int brow = ch0 + local + (GATED && lane >= 16 ? a.N / 2 : 0);
-    const float sb = valid ? a.b_scale[static_cast<int64_t>(w.e) * a.N + brow] : 0.f;
-    const float bias = valid && a.bias ? a.bias[ch0 + local] : 0.f;
-    // (the last tile's were read before the last chunk's barrier)
-    for (int i = htid; i < NT; i += 128) sa[i] = i < w.n ? a.a_scale[w.row + i] : 0.f;
-    named_bar_sync(1 + half, 128);
-    wait(smem_u32(&cb.dfull[db]), dph);
+  Tile w, after;
+  bool more = walk.next(w);
+  Scales sc = {}, nsc = {};
+  if (more) sc = load(w);
+  while (more) {
+    more = walk.next(after);
+    if (more) nsc = load(after);  // on its way during this tile
+    wait.on(smem_u32(&cb.dfull[db]), dph);
     tc_fence_after();
     const uint32_t dt = tmem + (static_cast<uint32_t>(32 * quad) << 16) + db * NT;
+    const int ch0 = first_channel(w);
     const int row_bytes = min(kChannels, width - ch0) * static_cast<int>(sizeof(T));
     for (int c = kChunk * half; c < w.n; c += 2 * kChunk) {
       uint32_t v[kChunk];
       tmem_ld_chunk(dt + c, v);
+      sas[lane] = sc.sa;
+      if (c + 2 * kChunk < w.n) sc.sa = row_scale(w, c + 2 * kChunk);
+      __syncwarp();
       tmem_wait_ld();
       uint8_t* sw = stg + buf * kTStagingBytes;
       if (GATED) {
         // two rows at a time: the low lanes take the first, the high lanes the second
-        uint8_t* at = sw + local * sizeof(T) + (lane >> 4) * kPitch;
+        uint8_t* at = sw + local * sizeof(T) + (lane >> 4) * kRow;
 #pragma unroll
         for (int j = 0; j < kChunk; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(sa + c + j);
+          const float4 s4 = *reinterpret_cast<const float4*>(sas + j);
           const float s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
-            const float z0 = __int2float_rn(static_cast<int>(v[j + q])) * s[q] * sb;
-            const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sb;
+            const float z0 = __int2float_rn(static_cast<int>(v[j + q])) * s[q] * sc.sb;
+            const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sc.sb;
             const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
             const float gate = lane < 16 ? z0 : got, up = lane < 16 ? got : z1;
-            *reinterpret_cast<T*>(at + (j + q) * kPitch) = out_cast<T>(silu_fast(gate) * up);
+            *reinterpret_cast<T*>(at + (j + q) * kRow) = out_cast<T>(silu_fast(gate) * up);
           }
         }
       } else {
         uint8_t* at = sw + local * sizeof(T);
 #pragma unroll
         for (int j = 0; j < kChunk; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(sa + c + j);
+          const float4 s4 = *reinterpret_cast<const float4*>(sas + j);
           const float s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<T*>(at + (j + q) * kPitch) =
-                out_cast<T>(fmaf(__int2float_rn(static_cast<int>(v[j + q])) * s[q], sb, bias));
+            *reinterpret_cast<T*>(at + (j + q) * kRow) =
+                out_cast<T>(fmaf(__int2float_rn(static_cast<int>(v[j + q])) * s[q], sc.sb, sc.bias));
         }
       }
-      // The other buffer's readers are past the last barrier, so one per chunk is enough.
-      named_bar_sync(1 + half, 128);
+      // One barrier a chunk: it also ends the reads of the scales and, as the
+      // buffers alternate, of the chunk before.
+      __syncwarp();
       const int rows = min(kChunk, w.n - c);
       uint8_t* o = reinterpret_cast<uint8_t*>(out) + (w.row + c) * pitch + static_cast<int64_t>(ch0) * sizeof(T);
       if (wide) {
 #pragma unroll
-        for (int i = 0; i < kChunk * kPieces / 128; ++i) {
-          const int x = htid + 128 * i, r = x / kPieces, piece = x % kPieces;
+        for (int i = 0; i < kChunk * kPieces / 32; ++i) {
+          const int x = lane + 32 * i, r = x / kPieces, piece = x % kPieces;
           if (r < rows && piece * 16 < row_bytes)
-            *reinterpret_cast<uint4*>(o + r * pitch + piece * 16) = lds128(smem_u32(sw + r * kPitch + piece * 16));
+            *reinterpret_cast<uint4*>(o + r * pitch + piece * 16) = lds128(smem_u32(sw + r * kRow + piece * 16));
         }
       } else {
-        for (int x = htid; x < kChunk * kChannels; x += 128) {
+        for (int x = lane; x < kChunk * kChannels; x += 32) {
           const int r = x / kChannels, q = x % kChannels * static_cast<int>(sizeof(T));
           if (r < rows && q < row_bytes)
-            *reinterpret_cast<T*>(o + r * pitch + q) = *reinterpret_cast<const T*>(sw + r * kPitch + q);
+            *reinterpret_cast<T*>(o + r * pitch + q) = *reinterpret_cast<const T*>(sw + r * kRow + q);
         }
       }
       buf ^= 1;
@@ -458,18 +506,20 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
       db = 0;
       dph ^= 1u;
     }
+    w = after;
+    sc = nsc;
   }
 }
 
 template <int NT, bool PAIR, bool GATED, typename T>
-__global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap ta,
-                                                            const __grid_constant__ CUtensorMap tb, const Int8Args a) {
+__global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constant__ Maps maps,
+                                                            const __grid_constant__ Int8Args a) {
   extern __shared__ uint8_t smem_raw[];
   using R = Ring<NT, PAIR>;
   const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (stages - smem_u32(smem_raw));
   uint8_t* staging = aligned + R::kStages * R::kBytes;
-  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(staging + 4 * kTStagingBytes);
+  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(staging + 2 * kTEpiWarps * kTStagingBytes);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < R::kStages; ++i) {
@@ -490,7 +540,13 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
     const int lo = a.offsets ? min(max(a.offsets[e], 0), a.P) : e * a.P;
     if (e < a.E) {
       const int hi = a.offsets ? min(max(a.offsets[e + 1], 0), a.P) : a.P;
-      cb.pre[e + 1] = (max(hi - lo, 0) + NT - 1) / NT;
+      const int n = max(hi - lo, 0), tiles = (n + NT - 1) / NT;
+      // an even share of the group's rows, so that its last tile has no mere
+      // rest; a multiple of the MMA's N, and no tile is empty
+      constexpr int kUnit = PAIR ? 32 : 16;
+      const int share = tiles > 0 ? ((n + tiles - 1) / tiles + kUnit - 1) / kUnit * kUnit : NT;
+      cb.rows[e] = static_cast<uint16_t>(share);
+      cb.pre[e + 1] = (n + share - 1) / share;
     } else {
       cb.routed = lo;
     }
@@ -518,7 +574,7 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = cb.tmem;
   if (warp == kTEpiWarps) {
-    if ((threadIdx.x & 31) == 0) tile_producer<NT, PAIR, GATED>(&ta, &tb, a, cb, stages);
+    if ((threadIdx.x & 31) == 0) tile_producer<NT, PAIR, GATED>(maps, a, cb, stages);
   } else if (warp == kTEpiWarps + 1) {
     if ((threadIdx.x & 31) == 0 && (!PAIR || cta_rank() == 0)) tile_mma<NT, PAIR>(a, cb, stages, tmem);
   } else {
@@ -589,19 +645,34 @@ EncodeTiled encode_fn() {
   return fn;
 }
 
+int encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  EncodeTiled fn = encode_fn();
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? MTP_OK
+             : MTP_ERR_CUDA;
+}
+
 // [rows, K] int8 with a row stride, in boxes of box_rows x 128 bytes.
 int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int K, int64_t stride, int box_rows) {
-  EncodeTiled fn = encode_fn();
-  if (!fn) return MTP_ERR_CUDA;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
   const cuuint32_t box[2] = {kTK, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t step[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-             ? MTP_OK
-             : MTP_ERR_CUDA;
+  return encode(map, 2, base, dims, strides, box);
+}
+
+// [E, 2, I, K] gate and up rows in one box of four blocks of 16 gate channels
+// and their 16 up channels. I a multiple of 16.
+int encode_gated(CUtensorMap* map, const void* base, int E, int I, int K, int64_t stride) {
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(K), 16, 2, static_cast<cuuint64_t>(I / 16),
+                              static_cast<cuuint64_t>(E)};
+  const cuuint64_t s = static_cast<cuuint64_t>(stride);
+  const cuuint64_t strides[4] = {s, s * I, s * 16, s * 2 * I};
+  const cuuint32_t box[5] = {kTK, 16, 2, 4, 1};
+  return encode(map, 5, base, dims, strides, box);
 }
 
 int device_sms() {
@@ -653,13 +724,18 @@ int run_tiles(Int8Args& a, const void* ap, int64_t a_stride, const void* bp, int
     if (slots < 1) return MTP_ERR_CUDA;
     configured_device = dev;
   }
-  CUtensorMap ta, tb;
-  int rc = encode_rows(&ta, ap, a.P, a.K, a_stride, kTBox);
-  if (rc == MTP_OK) rc = encode_rows(&tb, bp, static_cast<int64_t>(a.E) * a.N, a.K, b_stride, GATED ? 16 : kTM);
+  Maps maps;
+  maps.blocks = GATED && a.N % 32 == 0;
+  int rc = encode_rows(&maps.rows, ap, a.P, a.K, a_stride, Ring<NT, PAIR>::kRows);
+  if (rc == MTP_OK) rc = encode_rows(&maps.few, ap, a.P, a.K, a_stride, kTBox);
+  if (rc == MTP_OK)
+    rc = maps.blocks ? encode_gated(&maps.weights, bp, a.E, a.N / 2, a.K, b_stride)
+                     : encode_rows(&maps.weights, bp, static_cast<int64_t>(a.E) * a.N, a.K, b_stride, GATED ? 16 : kTM);
   if (rc != MTP_OK) return rc;
   const int channels = (GATED ? 64 : kTM) * (PAIR ? 2 : 1), width = GATED ? a.N / 2 : a.N;
   a.ctiles = (width + channels - 1) / channels;
-  // row tiles: at most one partial one per group that has rows
+  // row tiles: at most one that is not full per group that has rows, and the
+  // even shares add none
   const int64_t blocks = a.P / NT + std::min(a.P, a.E);
   const int64_t grid = std::min<int64_t>(slots, std::max<int64_t>(blocks * a.ctiles, 1)) * (PAIR ? 2 : 1);
   cudaLaunchAttribute attr[2];
@@ -675,7 +751,7 @@ int run_tiles(Int8Args& a, const void* ap, int64_t a_stride, const void* bp, int
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, a) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
     cudaGetLastError();
     return MTP_ERR_LAUNCH;
   }
