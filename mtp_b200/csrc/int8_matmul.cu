@@ -15,8 +15,8 @@
 //             against 98;
 //   warp 9    one thread issues tcgen05.mma kind::i8 (K = 32) into one of two
 //             accumulators of NT columns in tensor memory;
-//   warps 0-7 epilogue: each warp takes its 32 channels of every other chunk of
-//             rows on its own: tensor memory -> scales -> its own staging rows
+//   warps 0-7 epilogue: each warp takes its 32 channels of every other 32 rows on
+//             its own: tensor memory -> scales -> its own staging rows
 //             in shared memory -> 16 bytes a thread to the output, while the
 //             next tile's products run and the next scales are on their way.
 // PAIR: two CTAs of a cluster take 256 channels together (cta_group::2): each
@@ -36,12 +36,14 @@ namespace {
 
 constexpr int kTK = 128;            // K of a stage: one 128-byte swizzle row of int8
 constexpr int kTM = 128;            // channels of a CTA's tile
-constexpr int kTEpiWarps = 8;
+constexpr int kTEpiWarps = 8;    // two for each quarter of the tensor-memory lanes
+constexpr int kTParts = kTEpiWarps / 4;
 constexpr int kTThreads = (kTEpiWarps + 2) * 32;
 constexpr int kTMaxGroups = 1024;
+constexpr int kTBlocks = 1024;      // row tiles whose group is looked up once per CTA
 constexpr int kTBox = 32;           // rows of a small TMA box
 constexpr uint32_t kTWBytes = kTM * kTK;
-constexpr uint32_t kTStagingBytes = 2048;  // one chunk of output rows of an epilogue warp; two per warp
+constexpr uint32_t kTStagingBytes = 2048;  // one chunk of output rows of an epilogue warp
 constexpr uint64_t kTTimeoutNs = 2000000000ull;
 constexpr uint32_t kTIdesc = (2u << 4) | (1u << 7) | (1u << 10);  // D s32, A and B s8
 
@@ -62,13 +64,14 @@ struct alignas(16) TileCtrl {
   int first[kTMaxGroups + 1];     // first row of each group
   uint16_t rows[kTMaxGroups];     // rows of a tile of each group
   alignas(16) float sa[kTEpiWarps][32];  // row scales of a warp's chunk
+  int2 blocks[kTBlocks];          // the first row tiles: row, rows | group << 16
 };
-constexpr uint32_t kTCtrl = 11776;
+constexpr uint32_t kTCtrl = 20480;
 static_assert(sizeof(TileCtrl) <= kTCtrl, "control block");
 
 template <int NT, bool PAIR>
 constexpr size_t tile_smem() {
-  return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + 2 * kTEpiWarps * kTStagingBytes + kTCtrl;
+  return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + kTEpiWarps * kTStagingBytes + kTCtrl;
 }
 static_assert(tile_smem<256, true>() <= 227 * 1024 && tile_smem<128, false>() <= 227 * 1024 &&
                   tile_smem<64, false>() <= 227 * 1024 && tile_smem<32, false>() <= 227 * 1024,
@@ -167,8 +170,10 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
+// Relaxed: a release would wait for the thread's output stores (1000 cycles or
+// more), and what the arrival reports, reads of tensor memory, has completed.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -227,48 +232,74 @@ struct Tile {
   int e, row, n, ct;
 };
 
+// The first group at or after e whose row tiles end past blk.
+__device__ __forceinline__ int group_of(const TileCtrl& cb, int groups, int blk, int e) {
+  int hi = groups - 1;
+  while (e < hi) {
+    const int mid = (e + hi) >> 1;
+    if (cb.pre[mid + 1] > blk)
+      hi = mid;
+    else
+      e = mid + 1;
+  }
+  return e;
+}
+
+__device__ __forceinline__ int2 block_at(const TileCtrl& cb, int blk, int e) {
+  const int row = cb.first[e] + (blk - cb.pre[e]) * cb.rows[e];
+  return make_int2(row, min(static_cast<int>(cb.rows[e]), cb.first[e + 1] - row) | e << 16);
+}
+
+// The tiles of a CTA: channel tiles of a row tile next to each other, so that
+// the CTAs of a moment share rows and weights in L2. Stepped without a
+// division: what every role does per tile is on its critical path.
 template <int NT, bool PAIR>
 struct Walk {
   const TileCtrl& cb;
-  int groups, ctiles, ntiles, t, step, rank, e = 0;
+  int groups, ctiles, blocks, blk, ct, dblk, dct, rank;
   __device__ __forceinline__ Walk(const Int8Args& a, const TileCtrl& c)
-      : cb(c), groups(a.E), ctiles(a.ctiles), ntiles(c.pre[a.E] * a.ctiles) {
+      : cb(c), groups(a.E), ctiles(a.ctiles), blocks(c.pre[a.E]) {
     rank = PAIR ? static_cast<int>(cta_rank()) : 0;
-    t = PAIR ? blockIdx.x / 2 : blockIdx.x;
-    step = PAIR ? gridDim.x / 2 : gridDim.x;
+    const int t = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
+    blk = t / ctiles;
+    ct = t - blk * ctiles;
+    dblk = step / ctiles;
+    dct = step - dblk * ctiles;
   }
   __device__ __forceinline__ bool next(Tile& r) {
-    if (t >= ntiles) return false;
-    const int blk = t / ctiles;
-    r.ct = t - blk * ctiles;
-    if (PAIR) r.ct = 2 * r.ct + rank;
-    // first group whose tiles end past blk; tiles ascend, so the last one's
-    // group is a lower bound
-    int hi = groups - 1;
-    while (e < hi) {
-      const int mid = (e + hi) >> 1;
-      if (cb.pre[mid + 1] > blk)
-        hi = mid;
-      else
-        e = mid + 1;
+    if (blk >= blocks) return false;
+    const int2 b = blk < kTBlocks ? cb.blocks[blk] : block_at(cb, blk, group_of(cb, groups, blk, 0));
+    r.row = b.x;
+    r.n = b.y & 0xffff;
+    r.e = b.y >> 16;
+    r.ct = PAIR ? 2 * ct + rank : ct;
+    blk += dblk;
+    ct += dct;
+    if (ct >= ctiles) {
+      ct -= ctiles;
+      ++blk;
     }
-    r.e = e;
-    const int rows = cb.rows[e];
-    r.row = cb.first[e] + (blk - cb.pre[e]) * rows;
-    r.n = min(rows, cb.first[e + 1] - r.row);
-    t += step;
     return true;
   }
 };
 
-template <typename T>
-__device__ __forceinline__ T out_cast(float v);
-template <>
-__device__ __forceinline__ float out_cast(float v) { return v; }
-template <>
-__device__ __forceinline__ __half out_cast(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 out_cast(float v) { return __float2bfloat16_rn(v); }
+// Two values of neighbouring rows at p and p + pitch bytes. Conversions to 16
+// bits go in pairs: one at a time they run at 16 a cycle and SM, which alone
+// would take as long as a tile's products.
+__device__ __forceinline__ void put2(uint8_t* p, int pitch, float a, float b, float) {
+  *reinterpret_cast<float*>(p) = a;
+  *reinterpret_cast<float*>(p + pitch) = b;
+}
+__device__ __forceinline__ void put2(uint8_t* p, int pitch, float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  *reinterpret_cast<__half*>(p) = __low2half(v);
+  *reinterpret_cast<__half*>(p + pitch) = __high2half(v);
+}
+__device__ __forceinline__ void put2(uint8_t* p, int pitch, float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  *reinterpret_cast<__nv_bfloat16*>(p) = __low2bfloat16(v);
+  *reinterpret_cast<__nv_bfloat16*>(p + pitch) = __high2bfloat16(v);
+}
 
 // Tensor maps: rows of a in boxes of a ring's rows and of kTBox, weights.
 struct Maps {
@@ -388,11 +419,12 @@ template <int NT, bool PAIR, bool GATED, typename T>
 __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging, uint32_t tmem) {
   constexpr int kChannels = GATED ? 16 : 32;                // output channels of a warp
   constexpr int kRow = kChannels * sizeof(T);               // bytes of a staged row
-  constexpr int kChunk = 64 / sizeof(T);                    // rows of a chunk
+  constexpr int kChunk = 64 / sizeof(T);                    // rows staged together
+  constexpr int kUnits = (NT + 32 * kTParts - 1) / (32 * kTParts);  // units of 32 rows of a warp in a tile
   constexpr int kPieces = kRow / 16;
   static_assert(kChunk * kRow <= static_cast<int>(kTStagingBytes), "staging");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quad = warp & 3, half = warp >> 2;
+  const int quad = warp & 3, part = warp >> 2;
   const int width = GATED ? a.N / 2 : a.N;  // columns of the output
   T* out = static_cast<T*>(a.out);
   if (cb.routed < a.P)
@@ -400,30 +432,31 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
               reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width));
   const int64_t pitch = static_cast<int64_t>(width) * sizeof(T);
   const bool wide = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  uint8_t* stg = staging + warp * 2 * kTStagingBytes;
+  uint8_t* sw = staging + warp * kTStagingBytes;
   float* sas = cb.sa[warp];
   const uint32_t dbar = PAIR ? in_leader(smem_u32(&cb.dempty[0])) : smem_u32(&cb.dempty[0]);
   const int local = GATED ? lane & 15 : lane;  // channel of the warp's
-  // scales of a tile: this lane's channel (gated: of its gate or up row), its row of the warp's first chunk
+  // scales of a tile: this lane's channel (gated: of its gate or up row) and its row of each of the warp's units
   struct Scales {
-    float sb, bias, sa;
+    float sb, bias, sa[kUnits];
   };
   auto first_channel = [&](const Tile& w) { return w.ct * 4 * kChannels + quad * kChannels; };
-  auto row_scale = [&](const Tile& w, int c) {
-    return lane < kChunk && c + lane < w.n ? a.a_scale[w.row + c + lane] : 0.f;
-  };
   auto load = [&](const Tile& w) {
     const int ch = first_channel(w) + local;
     const bool in = ch < width;
     Scales r;
     r.sb = in ? a.b_scale[static_cast<int64_t>(w.e) * a.N + ch + (GATED && lane >= 16 ? a.N / 2 : 0)] : 0.f;
     r.bias = in && a.bias ? a.bias[ch] : 0.f;
-    r.sa = row_scale(w, kChunk * half);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int row = 32 * (part + kTParts * u) + lane;
+      r.sa[u] = row < w.n ? a.a_scale[w.row + row] : 0.f;
+    }
     return r;
   };
   Waits wait(a);
   Walk<NT, PAIR> walk(a, cb);
-  int db = 0, buf = 0;
+  int db = 0;
   uint32_t dph = 0;
   Tile w, after;
   bool more = walk.next(w);
@@ -437,70 +470,83 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
     const uint32_t dt = tmem + (static_cast<uint32_t>(32 * quad) << 16) + db * NT;
     const int ch0 = first_channel(w);
     const int row_bytes = min(kChannels, width - ch0) * static_cast<int>(sizeof(T));
-    for (int c = kChunk * half; c < w.n; c += 2 * kChunk) {
-      uint32_t v[kChunk];
-      tmem_ld_chunk(dt + c, v);
-      sas[lane] = sc.sa;
-      if (c + 2 * kChunk < w.n) sc.sa = row_scale(w, c + 2 * kChunk);
+    // The accumulator is free when a warp has read its last rows of it.
+    auto release = [&] {
+      tc_fence_before();
       __syncwarp();
-      tmem_wait_ld();
-      uint8_t* sw = stg + buf * kTStagingBytes;
-      if (GATED) {
-        // two rows at a time: the low lanes take the first, the high lanes the second
-        uint8_t* at = sw + local * sizeof(T) + (lane >> 4) * kRow;
+      if (lane == 0) {
+        if (PAIR)
+          mbar_arrive_cluster(dbar + 8 * db);
+        else
+          mbar_arrive(dbar + 8 * db);
+      }
+    };
+    if (32 * part >= w.n) release();
+#pragma unroll 1
+    for (int u = 0, c = 32 * part; c < w.n; ++u) {
+      sas[lane] = sc.sa[0];
 #pragma unroll
-        for (int j = 0; j < kChunk; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(sas + j);
-          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+      for (int x = 0; x + 1 < kUnits; ++x) sc.sa[x] = sc.sa[x + 1];
+      const int unit = c;
+      c += 32 * kTParts;
 #pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            const float z0 = __int2float_rn(static_cast<int>(v[j + q])) * s[q] * sc.sb;
-            const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sc.sb;
-            const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
-            const float gate = lane < 16 ? z0 : got, up = lane < 16 ? got : z1;
-            *reinterpret_cast<T*>(at + (j + q) * kRow) = out_cast<T>(silu_fast(gate) * up);
+      for (int h = 0; h < 32; h += kChunk) {
+        if (unit + h >= w.n) break;
+        uint32_t v[kChunk];
+        tmem_ld_chunk(dt + unit + h, v);
+        __syncwarp();  // the scales are there, and the last chunk's staged rows are read
+        tmem_wait_ld();
+        if (c >= w.n && (h + kChunk == 32 || unit + h + kChunk >= w.n)) release();
+        if (GATED) {
+          // two rows at a time: the low lanes take the first, the high lanes the second
+          uint8_t* at = sw + local * sizeof(T) + (lane >> 4) * kRow;
+#pragma unroll
+          for (int j = 0; j < kChunk; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(sas + h + j);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+            float o[2];
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              const float z0 = __int2float_rn(static_cast<int>(v[j + q])) * s[q] * sc.sb;
+              const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sc.sb;
+              const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
+              const float gate = lane < 16 ? z0 : got, up = lane < 16 ? got : z1;
+              o[q / 2] = silu_fast(gate) * up;
+            }
+            put2(at + j * kRow, 2 * kRow, o[0], o[1], T());
+          }
+        } else {
+          uint8_t* at = sw + local * sizeof(T);
+#pragma unroll
+          for (int j = 0; j < kChunk; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(sas + h + j);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+            float z[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              z[q] = fmaf(__int2float_rn(static_cast<int>(v[j + q])) * s[q], sc.sb, sc.bias);
+            put2(at + j * kRow, kRow, z[0], z[1], T());
+            put2(at + (j + 2) * kRow, kRow, z[2], z[3], T());
           }
         }
-      } else {
-        uint8_t* at = sw + local * sizeof(T);
+        __syncwarp();  // the rows are staged, and the scales are read
+        const int rows = min(kChunk, w.n - unit - h);
+        uint8_t* o = reinterpret_cast<uint8_t*>(out) + (w.row + unit + h) * pitch + static_cast<int64_t>(ch0) * sizeof(T);
+        if (wide) {
 #pragma unroll
-        for (int j = 0; j < kChunk; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(sas + j);
-          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<T*>(at + (j + q) * kRow) =
-                out_cast<T>(fmaf(__int2float_rn(static_cast<int>(v[j + q])) * s[q], sc.sb, sc.bias));
+          for (int i = 0; i < kChunk * kPieces / 32; ++i) {
+            const int x = lane + 32 * i, r = x / kPieces, piece = x % kPieces;
+            if (r < rows && piece * 16 < row_bytes)
+              *reinterpret_cast<uint4*>(o + r * pitch + piece * 16) = lds128(smem_u32(sw + r * kRow + piece * 16));
+          }
+        } else {
+          for (int x = lane; x < kChunk * kChannels; x += 32) {
+            const int r = x / kChannels, q = x % kChannels * static_cast<int>(sizeof(T));
+            if (r < rows && q < row_bytes)
+              *reinterpret_cast<T*>(o + r * pitch + q) = *reinterpret_cast<const T*>(sw + r * kRow + q);
+          }
         }
       }
-      // One barrier a chunk: it also ends the reads of the scales and, as the
-      // buffers alternate, of the chunk before.
-      __syncwarp();
-      const int rows = min(kChunk, w.n - c);
-      uint8_t* o = reinterpret_cast<uint8_t*>(out) + (w.row + c) * pitch + static_cast<int64_t>(ch0) * sizeof(T);
-      if (wide) {
-#pragma unroll
-        for (int i = 0; i < kChunk * kPieces / 32; ++i) {
-          const int x = lane + 32 * i, r = x / kPieces, piece = x % kPieces;
-          if (r < rows && piece * 16 < row_bytes)
-            *reinterpret_cast<uint4*>(o + r * pitch + piece * 16) = lds128(smem_u32(sw + r * kRow + piece * 16));
-        }
-      } else {
-        for (int x = lane; x < kChunk * kChannels; x += 32) {
-          const int r = x / kChannels, q = x % kChannels * static_cast<int>(sizeof(T));
-          if (r < rows && q < row_bytes)
-            *reinterpret_cast<T*>(o + r * pitch + q) = *reinterpret_cast<const T*>(sw + r * kRow + q);
-        }
-      }
-      buf ^= 1;
-    }
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) {
-      if (PAIR)
-        mbar_arrive_cluster(dbar + 8 * db);
-      else
-        mbar_arrive(dbar + 8 * db);
     }
     if (++db == 2) {
       db = 0;
@@ -519,7 +565,7 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
   const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (stages - smem_u32(smem_raw));
   uint8_t* staging = aligned + R::kStages * R::kBytes;
-  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(staging + 2 * kTEpiWarps * kTStagingBytes);
+  TileCtrl& cb = *reinterpret_cast<TileCtrl*>(staging + kTEpiWarps * kTStagingBytes);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < R::kStages; ++i) {
@@ -568,6 +614,9 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
     }
     if (lane == 0) cb.pre[0] = 0;
   }
+  __syncthreads();
+  for (int b = threadIdx.x; b < min(cb.pre[a.E], kTBlocks); b += kTThreads)
+    cb.blocks[b] = block_at(cb, b, group_of(cb, a.E, b, 0));
   tc_fence_before();
   if (PAIR) cluster_sync();
   __syncthreads();
