@@ -193,6 +193,22 @@ def call(name: str, *args) -> None:
         raise MtpError(name, status, msg)
 
 
+class Entry:
+    """One entry point, resolved at its first call: for calls so short that
+    looking the function up each time would show."""
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = getattr(load(), self.name)
+        status = fn(*args)
+        if status:
+            raise MtpError(self.name, status, load().mtp_status_string(status).decode())
+
+
 def expert_layout(hidden: int, inter: int, group_size: int) -> MtpExpertLayout:
     out = MtpExpertLayout()
     call("mtp_w4a16_expert_layout", hidden, inter, group_size, C.byref(out))

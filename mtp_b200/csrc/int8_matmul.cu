@@ -724,18 +724,6 @@ int encode_gated(CUtensorMap* map, const void* base, int E, int I, int K, int64_
   return encode(map, 5, base, dims, strides, box);
 }
 
-int device_sms() {
-  static int sms[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (!sms[dev]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    sms[dev] = n;
-  }
-  return sms[dev];
-}
-
 // Clusters of two CTAs that the device holds at once.
 template <typename F>
 int pair_slots(F* kernel, size_t smem, int sms) {
@@ -839,7 +827,7 @@ int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* 
 
 int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, const void* bp,
                        int64_t b_stride, cudaStream_t st) {
-  const int sms = device_sms();
+  const int sms = device_sm_count();
   if (!sms) return MTP_ERR_CUDA;
   // Rows of a tile: enough for the average group, fewer while the tiles do not
   // fill the SMs.

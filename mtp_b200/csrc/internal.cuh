@@ -133,6 +133,19 @@ struct PrefillWs {
 PrefillWs prefill_ws(int M, int E, int k, int H, int I, int has_shared);
 int launch_moe_prefill(PrefillArgs& a, int renorm, const float* logits, cudaStream_t st);
 
+// SMs of the current device (0 when it cannot be asked).
+inline int device_sm_count() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
 // Token sort and unsort (token_sort.cu). Strides and row sizes in bytes.
 struct SortArgs {
   int M, k, E, E_map, numel;

@@ -219,27 +219,52 @@ __global__ void __launch_bounds__(256) sort_copy_kernel(const SortArgs a) {
 // ---------------------------------------------------------------------------
 // unsort
 // ---------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-
+// N values of a row as fp32 and back. Conversions to 16 bits go in pairs: one
+// at a time they run at 16 a cycle and SM, below what HBM delivers.
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
+template <int N>
+__device__ __forceinline__ void to_floats(const Vec<float, N>& x, float* f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) f[n] = x.v[n];
+}
+template <int N>
+__device__ __forceinline__ void to_floats(const Vec<__half, N>& x, float* f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) f[n] = __half2float(x.v[n]);
+}
+template <int N>
+__device__ __forceinline__ void to_floats(const Vec<__nv_bfloat16, N>& x, float* f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) f[n] = __bfloat162float(x.v[n]);
+}
+template <int N>
+__device__ __forceinline__ void from_floats(const float* f, Vec<float, N>& x) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x.v[n] = f[n];
+}
+template <int N>
+__device__ __forceinline__ void from_floats(const float* f, Vec<__half, N>& x) {
+#pragma unroll
+  for (int n = 0; n + 1 < N; n += 2) {
+    const __half2 h = __floats2half2_rn(f[n], f[n + 1]);
+    x.v[n] = __low2half(h);
+    x.v[n + 1] = __high2half(h);
+  }
+  if (N % 2) x.v[N - 1] = __float2half_rn(f[N - 1]);
+}
+template <int N>
+__device__ __forceinline__ void from_floats(const float* f, Vec<__nv_bfloat16, N>& x) {
+#pragma unroll
+  for (int n = 0; n + 1 < N; n += 2) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[n], f[n + 1]);
+    x.v[n] = __low2bfloat16(h);
+    x.v[n + 1] = __high2bfloat16(h);
+  }
+  if (N % 2) x.v[N - 1] = __float2bfloat16_rn(f[N - 1]);
+}
 
 constexpr int kSlots = 8;  // slots whose rows a thread has in flight together
 
@@ -271,13 +296,15 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < kSlots; ++j)
-        if (here[j])
+        if (here[j]) {
+          float f[N];
+          to_floats(v[j], f);
 #pragma unroll
-          for (int n = 0; n < N; ++n) acc[n] = fmaf(w[j], to_f<T>(v[j].v[n]), acc[n]);
+          for (int n = 0; n < N; ++n) acc[n] = fmaf(w[j], f[n], acc[n]);
+        }
     }
     V o;
-#pragma unroll
-    for (int n = 0; n < N; ++n) o.v[n] = from_f<T>(acc[n]);
+    from_floats(acc, o);
     *reinterpret_cast<V*>(out + c) = o;
   }
 }
@@ -309,7 +336,8 @@ __global__ void __launch_bounds__(256) unsort_backward_kernel(const UnsortArgs a
     }
     if (in)
       for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
-        const V gv = *reinterpret_cast<const V*>(g + c);
+        float gf[N];
+        to_floats(*reinterpret_cast<const V*>(g + c), gf);
         V v[kSlots];
         if (a.grad_weights) {
 #pragma unroll
@@ -318,18 +346,23 @@ __global__ void __launch_bounds__(256) unsort_backward_kernel(const UnsortArgs a
               v[j] = *reinterpret_cast<const V*>(rows + static_cast<int64_t>(p[j]) * a.H + c);
 #pragma unroll
           for (int j = 0; j < kSlots; ++j)
-            if (p[j] >= 0 && p[j] < a.num_rows)
+            if (p[j] >= 0 && p[j] < a.num_rows) {
+              float f[N];
+              to_floats(v[j], f);
 #pragma unroll
-              for (int n = 0; n < N; ++n) dot[j] = fmaf(to_f<T>(gv.v[n]), to_f<T>(v[j].v[n]), dot[j]);
+              for (int n = 0; n < N; ++n) dot[j] = fmaf(gf[n], f[n], dot[j]);
+            }
         }
         if (grows)
 #pragma unroll
           for (int j = 0; j < kSlots; ++j) {
             const int r = p[j] >= 0 ? p[j] : ~p[j];
             if (r >= a.num_rows) continue;
-            V o;
+            float f[N];
 #pragma unroll
-            for (int n = 0; n < N; ++n) o.v[n] = from_f<T>(p[j] >= 0 ? w[j] * to_f<T>(gv.v[n]) : 0.f);
+            for (int n = 0; n < N; ++n) f[n] = p[j] >= 0 ? w[j] * gf[n] : 0.f;
+            V o;
+            from_floats(f, o);
             *reinterpret_cast<V*>(grows + static_cast<int64_t>(r) * a.H + c) = o;
           }
       }
@@ -348,6 +381,201 @@ __global__ void __launch_bounds__(256) unsort_backward_kernel(const UnsortArgs a
       __syncthreads();
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// unsort of large calls: the rows come by bulk copies
+// ---------------------------------------------------------------------------
+// Every warp runs a ring of its own in shared memory: a slot holds one segment
+// (32 * NP pieces of 16 bytes) of a token's k rows, for the gradient also of g.
+// Lane j finds pair j's row and issues its copy, a slot's meta data keeps row
+// and weight until the segment is summed. So the bytes in flight (about 190 KB
+// per SM) depend neither on registers nor on how long a row's position took;
+// with plain loads 8192 tokens x 8 x 2048 bf16 took 76 us forward and 222 us
+// backward.
+constexpr int kBulkWarps = 8;
+constexpr int kBulkRing = 24 * 1024;  // bytes of a warp's ring
+constexpr int kBulkSlots = 8;
+constexpr uint64_t kBulkTimeoutNs = 2000000000ull;
+
+struct BulkCtrl {
+  uint64_t full[kBulkWarps][kBulkSlots];
+  int pos[kBulkWarps][kBulkSlots][32];
+  float weight[kBulkWarps][kBulkSlots][32];
+};
+constexpr size_t kBulkSmem = kBulkWarps * kBulkRing + sizeof(BulkCtrl);
+
+template <typename T, int NP, bool BACKWARD>
+__global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const UnsortArgs a, int slots) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr int kSeg = NP * 512;  // bytes
+  using V = Vec<T, N>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  BulkCtrl& cb = *reinterpret_cast<BulkCtrl*>(smem + kBulkWarps * kBulkRing);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = smem + warp * kBulkRing;
+  const int row_bytes = a.H * static_cast<int>(sizeof(T));
+  const int segs = (row_bytes + kSeg - 1) / kSeg;
+  const int slot_bytes = (a.k + (BACKWARD ? 1 : 0)) * kSeg;
+  if (lane < slots) mbar_init(smem_u32(&cb.full[warp][lane]), 1);
+  fence_mbar_init();
+  __syncwarp();
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warps = gridDim.x * kBulkWarps, first = blockIdx.x * kBulkWarps + warp;
+  // Tasks: forward every segment on its own, backward a token's segments one
+  // after the other (its dot products stay with the warp).
+  struct Task {
+    int t, seg;
+  };
+  const int dt = BACKWARD ? warps : warps / segs, ds = BACKWARD ? 0 : warps % segs;
+  auto advance = [&](Task& q) {
+    if (BACKWARD) {
+      if (++q.seg == segs) {
+        q.seg = 0;
+        q.t += dt;
+      }
+    } else {
+      q.t += dt;
+      q.seg += ds;
+      if (q.seg >= segs) {
+        q.seg -= segs;
+        ++q.t;
+      }
+    }
+  };
+  Task use = BACKWARD ? Task{first, 0} : Task{first / segs, first % segs};
+  Task fetch = use;
+  const uint8_t* rows = static_cast<const uint8_t*>(a.rows);
+  const uint8_t* grad = static_cast<const uint8_t*>(a.grad);
+  int pos = -1;
+  float weight = 0.f;
+  auto load_meta = [&] {  // of the task that is fetched next
+    pos = -1;
+    weight = 1.f;
+    if (fetch.t < a.M && lane < a.k) {
+      const int64_t i = static_cast<int64_t>(fetch.t) * a.k + lane;
+      pos = a.positions[i];
+      if (a.weights) weight = a.weights[i];
+    }
+  };
+  auto issue = [&](int s) {
+    const int at = fetch.seg * kSeg, bytes = min(kSeg, row_bytes - at);
+    const bool here = lane < a.k && pos >= 0 && pos < a.num_rows;
+    const bool rows_too = !BACKWARD || a.grad_weights != nullptr;
+    const uint32_t bar = smem_u32(&cb.full[warp][s]);
+    cb.pos[warp][s][lane] = pos;
+    cb.weight[warp][s][lane] = weight;
+    const int copies = (rows_too ? __popc(__ballot_sync(kFullMask, here)) : 0) + (BACKWARD ? 1 : 0);
+    if (lane == 0) mbar_arrive_expect_tx(bar, copies * bytes);
+    __syncwarp();
+    const uint32_t dst = smem_u32(ring + s * slot_bytes);
+    if (rows_too && here)
+      bulk_g2s(dst + lane * kSeg, rows + static_cast<int64_t>(pos) * row_bytes + at, bytes, bar);
+    if (BACKWARD && lane == 31)
+      bulk_g2s(dst + a.k * kSeg, grad + static_cast<int64_t>(fetch.t) * row_bytes + at, bytes, bar);
+    advance(fetch);
+    load_meta();
+  };
+  load_meta();
+  int filled = 0;
+  for (; filled < slots && fetch.t < a.M; ++filled) issue(filled);
+  int s = 0;
+  uint32_t ph = 0;
+  float dot = 0.f;
+  float poison = 0.f;  // NaN once a wait ran out: the results from there on say so
+  while (use.t < a.M) {
+    if (!mbar_wait(smem_u32(&cb.full[warp][s]), ph, poison == 0.f ? global_timer_ns() + kBulkTimeoutNs : 0))
+      poison = __int_as_float(0x7fffffff);
+    const uint8_t* slot = ring + s * slot_bytes;
+    const int at = use.seg * kSeg, bytes = min(kSeg, row_bytes - at);
+    const int* ps = cb.pos[warp][s];
+    const float* ws = cb.weight[warp][s];
+    if (!BACKWARD) {
+      float acc[NP][N];
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[q][n] = poison;
+#pragma unroll 4
+      for (int j = 0; j < a.k; ++j) {
+        const int p = ps[j];
+        if (p < 0 || p >= a.num_rows) continue;
+        const float w = ws[j];
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          float f[N];
+          to_floats(*reinterpret_cast<const V*>(slot + j * kSeg + (q * 32 + lane) * 16), f);
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[q][n] = fmaf(w, f[n], acc[q][n]);
+        }
+      }
+      uint8_t* out = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(use.t) * row_bytes + at;
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        V o;
+        from_floats(acc[q], o);
+        if ((q * 32 + lane) * 16 < bytes) *reinterpret_cast<V*>(out + (q * 32 + lane) * 16) = o;
+      }
+    } else {
+      float g[NP][N];
+      bool in[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        in[q] = (q * 32 + lane) * 16 < bytes;
+        to_floats(*reinterpret_cast<const V*>(slot + a.k * kSeg + (q * 32 + lane) * 16), g[q]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) g[q][n] += poison;
+      }
+#pragma unroll 2
+      for (int j = 0; j < a.k; ++j) {
+        const int p = ps[j], r = p >= 0 ? p : ~p;
+        if (r >= a.num_rows) continue;
+        const float w = ws[j];
+        if (a.grad_weights && p >= 0) {
+          float d = 0.f;
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            float f[N];
+            to_floats(*reinterpret_cast<const V*>(slot + j * kSeg + (q * 32 + lane) * 16), f);
+#pragma unroll
+            for (int n = 0; n < N; ++n) d = in[q] ? fmaf(g[q][n], f[n], d) : d;
+          }
+          d = warp_sum(d);
+          if (lane == j) dot += d;
+        }
+        if (a.grad_rows) {
+          uint8_t* out = static_cast<uint8_t*>(a.grad_rows) + static_cast<int64_t>(r) * row_bytes + at;
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            float f[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) f[n] = p >= 0 ? w * g[q][n] : 0.f;
+            V o;
+            from_floats(f, o);
+            if (in[q]) *reinterpret_cast<V*>(out + (q * 32 + lane) * 16) = o;
+          }
+        }
+      }
+      if (use.seg == segs - 1) {
+        if (a.grad_weights && lane < a.k) a.grad_weights[static_cast<int64_t>(use.t) * a.k + lane] = dot;
+        dot = 0.f;
+      }
+    }
+    __syncwarp();  // the slot is read
+    if (fetch.t < a.M) issue(s);
+    advance(use);
+    if (++s == slots) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+  // after a wait that ran out, copies may still be on their way into this CTA
+  if (poison != 0.f)
+    for (int x = 0; x < filled; ++x, s = s + 1 == slots ? 0 : s + 1) {
+      mbar_wait(smem_u32(&cb.full[warp][s]), ph ^ 1u, global_timer_ns() + kBulkTimeoutNs);
+      if (s + 1 == slots) ph ^= 1u;
+    }
 }
 
 // Threads of a row (a power of two in [least, 256]) and rows of a CTA.
@@ -396,6 +624,21 @@ int sort_run(const SortArgs& a, cudaStream_t st) {
   return launch(sort_copy_kernel<V>, dim3((a.M + block.y - 1) / block.y), block, 0, st, a);
 }
 
+template <typename T, int NP, bool BACKWARD>
+int bulk_run(const UnsortArgs& a, int slots, int sms, cudaStream_t st) {
+  auto* kernel = unsort_bulk_kernel<T, NP, BACKWARD>;
+  static int configured_device = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
+  if (configured_device != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBulkSmem)) !=
+        cudaSuccess)
+      return MTP_ERR_CUDA;
+    configured_device = dev;
+  }
+  return launch(kernel, dim3(sms), dim3(kBulkWarps * 32), kBulkSmem, st, a, slots);
+}
+
 template <typename T>
 int unsort_run(const UnsortArgs& a, bool backward, cudaStream_t st) {
   // the widest vector that every row start and length allows
@@ -404,6 +647,22 @@ int unsort_run(const UnsortArgs& a, bool backward, cudaStream_t st) {
                          reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.grad_rows) |
                          static_cast<uintptr_t>(static_cast<int64_t>(a.H) * sizeof(T));
   const int n = (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
+  // Bulk copies where rows are wide (512 bytes: a segment) and there are tasks
+  // for every warp's ring; a small call is done before a ring would fill.
+  const int64_t row_bytes = static_cast<int64_t>(a.H) * sizeof(T);
+  const int parts = a.k + (backward ? 1 : 0);
+  if (n == kWide && row_bytes >= 512 && row_bytes < (1 << 30) && 2 * parts * 512 <= kBulkRing) {
+    const bool two = 2 * parts * 1024 <= kBulkRing && row_bytes >= 1024;
+    const int seg = two ? 1024 : 512;
+    const int sms = device_sm_count();
+    if (!sms) return MTP_ERR_CUDA;
+    const int64_t tasks = backward ? a.M : a.M * ((row_bytes + seg - 1) / seg);
+    if (tasks >= 2ll * sms * kBulkWarps) {
+      const int slots = std::min(kBulkSlots, kBulkRing / (parts * seg));
+      if (backward) return two ? bulk_run<T, 2, true>(a, slots, sms, st) : bulk_run<T, 1, true>(a, slots, sms, st);
+      return two ? bulk_run<T, 2, false>(a, slots, sms, st) : bulk_run<T, 1, false>(a, slots, sms, st);
+    }
+  }
   const dim3 block = row_block((a.H + n - 1) / n, backward ? 32 : 8);
   const dim3 grid((a.M + block.y - 1) / block.y);
   auto pick = [&](auto* wide, auto* pair, auto* one) { return n == kWide ? wide : n == kPair ? pair : one; };

@@ -33,8 +33,15 @@ MAX_K = 131071  # 128 * 128 * K stays below 2^31
 _SILU_MUL = 1
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_sort_entry = _lib.Entry("mtp_sort_tokens")
+_unsort_entry = _lib.Entry("mtp_unsort_tokens")
+_unsort_backward_entry = _lib.Entry("mtp_unsort_tokens_backward")
+_quantize_entry = _lib.Entry("mtp_quantize_int8")
+_matmul_entry = _lib.Entry("mtp_int8_matmul")
+_layer_entry = _lib.Entry("mtp_w8a8_moe_layer")
+
+# The handle of the current stream of a device (torch.cuda.current_stream builds a Stream object around it).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None, contiguous: bool = True):
@@ -47,7 +54,7 @@ def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None,
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
-    if t.dim() != ndim:
+    if t.ndim != ndim:
         raise ValueError(f"{name} must be {ndim}-D, got shape {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -90,25 +97,26 @@ class SortedTokens(NamedTuple):
 
 def _sort(x, ids, num_experts, expert_map, row_scales):
     m, k = ids.shape
-    dev, h = x.device, x.shape[1]
-    rows = torch.empty((m * k, h), dtype=x.dtype, device=dev)
-    positions = torch.empty((m, k), dtype=torch.int32, device=dev)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    scales = None if row_scales is None else torch.empty(m * k, dtype=torch.float32, device=dev)
-    _lib.call("mtp_sort_tokens", x.data_ptr() or None, _row_stride("hidden_states", x), DTYPES.get(x.dtype, _INT8), m, h,
+    h = x.shape[1]
+    rows = x.new_empty((m * k, h))
+    positions = torch.empty_like(ids)
+    offsets = ids.new_empty(num_experts + 1)
+    scales = None if row_scales is None else row_scales.new_empty(m * k)
+    _sort_entry(x.data_ptr() or None, _row_stride("hidden_states", x), DTYPES.get(x.dtype, _INT8), m, h,
               ids.data_ptr(), k, num_experts, None if expert_map is None else expert_map.data_ptr(),
               0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
               rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(),
-              offsets.data_ptr(), _stream(dev))
+              offsets.data_ptr(), _stream(x.get_device()))
     return rows, positions, offsets, scales
 
 
 def _unsort(rows, positions, weights):
     m, k = positions.shape
-    out = torch.empty((m, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    _lib.call("mtp_unsort_tokens", rows.data_ptr(), rows.shape[0], DTYPES[rows.dtype], positions.data_ptr(),
-              None if weights is None else weights.data_ptr(), m, k, rows.shape[1], out.data_ptr(),
-              _stream(rows.device))
+    r, h = rows.shape
+    out = rows.new_empty((m, h))
+    _unsort_entry(rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
+                  None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr(),
+                  _stream(rows.get_device()))
     return out
 
 
@@ -117,6 +125,7 @@ class _SortTokens(torch.autograd.Function):
     def forward(ctx, x, ids, num_experts, expert_map, row_scales):
         rows, positions, offsets, scales = _sort(x, ids, num_experts, expert_map, row_scales)
         ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(positions, offsets, *([] if scales is None else [scales]))
         return rows, positions, offsets, scales
 
@@ -124,6 +133,8 @@ class _SortTokens(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_rows, *_):
         (positions,) = ctx.saved_tensors
+        if grad_rows is None:
+            return None, None, None, None, None
         return _unsort(grad_rows.contiguous(), positions, None), None, None, None, None
 
 
@@ -141,13 +152,13 @@ class _UnsortTokens(torch.autograd.Function):
         grad = grad.contiguous()
         (m, k), h = positions.shape, grad.shape[1]
         need_rows, _, need_weights = ctx.needs_input_grad
-        grad_rows = torch.empty((ctx.num_rows, h), dtype=grad.dtype, device=grad.device) if need_rows else None
+        grad_rows = grad.new_empty((ctx.num_rows, h)) if need_rows else None
         grad_weights = torch.empty_like(weights) if need_weights else None
-        _lib.call("mtp_unsort_tokens_backward", grad.data_ptr(), None if rows is None else rows.data_ptr(),
-                  ctx.num_rows, DTYPES[grad.dtype], positions.data_ptr(),
-                  None if weights is None else weights.data_ptr(), m, k, h,
-                  None if grad_rows is None else grad_rows.data_ptr(),
-                  None if grad_weights is None else grad_weights.data_ptr(), _stream(grad.device))
+        _unsort_backward_entry(grad.data_ptr(), None if rows is None else rows.data_ptr(), ctx.num_rows,
+                               DTYPES[grad.dtype], positions.data_ptr(),
+                               None if weights is None else weights.data_ptr(), m, k, h,
+                               None if grad_rows is None else grad_rows.data_ptr(),
+                               None if grad_weights is None else grad_weights.data_ptr(), _stream(grad.get_device()))
         return grad_rows, None, grad_weights
 
 
@@ -223,11 +234,12 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     if k < 1:
         raise ValueError("x must have at least one column")
-    codes = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    _lib.call("mtp_quantize_int8", x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(),
-              codes.shape[1], scale.data_ptr(), _stream(x.device))
-    return codes[:, :k], scale
+    kp = (k + 15) // 16 * 16
+    codes = x.new_empty((m, kp), dtype=torch.int8)
+    scale = x.new_empty(m, dtype=torch.float32)
+    _quantize_entry(x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(), kp, scale.data_ptr(),
+                    _stream(x.get_device()))
+    return codes if kp == k else codes[:, :k], scale
 
 
 @lru_cache(maxsize=4096)
@@ -241,21 +253,20 @@ def _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, a_off, b_off) -> in
 
 
 def _product(a, a_scale, b, b_scale, bias, offsets, out_dtype, activation, status):
-    dev = a.device
     rows, k = a.shape
     n, groups = b.shape[-2], b.shape[0] if b.dim() == 3 else 1
-    out = torch.empty((rows, n // 2 if activation else n), dtype=out_dtype, device=dev)
+    out = a.new_empty((rows, n // 2 if activation else n), dtype=out_dtype)
     a_dtype, a_stride = DTYPES.get(a.dtype, _INT8), _row_stride("a", a)
     ap, bp = a.data_ptr(), b.data_ptr()
     size = _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, ap & 255, bp & 255)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    ws = b.new_empty(size) if size else None
     args = _lib.MtpInt8MatmulArgs(rows, n, k, groups, a_dtype, DTYPES[out_dtype], activation, 0, ap, a_stride,
                                   None if a_scale is None else a_scale.data_ptr(), bp, b_scale.data_ptr(),
                                   None if bias is None else bias.data_ptr(),
                                   None if offsets is None else offsets.data_ptr(), out.data_ptr(),
                                   None if status is None else status.data_ptr(),
                                   None if ws is None else ws.data_ptr(), size)
-    _lib.call("mtp_int8_matmul", C.byref(args), _stream(dev))
+    _matmul_entry(C.byref(args), _stream(a.get_device()))
     return out
 
 
@@ -421,7 +432,7 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
     given = router_logits is None
     dtype, p13, p2 = DTYPES[hidden_states.dtype], w13.data_ptr(), w2.data_ptr()
     size = _layer_workspace(m, h, i, e, top_k, dtype, not given, p13 & 255, p2 & 255)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = w13.new_empty(size)
     args = _lib.MtpW8A8LayerArgs(m, h, i, e, top_k, 1 if renormalize else 0, dtype,
                                  0 if expert_map is None else expert_map.numel(), hidden_states.data_ptr(),
                                  None if given else router_logits.data_ptr(),
@@ -429,5 +440,5 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
                                  None if expert_map is None else expert_map.data_ptr(), p13, w13_scale.data_ptr(), p2,
                                  w2_scale.data_ptr(), out.data_ptr(), None if status is None else status.data_ptr(),
                                  ws.data_ptr(), size)
-    _lib.call("mtp_w8a8_moe_layer", C.byref(args), _stream(dev))
+    _layer_entry(C.byref(args), _stream(hidden_states.get_device()))
     return out

@@ -132,7 +132,21 @@ def slots(positions):
 
 CASES = [(1, 8, 2048, 256, 0.0), (1, 1, 1, 1, 0.0), (5, 3, 31, 7, 0.5), (64, 8, 2048, 256, 0.0),
          (33, 9, 100, 12, 0.3), (17, 32, 130, 64, 0.2), (700, 6, 1000, 60, 0.6), (2000, 8, 512, 256, 0.0),
-         (9, 2, 5003, 4, 0.2), (50, 4, 64, 8, 1.0)]
+         (9, 2, 5003, 4, 0.2), (50, 4, 64, 8, 1.0),
+         # sizes that stream: one and two pieces a segment, short last segments, most slots and one more
+         (3000, 8, 2048, 256, 0.1), (2500, 11, 1000, 60, 0.3), (5000, 2, 520, 16, 0.0), (2600, 1, 256, 4, 0.5),
+         (2400, 12, 512, 32, 0.2), (2400, 22, 264, 64, 0.4), (2400, 23, 512, 64, 0.4), (2500, 5, 4104, 8, 0.2)]
+
+
+def test_only_one_gradient(cuda_device):
+    """Rows alone or weights alone, small and streamed: the same bits as both together."""
+    for m in (40, 3000):
+        pkg, positions, rows, w, grad = weighted(m, 8, 1024, 32, torch.bfloat16, 0.2, m, cuda_device)
+        both = torch.autograd.grad(pkg.unsort_tokens(rows.requires_grad_(), positions, w.requires_grad_()), (rows, w), grad)
+        rows, w = rows.detach(), w.detach()
+        r, v = rows.clone().requires_grad_(), w.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(pkg.unsort_tokens(r, positions, w), r, grad)[0], both[0])
+        assert torch.equal(torch.autograd.grad(pkg.unsort_tokens(rows, positions, v), v, grad)[0], both[1])
 
 
 @pytest.mark.parametrize("m,k,h,e,none", CASES)
