@@ -25,7 +25,7 @@
 // Gated tiles hold 16 gate channels, then their 16 up
 // channels, four times, so that a gate and its up value lie 16 lanes apart in
 // one warp.
-#include "internal.cuh"
+#include "int8_common.cuh"
 
 #include <cuda.h>
 
@@ -39,8 +39,6 @@ constexpr int kTM = 128;            // channels of a CTA's tile
 constexpr int kTEpiWarps = 8;    // two for each quarter of the tensor-memory lanes
 constexpr int kTParts = kTEpiWarps / 4;
 constexpr int kTThreads = (kTEpiWarps + 2) * 32;
-constexpr int kTMaxGroups = 1024;
-constexpr int kTBlocks = 1024;      // row tiles whose group is looked up once per CTA
 constexpr int kTBox = 32;           // rows of a small TMA box
 constexpr uint32_t kTWBytes = kTM * kTK;
 constexpr uint32_t kTStagingBytes = 2048;  // one chunk of output rows of an epilogue warp
@@ -59,12 +57,8 @@ struct alignas(16) TileCtrl {
   uint64_t full[8], empty[8];     // stage landed / consumed
   uint64_t dfull[2], dempty[2];   // accumulator complete / read
   uint32_t tmem;
-  int routed;                     // rows before offsets[E]
-  int pre[kTMaxGroups + 1];       // row tiles before each group
-  int first[kTMaxGroups + 1];     // first row of each group
-  uint16_t rows[kTMaxGroups];     // rows of a tile of each group
   alignas(16) float sa[kTEpiWarps][32];  // row scales of a warp's chunk
-  int2 blocks[kTBlocks];          // the first row tiles: row, rows | group << 16
+  RowBlocks rows;
 };
 constexpr uint32_t kTCtrl = 20480;
 static_assert(sizeof(TileCtrl) <= kTCtrl, "control block");
@@ -207,6 +201,29 @@ __device__ __forceinline__ uint64_t desc_swizzle128(uint32_t addr) {
          (1ull << 46) | (2ull << 61);
 }
 
+// One lane of a converged warp. The producer and MMA warps run their loops
+// with all lanes, so that addresses and descriptors stay in uniform registers,
+// and let the elected lane issue: with the whole loop inside one lane's branch
+// a stage took its thread 400 cycles, nearly as long as its products.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity) {
+  return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+}
+template <bool CLUSTER>
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity) {
+  const uint64_t deadline = global_timer_ns() + kTTimeoutNs;
+  do {
+    if (mbar_done<CLUSTER>(bar, parity)) return true;
+  } while (global_timer_ns() < deadline);
+  return false;
+}
+
 // A wait of at most kTTimeoutNs. After one that ran out (recorded in the
 // caller's status) this thread's waits only look once, so the kernel runs to
 // its end.
@@ -216,14 +233,11 @@ struct Waits {
   __device__ __forceinline__ explicit Waits(const Int8Args& a) : status(a.status) {}
   template <bool CLUSTER = false>  // CLUSTER: arrivals of the other CTA of the pair
   __device__ __forceinline__ void on(uint32_t bar, uint32_t parity) {
-    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-    if (done() || out) return;
-    const uint64_t deadline = global_timer_ns() + kTTimeoutNs;
-    do {
-      if (done()) return;
-    } while (global_timer_ns() < deadline);
-    out = true;
-    if (status) atomicOr(status, 1);
+    if (mbar_done<CLUSTER>(bar, parity) || out) return;
+    if (!mbar_wait_long<CLUSTER>(bar, parity)) {
+      out = true;
+      if (status) atomicOr(status, 1);
+    }
   }
 };
 
@@ -232,33 +246,15 @@ struct Tile {
   int e, row, n, ct;
 };
 
-// The first group at or after e whose row tiles end past blk.
-__device__ __forceinline__ int group_of(const TileCtrl& cb, int groups, int blk, int e) {
-  int hi = groups - 1;
-  while (e < hi) {
-    const int mid = (e + hi) >> 1;
-    if (cb.pre[mid + 1] > blk)
-      hi = mid;
-    else
-      e = mid + 1;
-  }
-  return e;
-}
-
-__device__ __forceinline__ int2 block_at(const TileCtrl& cb, int blk, int e) {
-  const int row = cb.first[e] + (blk - cb.pre[e]) * cb.rows[e];
-  return make_int2(row, min(static_cast<int>(cb.rows[e]), cb.first[e + 1] - row) | e << 16);
-}
-
 // The tiles of a CTA: channel tiles of a row tile next to each other, so that
 // the CTAs of a moment share rows and weights in L2. Stepped without a
 // division: what every role does per tile is on its critical path.
 template <int NT, bool PAIR>
 struct Walk {
-  const TileCtrl& cb;
+  const RowBlocks& rb;
   int groups, ctiles, blocks, blk, ct, dblk, dct, rank;
   __device__ __forceinline__ Walk(const Int8Args& a, const TileCtrl& c)
-      : cb(c), groups(a.E), ctiles(a.ctiles), blocks(c.pre[a.E]) {
+      : rb(c.rows), groups(a.E), ctiles(a.ctiles), blocks(c.rows.pre[a.E]) {
     rank = PAIR ? static_cast<int>(cta_rank()) : 0;
     const int t = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
     blk = t / ctiles;
@@ -268,10 +264,10 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(Tile& r) {
     if (blk >= blocks) return false;
-    const int2 b = blk < kTBlocks ? cb.blocks[blk] : block_at(cb, blk, group_of(cb, groups, blk, 0));
-    r.row = b.x;
-    r.n = b.y & 0xffff;
-    r.e = b.y >> 16;
+    const RowBlock b = rb.at(blk, groups);
+    r.row = b.row;
+    r.n = b.n;
+    r.e = b.e;
     r.ct = PAIR ? 2 * ct + rank : ct;
     blk += dblk;
     ct += dct;
@@ -328,27 +324,30 @@ __device__ void tile_producer(const Maps& m, const Int8Args& a, TileCtrl& cb, ui
       wait.on(smem_u32(&cb.empty[st]), ph ^ 1u);
       const uint32_t sb = stages + st * R::kBytes;
       uint32_t bar = smem_u32(&cb.full[st]);
-      if (PAIR) {
-        // both CTAs' bytes arrive on the first one's barrier
-        if (walk.rank == 0) mbar_arrive_expect_tx(bar, 2 * bytes);
-        bar = in_leader(bar);
-      } else {
-        mbar_arrive_expect_tx(bar, bytes);
-      }
-      if (!GATED) {
-        tma_2d<PAIR>(sb, &m.weights, s * kTK, ch, bar);
-      } else if (m.blocks) {
-        tma_5d<PAIR>(sb, &m.weights, s * kTK, w.ct * 4, w.e, bar);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tma_2d<PAIR>(sb + q * 4096, &m.weights, s * kTK, ch + 16 * q, bar);
-          tma_2d<PAIR>(sb + q * 4096 + 2048, &m.weights, s * kTK, ch + a.N / 2 + 16 * q, bar);
+      if (elect_one()) {
+        if (PAIR) {
+          // both CTAs' bytes arrive on the first one's barrier
+          if (walk.rank == 0) mbar_arrive_expect_tx(bar, 2 * bytes);
+          bar = in_leader(bar);
+        } else {
+          mbar_arrive_expect_tx(bar, bytes);
         }
+        if (!GATED) {
+          tma_2d<PAIR>(sb, &m.weights, s * kTK, ch, bar);
+        } else if (m.blocks) {
+          tma_5d<PAIR>(sb, &m.weights, s * kTK, w.ct * 4, w.e, bar);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tma_2d<PAIR>(sb + q * 4096, &m.weights, s * kTK, ch + 16 * q, bar);
+            tma_2d<PAIR>(sb + q * 4096 + 2048, &m.weights, s * kTK, ch + a.N / 2 + 16 * q, bar);
+          }
+        }
+        if (!boxes) tma_2d<PAIR>(sb + kTWBytes, &m.rows, s * kTK, row, bar);
+        for (int q = 0; q < boxes; ++q)
+          tma_2d<PAIR>(sb + kTWBytes + q * (kTBox * kTK), &m.few, s * kTK, row + q * kTBox, bar);
       }
-      if (!boxes) tma_2d<PAIR>(sb + kTWBytes, &m.rows, s * kTK, row, bar);
-      for (int q = 0; q < boxes; ++q)
-        tma_2d<PAIR>(sb + kTWBytes + q * (kTBox * kTK), &m.few, s * kTK, row + q * kTBox, bar);
+      __syncwarp();
       ++issued;
       if (++st == R::kStages) {
         st = 0;
@@ -383,36 +382,24 @@ __device__ void tile_mma(const Int8Args& a, TileCtrl& cb, uint32_t stages, uint3
       tc_fence_after();
       const uint64_t wd = desc_swizzle128(stages + st * R::kBytes);
       const uint64_t xd = desc_swizzle128(stages + st * R::kBytes + kTWBytes);
+      if (elect_one()) {
 #pragma unroll
-      for (int j = 0; j < kTK / 32; ++j) umma_i8_ss<PAIR>(d, wd + 2 * j, xd + 2 * j, idesc, (s | j) != 0);
-      tile_commit<PAIR>(smem_u32(&cb.empty[st]));
+        for (int j = 0; j < kTK / 32; ++j) umma_i8_ss<PAIR>(d, wd + 2 * j, xd + 2 * j, idesc, (s | j) != 0);
+        tile_commit<PAIR>(smem_u32(&cb.empty[st]));
+      }
+      __syncwarp();
       if (++st == R::kStages) {
         st = 0;
         ph ^= 1u;
       }
     }
-    tile_commit<PAIR>(smem_u32(&cb.dfull[db]));
+    if (elect_one()) tile_commit<PAIR>(smem_u32(&cb.dfull[db]));
+    __syncwarp();
     if (++db == 2) {
       db = 0;
       dph ^= 1u;
     }
   }
-}
-
-// Rows behind the last group's are zero: the bytes [from, to) of the output,
-// shared out over all epilogue threads of the grid.
-__device__ __forceinline__ void zero_tail(uint8_t* from, uint8_t* to) {
-  const int64_t tid = static_cast<int64_t>(blockIdx.x) * (kTEpiWarps * 32) + threadIdx.x;
-  const int64_t all = static_cast<int64_t>(gridDim.x) * (kTEpiWarps * 32);
-  uint8_t* lo = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(from) + 15) & ~static_cast<uintptr_t>(15));
-  uint8_t* hi = reinterpret_cast<uint8_t*>(reinterpret_cast<uintptr_t>(to) & ~static_cast<uintptr_t>(15));
-  if (lo >= hi) {
-    for (int64_t i = tid; i < to - from; i += all) from[i] = 0;
-    return;
-  }
-  for (int64_t i = tid; i < (hi - lo) / 16; i += all) reinterpret_cast<uint4*>(lo)[i] = make_uint4(0, 0, 0, 0);
-  if (tid < lo - from) from[tid] = 0;
-  if (tid < to - hi) hi[tid] = 0;
 }
 
 template <int NT, bool PAIR, bool GATED, typename T>
@@ -427,9 +414,9 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
   const int quad = warp & 3, part = warp >> 2;
   const int width = GATED ? a.N / 2 : a.N;  // columns of the output
   T* out = static_cast<T*>(a.out);
-  if (cb.routed < a.P)
-    zero_tail(reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.routed) * width),
-              reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width));
+  if (cb.rows.routed < a.P)
+    zero_tail(reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.rows.routed) * width),
+              reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width), kTEpiWarps * 32);
   const int64_t pitch = static_cast<int64_t>(width) * sizeof(T);
   const bool wide = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   uint8_t* sw = staging + warp * kTStagingBytes;
@@ -581,51 +568,16 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
   if (warp == kTEpiWarps + 1) tile_tmem_alloc<PAIR>(smem_u32(&cb.tmem), 2 * NT);
   pdl_launch_dependents();
   pdl_wait();
-  // first row and row tiles of every group, then the tiles' running sum
-  for (int e = threadIdx.x; e <= a.E; e += kTThreads) {
-    const int lo = a.offsets ? min(max(a.offsets[e], 0), a.P) : e * a.P;
-    if (e < a.E) {
-      const int hi = a.offsets ? min(max(a.offsets[e + 1], 0), a.P) : a.P;
-      const int n = max(hi - lo, 0), tiles = (n + NT - 1) / NT;
-      // an even share of the group's rows, so that its last tile has no mere
-      // rest; a multiple of the MMA's N, and no tile is empty
-      constexpr int kUnit = PAIR ? 32 : 16;
-      const int share = tiles > 0 ? ((n + tiles - 1) / tiles + kUnit - 1) / kUnit * kUnit : NT;
-      cb.rows[e] = static_cast<uint16_t>(share);
-      cb.pre[e + 1] = (n + share - 1) / share;
-    } else {
-      cb.routed = lo;
-    }
-    cb.first[e] = lo;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const int lane = threadIdx.x;
-    int run = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 32) {
-      int x = e0 + lane < a.E ? cb.pre[e0 + lane + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(kFullMask, x, o);
-        if (lane >= o) x += y;
-      }
-      if (e0 + lane < a.E) cb.pre[e0 + lane + 1] = run + x;
-      run += __shfl_sync(kFullMask, x, 31);
-    }
-    if (lane == 0) cb.pre[0] = 0;
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < min(cb.pre[a.E], kTBlocks); b += kTThreads)
-    cb.blocks[b] = block_at(cb, b, group_of(cb, a.E, b, 0));
+  build_row_blocks(a, cb.rows, NT, PAIR ? 32 : 16, kTThreads);
   tc_fence_before();
   if (PAIR) cluster_sync();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = cb.tmem;
   if (warp == kTEpiWarps) {
-    if ((threadIdx.x & 31) == 0) tile_producer<NT, PAIR, GATED>(maps, a, cb, stages);
+    tile_producer<NT, PAIR, GATED>(maps, a, cb, stages);
   } else if (warp == kTEpiWarps + 1) {
-    if ((threadIdx.x & 31) == 0 && (!PAIR || cta_rank() == 0)) tile_mma<NT, PAIR>(a, cb, stages, tmem);
+    if (!PAIR || cta_rank() == 0) tile_mma<NT, PAIR>(a, cb, stages, tmem);
   } else {
     tile_epilogue<NT, PAIR, GATED, T>(a, cb, staging, tmem);
   }
@@ -640,7 +592,8 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
 }
 
 // ---------------------------------------------------------------------------
-// rows into a layout that TMA takes (16-byte aligned base and stride)
+// rows into a layout that TMA and 16-byte loads take (aligned base and stride),
+// zeros behind each row
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict__ src, int64_t stride, int64_t rows,
                                                        int K, int8_t* __restrict__ dst, int64_t dst_stride) {
@@ -648,7 +601,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict_
   pdl_wait();
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows;
        r += static_cast<int64_t>(gridDim.x) * 8)
-    for (int c = (threadIdx.x & 31) * 4; c < K; c += 128) {
+    for (int c = (threadIdx.x & 31) * 4; c < dst_stride; c += 128) {
       uint32_t w = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
@@ -825,10 +778,12 @@ int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* 
                 stride, rows, K, static_cast<int8_t*>(dst), dst_stride);
 }
 
-int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, const void* bp,
-                       int64_t b_stride, cudaStream_t st) {
+int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, bool a_padded,
+                       const void* bp, int64_t b_stride, cudaStream_t st) {
   const int sms = device_sm_count();
   if (!sms) return MTP_ERR_CUDA;
+  if (!a.offsets && !gated && int8_stream_takes(a.P) && (a.K % 16 == 0 || a_padded))
+    return launch_int8_stream(a, out_dtype, ap, a_stride, bp, b_stride, st);
   // Rows of a tile: enough for the average group, fewer while the tiles do not
   // fill the SMs.
   const int per_group = (a.P + a.E - 1) / a.E, width = gated ? a.N / 2 : a.N;

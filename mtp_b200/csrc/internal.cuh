@@ -191,7 +191,16 @@ struct Int8Args {
 bool tma_rows_ok(const void* base, int64_t stride);
 int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* dst, int64_t dst_stride,
                     cudaStream_t st);
-int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, const void* bp,
-                       int64_t b_stride, cudaStream_t st);
+// a_padded: ap is a workspace whose rows may be read up to a multiple of 16.
+int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, bool a_padded,
+                       const void* bp, int64_t b_stride, cudaStream_t st);
+// A few rows of one group (int8_stream.cu), given as codes or quantised in the
+// same kernel.
+bool int8_stream_takes(int rows);
+int launch_int8_stream(Int8Args a, int out_dtype, const void* ap, int64_t a_stride, const void* bp, int64_t b_stride,
+                       cudaStream_t st);
+bool int8_stream_quantises(int rows, int K);
+int launch_int8_stream_quantise(Int8Args a, int out_dtype, const void* x, int64_t x_stride, int x_dtype, const void* bp,
+                                int64_t b_stride, cudaStream_t st);
 
 }  // namespace mtp

@@ -135,7 +135,11 @@ inline size_t rank_smem(int E) { return static_cast<size_t>(kRankWarps + 2) * (E
 // Every warp of the cluster takes one contiguous range of the pairs and walks
 // it twice: first it counts its pairs of every key, then, with the counts of
 // the ranges before its own summed (over the warps of the CTA in shared memory,
-// over the CTAs through distributed shared memory), it numbers them.
+// over the CTAs through distributed shared memory), it numbers them. Up to
+// kRankKeys rounds of 32 keys are loaded together and kept for the second walk
+// (one load after the other made 65536 pairs take 23 us instead of 11).
+constexpr int kRankKeys = 16;
+
 __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads, 1) sort_rank_kernel(const SortArgs a) {
   extern __shared__ int sm[];
   __shared__ int scan_tmp[32];
@@ -153,12 +157,24 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
   const int64_t begin = (static_cast<int64_t>(cta) * kRankWarps + warp) * span;
   const int64_t end = min(begin + span, static_cast<int64_t>(a.numel));
   int* mine = wcnt + warp * bins;
-  for (int64_t c = begin; c < end; c += 32) {
-    const int64_t i = c + lane;
-    const int key = i < end ? sort_key(a, static_cast<int>(i)) : -1;
-    const unsigned same = __match_any_sync(kFullMask, key);
-    if (key >= 0 && lane == __ffs(same) - 1) mine[key] += __popc(same);
-    __syncwarp();
+  int key[kRankKeys];
+  auto load = [&](int64_t c) {
+#pragma unroll
+    for (int r = 0; r < kRankKeys; ++r) {
+      const int64_t i = c + r * 32 + lane;
+      key[r] = i < end ? sort_key(a, static_cast<int>(i)) : -1;
+    }
+  };
+  constexpr int64_t kBatch = kRankKeys * 32;
+  for (int64_t c = begin; c < end; c += kBatch) {
+    load(c);
+#pragma unroll
+    for (int r = 0; r < kRankKeys; ++r) {
+      if (c + r * 32 >= end) break;
+      const unsigned same = __match_any_sync(kFullMask, key[r]);
+      if (key[r] >= 0 && lane == __ffs(same) - 1) mine[key[r]] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   for (int b = tid; b < bins; b += kRankThreads) {
@@ -191,18 +207,21 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
     base[a.E] = routed + unrouted;
   }
   cluster_sync_all();  // also: no CTA leaves while another reads its counts
-  for (int64_t c = begin; c < end; c += 32) {
-    const int64_t i = c + lane;
-    const int key = i < end ? sort_key(a, static_cast<int>(i)) : -1;
-    const unsigned same = __match_any_sync(kFullMask, key);
-    int p = 0;
-    if (key >= 0) p = base[key] + mine[key] + __popc(same & ((1u << lane) - 1u));
-    __syncwarp();
-    if (key >= 0) {
-      a.positions[i] = key < a.E ? p : ~p;
-      if (lane == __ffs(same) - 1) mine[key] += __popc(same);
+  for (int64_t c = begin; c < end; c += kBatch) {
+    if (span > kBatch) load(c);
+#pragma unroll
+    for (int r = 0; r < kRankKeys; ++r) {
+      if (c + r * 32 >= end) break;
+      const unsigned same = __match_any_sync(kFullMask, key[r]);
+      int p = 0;
+      if (key[r] >= 0) p = base[key[r]] + mine[key[r]] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (key[r] >= 0) {
+        a.positions[c + r * 32 + lane] = key[r] < a.E ? p : ~p;
+        if (lane == __ffs(same) - 1) mine[key[r]] += __popc(same);
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 

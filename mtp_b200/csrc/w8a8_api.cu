@@ -23,6 +23,7 @@ constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31
 struct MatmulWs {
   int64_t codes, scales, b, total;  // -1: not needed
   int64_t kp;
+  bool fused;  // quantised by the product kernel
 };
 
 int matmul_shapes(const MtpInt8MatmulArgs& a) {
@@ -41,8 +42,10 @@ MatmulWs matmul_ws(const MtpInt8MatmulArgs& a) {
   Carver c;
   w.kp = round_up(a.k, 16);
   w.codes = w.scales = w.b = -1;
-  if (a.a_dtype != MTP_DTYPE_INT8 || !tma_rows_ok(a.a, a.rows > 1 ? a.a_stride : 0)) w.codes = c.take(w.kp * a.rows);
-  if (a.a_dtype != MTP_DTYPE_INT8) w.scales = c.take(4ll * a.rows);
+  const bool quantise = a.a_dtype != MTP_DTYPE_INT8;
+  w.fused = quantise && !a.offsets && a.activation == MTP_ACT_NONE && int8_stream_quantises(a.rows, a.k);
+  if (!w.fused && (quantise || !tma_rows_ok(a.a, a.rows > 1 ? a.a_stride : 0))) w.codes = c.take(w.kp * a.rows);
+  if (!w.fused && quantise) w.scales = c.take(4ll * a.rows);
   if (!tma_rows_ok(a.b, a.k)) w.b = c.take(w.kp * a.num_groups * a.n);
   w.total = c.at;
   return w;
@@ -170,7 +173,7 @@ int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream) {
   const void* bp = p.b;
   int64_t a_stride = p.rows > 1 ? p.a_stride : w.kp, b_stride = p.k;
   const float* a_scale = p.a_scale;
-  if (quantise) {
+  if (quantise && !w.fused) {
     int8_t* codes = reinterpret_cast<int8_t*>(ws + w.codes);
     float* scales = reinterpret_cast<float*>(ws + w.scales);
     rc = launch_quantize_int8(p.a, p.a_stride, p.a_dtype, p.rows, p.k, codes, w.kp, scales, st);
@@ -201,7 +204,9 @@ int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream) {
   a.offsets = p.offsets;
   a.out = p.out;
   a.status = p.status;
-  return launch_int8_matmul(a, p.activation == MTP_ACT_SILU_MUL, p.out_dtype, ap, a_stride, bp, b_stride, st);
+  if (w.fused) return launch_int8_stream_quantise(a, p.out_dtype, p.a, p.a_stride, p.a_dtype, bp, b_stride, st);
+  return launch_int8_matmul(a, p.activation == MTP_ACT_SILU_MUL, p.out_dtype, ap, a_stride, w.codes >= 0, bp, b_stride,
+                            st);
 }
 
 }  // extern "C"
@@ -341,7 +346,7 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   g.offsets = i32(w.offsets);
   g.out = f32(w.h);
   g.status = p.status;
-  rc = launch_int8_matmul(g, true, MTP_DTYPE_FP32, ws + w.rows, w.hp, w13, w13_stride, st);
+  rc = launch_int8_matmul(g, true, MTP_DTYPE_FP32, ws + w.rows, w.hp, true, w13, w13_stride, st);
   if (rc != MTP_OK) return rc;
   rc = launch_quantize_int8(f32(w.h), I, MTP_DTYPE_FP32, P, I, reinterpret_cast<int8_t*>(ws + w.hq), w.ip, f32(w.hs),
                             st);
@@ -351,7 +356,7 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   g.a_scale = f32(w.hs);
   g.b_scale = p.w2_scale;
   g.out = ws + w.y;
-  rc = launch_int8_matmul(g, false, p.dtype, ws + w.hq, w.ip, w2, w2_stride, st);
+  rc = launch_int8_matmul(g, false, p.dtype, ws + w.hq, w.ip, true, w2, w2_stride, st);
   if (rc != MTP_OK) return rc;
 
   UnsortArgs u = {};
