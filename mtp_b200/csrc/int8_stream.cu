@@ -26,7 +26,7 @@ namespace {
 constexpr int kSWarps = 8;
 constexpr int kSThreads = kSWarps * 32;
 constexpr int kSRows = 8;
-constexpr int kSteps = 4;              // 128 bytes of K in flight per round and warp
+constexpr int kSteps = 2;              // 128 bytes of K in flight per round and warp
 constexpr int kSRowBytes = 48 * 1024;  // QUANT: most bytes of quantised rows
 
 struct StreamArgs {

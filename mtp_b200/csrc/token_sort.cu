@@ -126,8 +126,20 @@ __device__ __forceinline__ int ld_cluster(uint32_t local, int cta) {
   uint32_t remote;
   int v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(cta));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote));
   return v;
+}
+
+// The lanes whose key (below 2^bits) is this lane's: a vote per bit. match.any
+// gives the same at about 200 cycles a warp, which made it most of this kernel.
+__device__ __forceinline__ unsigned same_key(int key, int bits) {
+  unsigned same = kFullMask;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (key >> b) & 1;
+    const unsigned votes = __ballot_sync(kFullMask, one);
+    same &= one ? votes : ~votes;
+  }
+  return same;
 }
 
 inline size_t rank_smem(int E) { return static_cast<size_t>(kRankWarps + 2) * (E + 1) * sizeof(int); }
@@ -136,8 +148,8 @@ inline size_t rank_smem(int E) { return static_cast<size_t>(kRankWarps + 2) * (E
 // it twice: first it counts its pairs of every key, then, with the counts of
 // the ranges before its own summed (over the warps of the CTA in shared memory,
 // over the CTAs through distributed shared memory), it numbers them. Up to
-// kRankKeys rounds of 32 keys are loaded together and kept for the second walk
-// (one load after the other made 65536 pairs take 23 us instead of 11).
+// kRankKeys rounds of 32 keys are loaded together and kept, with each pair's rank
+// among its round's equal keys, for the second walk.
 constexpr int kRankKeys = 16;
 
 __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads, 1) sort_rank_kernel(const SortArgs a) {
@@ -157,13 +169,20 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
   const int64_t begin = (static_cast<int64_t>(cta) * kRankWarps + warp) * span;
   const int64_t end = min(begin + span, static_cast<int64_t>(a.numel));
   int* mine = wcnt + warp * bins;
-  int key[kRankKeys];
+  const int bits = 32 - __clz(bins);
+  int key[kRankKeys];   // key, then rank << 16 | equal keys << 24
   auto load = [&](int64_t c) {
 #pragma unroll
     for (int r = 0; r < kRankKeys; ++r) {
       const int64_t i = c + r * 32 + lane;
-      key[r] = i < end ? sort_key(a, static_cast<int>(i)) : -1;
+      key[r] = i < end ? sort_key(a, static_cast<int>(i)) : bins;
     }
+#pragma unroll
+    for (int r = 0; r < kRankKeys; ++r)
+      if (c + r * 32 < end) {
+        const unsigned same = same_key(key[r], bits);
+        key[r] |= __popc(same & ((1u << lane) - 1u)) << 16 | __popc(same) << 24;
+      }
   };
   constexpr int64_t kBatch = kRankKeys * 32;
   for (int64_t c = begin; c < end; c += kBatch) {
@@ -171,29 +190,35 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
 #pragma unroll
     for (int r = 0; r < kRankKeys; ++r) {
       if (c + r * 32 >= end) break;
-      const unsigned same = __match_any_sync(kFullMask, key[r]);
-      if (key[r] >= 0 && lane == __ffs(same) - 1) mine[key[r]] += __popc(same);
+      const int k = key[r] & 0xffff;
+      if (k < bins && (key[r] >> 16 & 0xff) == 0) mine[k] += key[r] >> 24;
       __syncwarp();
     }
   }
   __syncthreads();
   for (int b = tid; b < bins; b += kRankThreads) {
-    int run = 0;
+    int v[kRankWarps], run = 0;
+#pragma unroll
+    for (int w = 0; w < kRankWarps; ++w) v[w] = wcnt[w * bins + b];
+#pragma unroll
     for (int w = 0; w < kRankWarps; ++w) {
-      const int v = wcnt[w * bins + b];
       wcnt[w * bins + b] = run;
-      run += v;
+      run += v[w];
     }
     tot[b] = run;
   }
   cluster_sync_all();
   int all = 0, before = 0;
-  if (tid < a.E)
+  if (tid < a.E) {
+    int v[kRankCtas];
+#pragma unroll
+    for (int r = 0; r < kRankCtas; ++r) v[r] = ld_cluster(smem_u32(tot + tid), r);
+#pragma unroll
     for (int r = 0; r < kRankCtas; ++r) {
-      const int v = ld_cluster(smem_u32(tot + tid), r);
-      before += r < cta ? v : 0;
-      all += v;
+      before += r < cta ? v[r] : 0;
+      all += v[r];
     }
+  }
   int routed;
   const int off = block_exclusive_scan(all, &routed, scan_tmp);
   if (tid < a.E) {
@@ -212,13 +237,13 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
 #pragma unroll
     for (int r = 0; r < kRankKeys; ++r) {
       if (c + r * 32 >= end) break;
-      const unsigned same = __match_any_sync(kFullMask, key[r]);
+      const int k = key[r] & 0xffff, rank = key[r] >> 16 & 0xff;
       int p = 0;
-      if (key[r] >= 0) p = base[key[r]] + mine[key[r]] + __popc(same & ((1u << lane) - 1u));
+      if (k < bins) p = base[k] + mine[k] + rank;
       __syncwarp();
-      if (key[r] >= 0) {
-        a.positions[c + r * 32 + lane] = key[r] < a.E ? p : ~p;
-        if (lane == __ffs(same) - 1) mine[key[r]] += __popc(same);
+      if (k < bins) {
+        a.positions[c + r * 32 + lane] = k < a.E ? p : ~p;
+        if (rank == 0) mine[k] += key[r] >> 24;
       }
       __syncwarp();
     }
