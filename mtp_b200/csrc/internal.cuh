@@ -203,4 +203,27 @@ bool int8_stream_quantises(int rows, int K);
 int launch_int8_stream_quantise(Int8Args a, int out_dtype, const void* x, int64_t x_stride, int x_dtype, const void* bp,
                                 int64_t b_stride, cudaStream_t st);
 
+// The W8A8 layer of a few tokens (w8a8_decode.cu). Rows and
+// weights start on 16 bytes.
+struct DecodeArgs {
+  int M, H, I, E, k, renorm, E_map;
+  const void* x;               // [M, H]
+  const float* logits;         // [M, E] or NULL
+  const float* topk_weights;   // [M, k] without logits
+  const int32_t* topk_ids;
+  const int32_t* emap;         // [E_map] or NULL
+  const int8_t* w13;           // [E, 2I, H]
+  const float* s13;
+  const int8_t* w2;            // [E, H, I]
+  const float* s2;
+  float* h;                    // [M * k, I]
+  float* y;                    // [M * k, H]
+  void* out;                   // [M, H]
+  void* lists;                 // w8a8_decode_list_bytes
+  int32_t* done;               // [H / 16] blocks whose strip of y is written
+};
+int64_t w8a8_decode_list_bytes();
+bool w8a8_decode_takes(int M, int H, int I, int E, int k);
+int launch_w8a8_decode(const DecodeArgs& a, int dtype, cudaStream_t st);
+
 }  // namespace mtp

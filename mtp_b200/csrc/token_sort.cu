@@ -449,6 +449,13 @@ struct BulkCtrl {
 };
 constexpr size_t kBulkSmem = kBulkWarps * kBulkRing + sizeof(BulkCtrl);
 
+// The timer is read only where the bytes are not there yet (a read takes longer
+// than many waits).
+__device__ __forceinline__ bool bulk_wait(uint32_t bar, uint32_t parity, bool patient) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return patient && mbar_wait(bar, parity, global_timer_ns() + kBulkTimeoutNs);
+}
+
 template <typename T, int NP, bool BACKWARD>
 __global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const UnsortArgs a, int slots) {
   constexpr int N = 16 / sizeof(T);
@@ -529,8 +536,7 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const U
   float dot = 0.f;
   float poison = 0.f;  // NaN once a wait ran out: the results from there on say so
   while (use.t < a.M) {
-    if (!mbar_wait(smem_u32(&cb.full[warp][s]), ph, poison == 0.f ? global_timer_ns() + kBulkTimeoutNs : 0))
-      poison = __int_as_float(0x7fffffff);
+    if (!bulk_wait(smem_u32(&cb.full[warp][s]), ph, poison == 0.f)) poison = __int_as_float(0x7fffffff);
     const uint8_t* slot = ring + s * slot_bytes;
     const int at = use.seg * kSeg, bytes = min(kSeg, row_bytes - at);
     const int* ps = cb.pos[warp][s];

@@ -214,8 +214,9 @@ int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream) {
 namespace {
 
 struct LayerWs8 {
-  int64_t tw, tid, xq, xs, rows, rs, positions, offsets, h, hq, hs, y, w13, w2, total;
+  int64_t tw, tid, xq, xs, rows, rs, positions, offsets, h, hq, hs, y, w13, w2, lists, done, total;
   int64_t hp, ip;
+  bool decode;  // the kernels for a few tokens
 };
 
 int layer_shapes(const MtpW8A8LayerArgs& a) {
@@ -235,11 +236,21 @@ int layer_shapes(const MtpW8A8LayerArgs& a) {
 }
 
 LayerWs8 layer_ws8(const MtpW8A8LayerArgs& a) {
-  LayerWs8 w;
+  LayerWs8 w = {};
   Carver c;
   const int64_t m = a.num_tokens, p = m * a.top_k;
   w.hp = round_up(a.hidden, 16);
   w.ip = round_up(a.inter, 16);
+  w.decode = w8a8_decode_takes(a.num_tokens, a.hidden, a.inter, a.num_experts, a.top_k) && aligned(a.hidden_states, 16) &&
+             tma_rows_ok(a.w13, a.hidden) && tma_rows_ok(a.w2, a.inter);
+  if (w.decode) {
+    w.h = c.take(4 * p * a.inter);
+    w.y = c.take(4 * p * a.hidden);
+    w.lists = c.take(w8a8_decode_list_bytes());
+    w.done = c.take(4ll * (a.hidden / 16));
+    w.total = c.at;
+    return w;
+  }
   w.tw = c.take(a.router_logits ? 4 * p : 0);
   w.tid = c.take(a.router_logits ? 4 * p : 0);
   w.xq = c.take(m * w.hp);
@@ -289,6 +300,32 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int M = p.num_tokens, H = p.hidden, I = p.inter, E = p.num_experts, k = p.top_k;
   const int P = M * k;
+
+  if (w.decode) {
+    DecodeArgs d = {};
+    d.M = M;
+    d.H = H;
+    d.I = I;
+    d.E = E;
+    d.k = k;
+    d.renorm = p.renormalize ? 1 : 0;
+    d.E_map = p.global_num_experts;
+    d.x = p.hidden_states;
+    d.logits = p.router_logits;
+    d.topk_weights = p.topk_weights;
+    d.topk_ids = p.topk_ids;
+    d.emap = p.expert_map;
+    d.w13 = p.w13;
+    d.s13 = p.w13_scale;
+    d.w2 = p.w2;
+    d.s2 = p.w2_scale;
+    d.h = f32(w.h);
+    d.y = f32(w.y);
+    d.out = p.out;
+    d.lists = ws + w.lists;
+    d.done = i32(w.done);
+    return launch_w8a8_decode(d, p.dtype, st);
+  }
 
   const float* weights = p.topk_weights;
   const int32_t* ids = p.topk_ids;

@@ -366,8 +366,8 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
 # the layer
 # ---------------------------------------------------------------------------
 @lru_cache(maxsize=4096)
-def _layer_workspace(m, h, i, e, k, dtype, logits, w13_off, w2_off) -> int:
-    args = _lib.MtpW8A8LayerArgs(m, h, i, e, k, 0, dtype, 0, None, 256 if logits else None, None, None, None,
+def _layer_workspace(m, h, i, e, k, dtype, logits, x_off, w13_off, w2_off) -> int:
+    args = _lib.MtpW8A8LayerArgs(m, h, i, e, k, 0, dtype, 0, 256 + x_off, 256 if logits else None, None, None, None,
                                  256 + w13_off, None, 256 + w2_off, None, None, None, None, 0)
     out = _lib.i64()
     _lib.call("mtp_w8a8_moe_layer_workspace_size", C.byref(args), C.byref(out))
@@ -430,11 +430,11 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
             raise ValueError(f"out must be {(m, h)}, got {tuple(out.shape)}")
     _check_out(hidden_states.dtype, status, dev)
     given = router_logits is None
-    dtype, p13, p2 = DTYPES[hidden_states.dtype], w13.data_ptr(), w2.data_ptr()
-    size = _layer_workspace(m, h, i, e, top_k, dtype, not given, p13 & 255, p2 & 255)
+    dtype, px, p13, p2 = DTYPES[hidden_states.dtype], hidden_states.data_ptr(), w13.data_ptr(), w2.data_ptr()
+    size = _layer_workspace(m, h, i, e, top_k, dtype, not given, px & 255, p13 & 255, p2 & 255)
     ws = w13.new_empty(size)
     args = _lib.MtpW8A8LayerArgs(m, h, i, e, top_k, 1 if renormalize else 0, dtype,
-                                 0 if expert_map is None else expert_map.numel(), hidden_states.data_ptr(),
+                                 0 if expert_map is None else expert_map.numel(), px,
                                  None if given else router_logits.data_ptr(),
                                  topk_weights.data_ptr() if given else None, topk_ids.data_ptr() if given else None,
                                  None if expert_map is None else expert_map.data_ptr(), p13, w13_scale.data_ptr(), p2,

@@ -327,7 +327,8 @@ def check_layer(out, ref):
 
 @pytest.mark.parametrize("m,e,k,h,i", [(1, 256, 8, 512, 128), (4, 8, 2, 256, 128), (33, 16, 4, 272, 96),
                                        (300, 32, 8, 512, 256), (1025, 8, 3, 128, 64), (50, 5, 2, 100, 30),
-                                       (2, 1024, 8, 64, 48), (7, 1, 1, 48, 16)])
+                                       (2, 1024, 8, 64, 48), (7, 1, 1, 48, 16),
+                                       (8, 64, 32, 256, 64), (1, 4, 2, 2048, 1024), (3, 6, 2, 4096, 16), (6, 300, 4, 80, 528)])
 @pytest.mark.parametrize("dtype", list(U))
 def test_layer_against_its_definition(cuda_device, m, e, k, h, i, dtype):
     import mtp_b200
@@ -340,6 +341,44 @@ def test_layer_against_its_definition(cuda_device, m, e, k, h, i, dtype):
     assert int(status) == 0
     given = mtp_b200.moe_layer_w8a8(c["x"], None, c["w13"], c["s13"], c["w2"], c["s2"], k, topk_weights=w, topk_ids=ids)
     assert torch.equal(given, out)
+
+
+@pytest.mark.parametrize("m", [1, 5, 8, 9, 40])
+def test_layer_with_many_pairs_of_one_expert(cuda_device, m):
+    """Given ids: an expert several times in one token (more than 8 pairs in all), ids of nobody, a token without any."""
+    import mtp_b200
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    c = layer_case(g, m, 5, 160, 48, torch.bfloat16, cuda_device)
+    ids = torch.randint(-1, 6, (m, 7), generator=g, device=cuda_device, dtype=torch.int32)
+    ids[:, :3] = 2
+    ids[m // 2] = -1
+    w = torch.rand(m, 7, generator=g, device=cuda_device) / 7
+    out = mtp_b200.moe_layer_w8a8(c["x"], None, c["w13"], c["s13"], c["w2"], c["s2"], 7, topk_weights=w, topk_ids=ids)
+    check_layer(out, plain_layer(c, w, ids))
+    assert not out[m // 2].any()
+
+
+def test_layer_in_a_graph_and_on_a_side_stream(cuda_device):
+    import mtp_b200
+    for m in (2, 30):
+        g = torch.Generator(device=cuda_device).manual_seed(m)
+        c = layer_case(g, m, 16, 256, 128, torch.bfloat16, cuda_device)
+        call = lambda: mtp_b200.moe_layer_w8a8(c["x"], c["logits"], c["w13"], c["s13"], c["w2"], c["s2"], 4)
+        first = call()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            second = call()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                third = call()
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(first, second)
+        c["x"].mul_(-1)
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(third, want)
 
 
 @pytest.mark.parametrize("m", [3, 400])
