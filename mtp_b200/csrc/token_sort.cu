@@ -134,24 +134,29 @@ __device__ __forceinline__ int ld_cluster(uint32_t local, int cta) {
 // gives the same at about 200 cycles a warp, which made it most of this kernel.
 __device__ __forceinline__ unsigned same_key(int key, int bits) {
   unsigned same = kFullMask;
-  for (int b = 0; b < bits; ++b) {
-    const bool one = (key >> b) & 1;
+#pragma unroll
+  for (int b = 0; b < 11; ++b) {  // keys go up to 1025
+    if (b >= bits) break;
+    const bool one = (key & (1 << b)) != 0;
     const unsigned votes = __ballot_sync(kFullMask, one);
     same &= one ? votes : ~votes;
   }
   return same;
 }
 
-inline size_t rank_smem(int E) { return static_cast<size_t>(kRankWarps + 2) * (E + 1) * sizeof(int); }
+// Keys of a CTA that stay in shared memory between its two walks.
+constexpr int kRankKeep = 16384;
+
+inline size_t rank_smem(int E) {
+  return (static_cast<size_t>(kRankWarps + 2) * (E + 1) + kRankKeep) * sizeof(int);
+}
 
 // Every warp of the cluster takes one contiguous range of the pairs and walks
 // it twice: first it counts its pairs of every key, then, with the counts of
 // the ranges before its own summed (over the warps of the CTA in shared memory,
-// over the CTAs through distributed shared memory), it numbers them. Up to
-// kRankKeys rounds of 32 keys are loaded together and kept, with each pair's rank
-// among its round's equal keys, for the second walk.
-constexpr int kRankKeys = 16;
-
+// over the CTAs through distributed shared memory), it numbers them. The loops
+// stay rolled: a launch this short runs each instruction from a cold cache, and
+// unrolling them by 16 made the first walk 7000 cycles longer.
 __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads, 1) sort_rank_kernel(const SortArgs a) {
   extern __shared__ int sm[];
   __shared__ int scan_tmp[32];
@@ -159,6 +164,7 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
   int* wcnt = sm;                       // [warps][bins]
   int* tot = sm + kRankWarps * bins;    // [bins] this CTA's pairs of every key
   int* base = tot + bins;               // [bins] first row of this CTA's pairs of a key
+  int* kept = base + bins;              // [kRankKeep] key | rank in its round << 16 | equal keys << 24
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   for (int x = tid; x < kRankWarps * bins; x += kRankThreads) wcnt[x] = 0;
   pdl_launch_dependents();
@@ -170,30 +176,29 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
   const int64_t end = min(begin + span, static_cast<int64_t>(a.numel));
   int* mine = wcnt + warp * bins;
   const int bits = 32 - __clz(bins);
-  int key[kRankKeys];   // key, then rank << 16 | equal keys << 24
-  auto load = [&](int64_t c) {
-#pragma unroll
-    for (int r = 0; r < kRankKeys; ++r) {
-      const int64_t i = c + r * 32 + lane;
-      key[r] = i < end ? sort_key(a, static_cast<int>(i)) : bins;
-    }
-#pragma unroll
-    for (int r = 0; r < kRankKeys; ++r)
-      if (c + r * 32 < end) {
-        const unsigned same = same_key(key[r], bits);
-        key[r] |= __popc(same & ((1u << lane) - 1u)) << 16 | __popc(same) << 24;
-      }
+  const bool keep = span * kRankWarps <= kRankKeep;
+  if (keep) {
+    const int64_t first = static_cast<int64_t>(cta) * kRankWarps * span;
+#pragma unroll 4
+    for (int x = tid; x < span * kRankWarps; x += kRankThreads)
+      kept[x] = first + x < a.numel ? sort_key(a, static_cast<int>(first + x)) : bins;
+    __syncthreads();
+  }
+  int* own = kept + warp * static_cast<int>(keep ? span : 0) + lane;
+  // this lane's pair of round r: its key, rank among the round's equal keys, and their number
+  auto ranked = [&](int r) {
+    const int64_t i = begin + r * 32 + lane;
+    const int key = keep ? own[r * 32] : i < end ? sort_key(a, static_cast<int>(i)) : bins;
+    const unsigned same = same_key(key, bits);
+    return key | __popc(same & ((1u << lane) - 1u)) << 16 | __popc(same) << 24;
   };
-  constexpr int64_t kBatch = kRankKeys * 32;
-  for (int64_t c = begin; c < end; c += kBatch) {
-    load(c);
-#pragma unroll
-    for (int r = 0; r < kRankKeys; ++r) {
-      if (c + r * 32 >= end) break;
-      const int k = key[r] & 0xffff;
-      if (k < bins && (key[r] >> 16 & 0xff) == 0) mine[k] += key[r] >> 24;
-      __syncwarp();
-    }
+  const int rounds = static_cast<int>((max(end - begin, static_cast<int64_t>(0)) + 31) / 32);
+#pragma unroll 1
+  for (int r = 0; r < rounds; ++r) {
+    const int x = ranked(r), k = x & 0xffff;
+    if (keep) own[r * 32] = x;
+    if (k < bins && (x >> 16 & 0xff) == 0) mine[k] += x >> 24;
+    __syncwarp();
   }
   __syncthreads();
   for (int b = tid; b < bins; b += kRankThreads) {
@@ -232,21 +237,17 @@ __global__ void __cluster_dims__(kRankCtas, 1, 1) __launch_bounds__(kRankThreads
     base[a.E] = routed + unrouted;
   }
   cluster_sync_all();  // also: no CTA leaves while another reads its counts
-  for (int64_t c = begin; c < end; c += kBatch) {
-    if (span > kBatch) load(c);
-#pragma unroll
-    for (int r = 0; r < kRankKeys; ++r) {
-      if (c + r * 32 >= end) break;
-      const int k = key[r] & 0xffff, rank = key[r] >> 16 & 0xff;
-      int p = 0;
-      if (k < bins) p = base[k] + mine[k] + rank;
-      __syncwarp();
-      if (k < bins) {
-        a.positions[c + r * 32 + lane] = k < a.E ? p : ~p;
-        if (rank == 0) mine[k] += key[r] >> 24;
-      }
-      __syncwarp();
+#pragma unroll 1
+  for (int r = 0; r < rounds; ++r) {
+    const int x = keep ? own[r * 32] : ranked(r), k = x & 0xffff, rank = x >> 16 & 0xff;
+    int p = 0;
+    if (k < bins) p = base[k] + mine[k] + rank;
+    __syncwarp();
+    if (k < bins) {
+      a.positions[begin + r * 32 + lane] = k < a.E ? p : ~p;
+      if (rank == 0) mine[k] += x >> 24;
     }
+    __syncwarp();
   }
 }
 

@@ -62,7 +62,7 @@ def check_sort(x, ids, e, emap=None, scales=None, dev=None):
 
 @pytest.mark.parametrize("m,k,e", [(0, 2, 4), (1, 1, 1), (1, 8, 256), (7, 3, 5), (64, 8, 256), (100, 32, 1024),
                                    (512, 8, 256), (513, 8, 256), (4097, 1, 3), (2048, 8, 1024), (3000, 7, 60),
-                                   (8192, 8, 256), (20000, 8, 64)])
+                                   (8192, 8, 256), (20000, 8, 64), (70000, 4, 17)])
 @pytest.mark.parametrize("none", [0.0, 0.6, 1.0])
 def test_sort_bit_exact(cuda_device, m, k, e, none):
     g = torch.Generator().manual_seed(m * 31 + k + e)
