@@ -6,83 +6,165 @@
 // product with it is NaN rather than a number. Rows below 2^-64 are scaled by
 // 2^64 first, where 127 / max|x| would overflow.
 //
-// HBM-bound: a row is read once into registers (up to kUnits units of 8
-// elements per thread), its maximum is a warp or CTA reduction, and the codes
-// are written 8 bytes at a time. Longer rows read the rest a second time.
+// HBM-bound: a row is read once into registers (as it is stored, up to kUnits
+// pieces of 16 bytes a thread), its maximum is a warp or CTA reduction, and the
+// codes are written 8 (fp32: 4) bytes a thread. Longer rows read the rest a
+// second time. 8192 x 2048 bf16 took 18.7 us with the row kept as fp32 (fewer
+// warps resident) and a conversion per code.
 #include "quantize.cuh"
 
-#include <algorithm>
+#include <type_traits>
 
 namespace mtp {
 namespace {
 
 constexpr int kUnits = 8;
 
-// A row per warp (CTA false) or per CTA of 256 threads.
-template <typename T, bool WIDE, bool CTA>
+// N elements in 16 bytes, as they are stored.
+template <typename T>
+struct Piece {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void floats(float* v) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) {
+        v[i] = __uint_as_float(w[i]);
+      } else if (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t magnitude() const {
+    float v[N];
+    floats(v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ void store(int8_t* q, RowScale r) const {
+    float v[N];
+    floats(v);
+    uint32_t w[2];
+    codes_of<N>(v, r, w);
+    if (N == 8)
+      *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(q) = w[0];
+  }
+};
+
+__device__ __forceinline__ uint32_t cta_max(uint32_t most, uint32_t* red) {
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) most = max(most, red[w]);
+  return most;
+}
+
+// WPR warps a row, 8 / WPR rows a CTA; rows and codes aligned.
+template <typename T, int WPR>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t x_stride, int M, int K,
                                                        int8_t* __restrict__ q, int64_t q_stride,
                                                        float* __restrict__ scale) {
+  using P = Piece<T>;
   __shared__ uint32_t red[8];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t m = CTA ? static_cast<int64_t>(blockIdx.x) : static_cast<int64_t>(blockIdx.x) * 8 + warp;
-  if (m >= M) return;
-  const int first = (CTA ? threadIdx.x : lane) * 8;
-  constexpr int kStep = (CTA ? 256 : 32) * 8;
+  const int64_t m = static_cast<int64_t>(blockIdx.x) * (8 / WPR) + warp / WPR;
+  const int k = m < M ? K : 0;
+  const int first = (warp % WPR * 32 + lane) * P::N;
+  constexpr int kStep = WPR * 32 * P::N;
   const T* row = x + m * x_stride;
   int8_t* out = q + m * q_stride;
-  float v[kUnits][8];
+  P v[kUnits];
   uint32_t most = 0;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u)
-    if (first + u * kStep < K) load_unit<T, WIDE>(row, first + u * kStep, K, v[u]);
+    if (first + u * kStep < k) v[u].load(row + first + u * kStep);
 #pragma unroll
   for (int u = 0; u < kUnits; ++u)
-    if (first + u * kStep < K) most = max(most, magnitude(v[u]));
-  for (int c = first + kUnits * kStep; c < K; c += kStep) {
-    float t[8];
-    load_unit<T, WIDE>(row, c, K, t);
-    most = max(most, magnitude(t));
+    if (first + u * kStep < k) most = max(most, v[u].magnitude());
+  P t;
+  for (int c = first + kUnits * kStep; c < k; c += kStep) {
+    t.load(row + c);
+    most = max(most, t.magnitude());
   }
   most = __reduce_max_sync(kFullMask, most);
-  if (CTA) {
+  if (WPR > 1) {
     if (lane == 0) red[warp] = most;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) most = max(most, red[w]);
+    for (int w = 0; w < WPR; ++w) most = max(most, red[warp / WPR * WPR + w]);
   }
   const RowScale r = row_scale(most);
-  if (first == 0) scale[m] = __fdiv_rn(__uint_as_float(most), 127.f);
+  if (first == 0 && m < M) scale[m] = __fdiv_rn(__uint_as_float(most), 127.f);
 #pragma unroll
   for (int u = 0; u < kUnits; ++u)
-    if (first + u * kStep < K) store_unit<WIDE>(out, first + u * kStep, K, v[u], r);
-  for (int c = first + kUnits * kStep; c < K; c += kStep) {
-    float t[8];
-    load_unit<T, WIDE>(row, c, K, t);
-    store_unit<WIDE>(out, c, K, t, r);
+    if (first + u * kStep < k) v[u].store(out + first + u * kStep, r);
+  for (int c = first + kUnits * kStep; c < k; c += kStep) {
+    t.load(row + c);
+    t.store(out + c, r);
+  }
+}
+
+// Any alignment: a row per CTA, read twice.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__ x, int64_t x_stride, int K,
+                                                           int8_t* __restrict__ q, int64_t q_stride,
+                                                           float* __restrict__ scale) {
+  __shared__ uint32_t red[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t m = blockIdx.x;
+  const T* row = x + m * x_stride;
+  uint32_t most = 0;
+  for (int c = threadIdx.x; c < K; c += 256) most = max(most, __float_as_uint(one(row + c)) & 0x7fffffffu);
+  most = cta_max(__reduce_max_sync(kFullMask, most), red);
+  RowScale r = row_scale(most);
+  if (threadIdx.x == 0) scale[m] = __fdiv_rn(__uint_as_float(most), 127.f);
+  for (int c = threadIdx.x; c < K; c += 256) {
+    float v[4] = {one(row + c), 0.f, 0.f, 0.f};
+    uint32_t w;
+    codes_of<4>(v, r, &w);
+    q[m * q_stride + c] = static_cast<int8_t>(w);
   }
 }
 
 template <typename T>
 int run(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale, cudaStream_t st) {
-  const bool wide = aligned(x, 16) && x_stride * sizeof(T) % 16 == 0 && K % 8 == 0 && aligned(q, 8) && q_stride % 8 == 0;
-  // A warp per row where the row fits its registers and there are rows for
-  // every warp; a CTA per row where rows are long or few.
-  const bool cta = K > kUnits * 32 * 8 || M < 148 * 8;
+  constexpr int N = Piece<T>::N;
+  const bool wide = aligned(x, 16) && x_stride * sizeof(T) % 16 == 0 && K % N == 0 && aligned(q, N) && q_stride % N == 0;
+  // Warps of a row: as few as hold it in their registers, so that a warp has as
+  // many loads in flight as it can, but a CTA for each row where rows are few.
+  int wpr = M < 148 * 8 ? 8 : 1;
+  while (wpr < 8 && K > kUnits * 32 * N * wpr) wpr *= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cta ? M : (M + 7) / 8);
+  cfg.gridDim = dim3(wide ? static_cast<unsigned>((static_cast<int64_t>(M) * wpr + 7) / 8) : M);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto* kernel = wide ? (cta ? quantize_kernel<T, true, true> : quantize_kernel<T, true, false>)
-                      : (cta ? quantize_kernel<T, false, true> : quantize_kernel<T, false, false>);
-  if (cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(x), x_stride, M, K, q, q_stride, scale) != cudaSuccess) {
+  const T* p = static_cast<const T*>(x);
+  auto* kernel = wpr == 1   ? quantize_kernel<T, 1>
+                 : wpr == 2 ? quantize_kernel<T, 2>
+                 : wpr == 4 ? quantize_kernel<T, 4>
+                            : quantize_kernel<T, 8>;
+  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, kernel, p, x_stride, M, K, q, q_stride, scale)
+                             : cudaLaunchKernelEx(&cfg, quantize_any_kernel<T>, p, x_stride, K, q, q_stride, scale);
+  if (e != cudaSuccess) {
     cudaGetLastError();
     return MTP_ERR_LAUNCH;
   }

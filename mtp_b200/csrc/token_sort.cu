@@ -71,23 +71,29 @@ __device__ __forceinline__ void copy_row(const SortArgs& a, int t, const int* po
 // ---------------------------------------------------------------------------
 template <typename V>
 __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArgs a) {
-  extern __shared__ int keys[];  // [numel], then the token's k positions
-  int* pos = keys + a.numel;
+  // [numel] keys, up to a multiple of 128 with a key above all, then the token's k positions
+  extern __shared__ __align__(16) int keys[];
+  const int padded = (a.numel + 127) / 128 * 128;
+  int* pos = keys + padded;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   pdl_launch_dependents();
   pdl_wait();
-  for (int i = tid; i < a.numel; i += blockDim.x) keys[i] = sort_key(a, i);
+  for (int i = tid; i < padded; i += blockDim.x) keys[i] = i < a.numel ? sort_key(a, i) : INT_MAX;
   __syncthreads();
+  // of the keys that this lane looks at (four at a time), how many does f count
+  auto count = [&](auto f) {
+    int n = 0;
+    for (int q = 4 * lane; q < padded; q += 128) {
+      const int4 k4 = *reinterpret_cast<const int4*>(keys + q);
+      n += f(k4.x, q) + f(k4.y, q + 1) + f(k4.z, q + 2) + f(k4.w, q + 3);
+    }
+    return __reduce_add_sync(kFullMask, n);
+  };
   const int t = blockIdx.x;
   if (t < a.M) {
     for (int j = warp; j < a.k; j += warps) {
       const int i = t * a.k + j, key = keys[i];
-      int before = 0;
-      for (int q = lane; q < a.numel; q += 32) {
-        const int kq = keys[q];
-        before += kq < key || (kq == key && q < i) ? 1 : 0;
-      }
-      before = __reduce_add_sync(kFullMask, before);
+      const int before = count([&](int kq, int q) { return kq < key || (kq == key && q < i) ? 1 : 0; });
       if (lane == 0) {
         const int p = key < a.E ? before : ~before;
         pos[j] = p;
@@ -106,9 +112,7 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArg
     }
   } else {
     for (int e = t + warp * gridDim.x; e <= a.E; e += warps * gridDim.x) {
-      int before = 0;
-      for (int q = lane; q < a.numel; q += 32) before += keys[q] < e ? 1 : 0;
-      before = __reduce_add_sync(kFullMask, before);
+      const int before = count([&](int kq, int) { return kq < e ? 1 : 0; });
       if (lane == 0) a.offsets[e] = before;
     }
   }
@@ -578,34 +582,54 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const U
 #pragma unroll
         for (int n = 0; n < N; ++n) g[q][n] += poison;
       }
-#pragma unroll 2
-      for (int j = 0; j < a.k; ++j) {
-        const int p = ps[j], r = p >= 0 ? p : ~p;
-        if (r >= a.num_rows) continue;
-        const float w = ws[j];
-        if (a.grad_weights && p >= 0) {
-          float d = 0.f;
+      // eight pairs together: their dot products are reduced as one
+#pragma unroll 1
+      for (int j0 = 0; j0 < a.k; j0 += 8) {
+        float d[8];
 #pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            float f[N];
-            to_floats(*reinterpret_cast<const V*>(slot + j * kSeg + (q * 32 + lane) * 16), f);
+        for (int x = 0; x < 8; ++x) {
+          d[x] = 0.f;
+          const int j = j0 + x, p = j < a.k ? ps[j] : INT_MIN, r = p >= 0 ? p : ~p;
+          if (r >= a.num_rows) continue;
+          const float w = ws[j];
+          if (a.grad_weights && p >= 0)
 #pragma unroll
-            for (int n = 0; n < N; ++n) d = in[q] ? fmaf(g[q][n], f[n], d) : d;
+            for (int q = 0; q < NP; ++q) {
+              float f[N];
+              to_floats(*reinterpret_cast<const V*>(slot + j * kSeg + (q * 32 + lane) * 16), f);
+#pragma unroll
+              for (int n = 0; n < N; ++n) d[x] = in[q] ? fmaf(g[q][n], f[n], d[x]) : d[x];
+            }
+          if (a.grad_rows) {
+            uint8_t* out = static_cast<uint8_t*>(a.grad_rows) + static_cast<int64_t>(r) * row_bytes + at;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+              float f[N];
+#pragma unroll
+              for (int n = 0; n < N; ++n) f[n] = p >= 0 ? w * g[q][n] : 0.f;
+              V o;
+              from_floats(f, o);
+              if (in[q]) *reinterpret_cast<V*>(out + (q * 32 + lane) * 16) = o;
+            }
           }
-          d = warp_sum(d);
-          if (lane == j) dot += d;
         }
-        if (a.grad_rows) {
-          uint8_t* out = static_cast<uint8_t*>(a.grad_rows) + static_cast<int64_t>(r) * row_bytes + at;
+        if (a.grad_weights) {
+          // halve the values and the lanes that hold each, then sum over the last four lanes:
+          // lane bits 4, 3, 2 number the value that a lane ends with
 #pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            float f[N];
+          for (int half = 4; half > 0; half /= 2) {
+            const bool upper = lane & (4 * half);
 #pragma unroll
-            for (int n = 0; n < N; ++n) f[n] = p >= 0 ? w * g[q][n] : 0.f;
-            V o;
-            from_floats(f, o);
-            if (in[q]) *reinterpret_cast<V*>(out + (q * 32 + lane) * 16) = o;
+            for (int x = 0; x < half; ++x) {
+              const float give = upper ? d[x] : d[x + half], keep = upper ? d[x + half] : d[x];
+              d[x] = keep + __shfl_xor_sync(kFullMask, give, 4 * half);
+            }
           }
+          d[0] += __shfl_xor_sync(kFullMask, d[0], 2);
+          d[0] += __shfl_xor_sync(kFullMask, d[0], 1);
+          // lane j keeps pair j's sum
+          const float mine = __shfl_sync(kFullMask, d[0], 4 * (lane & 7));
+          if (lane >> 3 == j0 >> 3) dot += mine;
         }
       }
       if (use.seg == segs - 1) {
@@ -659,7 +683,7 @@ template <typename V>
 int sort_run(const SortArgs& a, cudaStream_t st) {
   if (a.numel <= kSmallPairs)
     return launch(sort_small_kernel<V>, dim3(std::max(a.M, 1)), dim3(kSmallThreads),
-                  static_cast<size_t>(a.numel + a.k) * sizeof(int), st, a);
+                  static_cast<size_t>((a.numel + 127) / 128 * 128 + a.k) * sizeof(int), st, a);
   static int configured_device = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
@@ -698,20 +722,28 @@ int unsort_run(const UnsortArgs& a, bool backward, cudaStream_t st) {
                          reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.grad_rows) |
                          static_cast<uintptr_t>(static_cast<int64_t>(a.H) * sizeof(T));
   const int n = (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
-  // Bulk copies where rows are wide (512 bytes: a segment) and there are tasks
-  // for every warp's ring; a small call is done before a ring would fill.
+  // Bulk copies where rows are wide (512 bytes: a segment) and there is enough
+  // to fill the rings; a small call is done before that (backward of 8 x 2048
+  // bf16: 512 tokens 11 us against 13 by bulk copies, 1024 tokens 28 against 17).
   const int64_t row_bytes = static_cast<int64_t>(a.H) * sizeof(T);
   const int parts = a.k + (backward ? 1 : 0);
   if (n == kWide && row_bytes >= 512 && row_bytes < (1 << 30) && 2 * parts * 512 <= kBulkRing) {
-    const bool two = 2 * parts * 1024 <= kBulkRing && row_bytes >= 1024;
-    const int seg = two ? 1024 : 512;
+    // the widest segment of which a ring holds two tasks
+    int seg = 2048;
+    while (seg > 512 && (2 * parts * seg > kBulkRing || row_bytes < seg)) seg /= 2;
     const int sms = device_sm_count();
     if (!sms) return MTP_ERR_CUDA;
-    const int64_t tasks = backward ? a.M : a.M * ((row_bytes + seg - 1) / seg);
-    if (tasks >= 2ll * sms * kBulkWarps) {
+    const int64_t tasks = a.M * (backward ? 1 : (row_bytes + seg - 1) / seg);
+    if (tasks >= (backward ? 4ll : 16ll) * sms) {
       const int slots = std::min(kBulkSlots, kBulkRing / (parts * seg));
-      if (backward) return two ? bulk_run<T, 2, true>(a, slots, sms, st) : bulk_run<T, 1, true>(a, slots, sms, st);
-      return two ? bulk_run<T, 2, false>(a, slots, sms, st) : bulk_run<T, 1, false>(a, slots, sms, st);
+      switch (seg / 512 * 2 + (backward ? 1 : 0)) {
+        case 8: return bulk_run<T, 4, false>(a, slots, sms, st);
+        case 9: return bulk_run<T, 4, true>(a, slots, sms, st);
+        case 4: return bulk_run<T, 2, false>(a, slots, sms, st);
+        case 5: return bulk_run<T, 2, true>(a, slots, sms, st);
+        case 2: return bulk_run<T, 1, false>(a, slots, sms, st);
+        default: return bulk_run<T, 1, true>(a, slots, sms, st);
+      }
     }
   }
   const dim3 block = row_block((a.H + n - 1) / n, backward ? 32 : 8);
