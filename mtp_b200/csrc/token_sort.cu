@@ -28,7 +28,6 @@ constexpr int kRankThreads = 1024;
 constexpr int kRankWarps = kRankThreads / 32;
 // Up to this many pairs every CTA of the copy ranks its own token's pairs by
 // counting over all keys in shared memory (one launch); above, a cluster ranks
-
 // all pairs first (8 x 2048 bf16: 384 tokens 8.5 us, 512 tokens 11.1 in one
 // launch against 9.4 in two).
 constexpr int kSmallPairs = 3328;  // at most 4096: 12 bits
