@@ -17,6 +17,7 @@
 // into shared memory, while its first weights are on their way: a second launch
 // for so few rows costs more than quantising them again in every CTA.
 #include "quantize.cuh"
+#include "w8a8_common.cuh"
 
 #include <algorithm>
 
@@ -41,23 +42,6 @@ struct StreamArgs {
   int x_dtype, x_wide;
   int pitch;            // QUANT: bytes between quantised rows
 };
-
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-template <typename T>
-__device__ __forceinline__ T out_cast(float v);
-template <>
-__device__ __forceinline__ float out_cast(float v) { return v; }
-template <>
-__device__ __forceinline__ __half out_cast(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 out_cast(float v) { return __float2bfloat16_rn(v); }
 
 // Rows quantised into shared memory by the whole CTA, warps_per_row warps a row.
 template <typename X, bool WIDE>

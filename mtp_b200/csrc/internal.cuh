@@ -177,6 +177,11 @@ int launch_unsort_tokens(const UnsortArgs& a, int dtype, bool backward, cudaStre
 int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
                          float* scale, cudaStream_t st);
 
+// Contiguous rows to int8 and their tokens' top-k (as launch_router_topk).
+int launch_route_quantize(const void* x, int dtype, int M, int K, int8_t* q, int64_t q_stride, float* scale,
+                          const float* logits, int E, int k, int renorm, float* weights, int32_t* ids,
+                          cudaStream_t st);
+
 // int8 products (int8_matmul.cu).
 struct Int8Args {
   int P, N, K, E;              // rows, rows of b per group, K, groups

@@ -12,6 +12,7 @@
 // second time. 8192 x 2048 bf16 took 18.7 us with the row kept as fp32 (fewer
 // warps resident) and a conversion per code.
 #include "quantize.cuh"
+#include "w8a8_common.cuh"
 
 #include <type_traits>
 
@@ -70,17 +71,14 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t most, uint32_t* red) {
   return most;
 }
 
-// WPR warps a row, 8 / WPR rows a CTA; rows and codes aligned.
+// WPR warps a row, 8 / WPR rows a CTA of 256 threads; rows and codes aligned.
 template <typename T, int WPR>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t x_stride, int M, int K,
-                                                       int8_t* __restrict__ q, int64_t q_stride,
-                                                       float* __restrict__ scale) {
+__device__ __forceinline__ void quantize_rows(int block, const T* __restrict__ x, int64_t x_stride, int M, int K,
+                                              int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scale) {
   using P = Piece<T>;
   __shared__ uint32_t red[8];
-  pdl_launch_dependents();
-  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t m = static_cast<int64_t>(blockIdx.x) * (8 / WPR) + warp / WPR;
+  const int64_t m = static_cast<int64_t>(block) * (8 / WPR) + warp / WPR;
   const int k = m < M ? K : 0;
   const int first = (warp % WPR * 32 + lane) * P::N;
   constexpr int kStep = WPR * 32 * P::N;
@@ -117,6 +115,42 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   }
 }
 
+template <typename T, int WPR>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t x_stride, int M, int K,
+                                                       int8_t* __restrict__ q, int64_t q_stride,
+                                                       float* __restrict__ scale) {
+  pdl_launch_dependents();
+  pdl_wait();
+  quantize_rows<T, WPR>(blockIdx.x, x, x_stride, M, K, q, q_stride, scale);
+}
+
+// The rows of a layer quantised and its tokens routed, which do not depend on
+// each other, in one launch: the first CTAs route 8 tokens each (a warp a
+// token), the others quantise.
+template <typename T, int WPR, int VPT>
+__global__ void __launch_bounds__(256) route_quantize_kernel(const T* __restrict__ x, int M, int K,
+                                                             int8_t* __restrict__ q, int64_t q_stride,
+                                                             float* __restrict__ scale, const float* __restrict__ logits,
+                                                             int E, int k, int renorm, float* __restrict__ weights,
+                                                             int32_t* __restrict__ ids) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int routing = (M + 7) / 8;
+  if (static_cast<int>(blockIdx.x) >= routing) {
+    quantize_rows<T, WPR>(blockIdx.x - routing, x, K, M, K, q, q_stride, scale);
+    return;
+  }
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= M) return;
+  float w;
+  int id;
+  route_token<VPT>(logits + static_cast<int64_t>(t) * E, E, k, renorm, &w, &id);
+  if (lane < k) {
+    weights[static_cast<int64_t>(t) * k + lane] = w;
+    ids[static_cast<int64_t>(t) * k + lane] = id;
+  }
+}
+
 // Any alignment: a row per CTA, read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__ x, int64_t x_stride, int K,
@@ -141,13 +175,63 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__
 }
 
 template <typename T>
-int run(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale, cudaStream_t st) {
+bool wide_rows(const void* x, int64_t x_stride, int K, const void* q, int64_t q_stride) {
   constexpr int N = Piece<T>::N;
-  const bool wide = aligned(x, 16) && x_stride * sizeof(T) % 16 == 0 && K % N == 0 && aligned(q, N) && q_stride % N == 0;
-  // Warps of a row: as few as hold it in their registers, so that a warp has as
-  // many loads in flight as it can, but a CTA for each row where rows are few.
+  return aligned(x, 16) && x_stride * sizeof(T) % 16 == 0 && K % N == 0 && aligned(q, N) && q_stride % N == 0;
+}
+
+// Warps of a row: as few as hold it in their registers, so that a warp has as
+// many loads in flight as it can, but a CTA for each row where rows are few.
+template <typename T>
+int warps_per_row(int M, int K) {
   int wpr = M < 148 * 8 ? 8 : 1;
-  while (wpr < 8 && K > kUnits * 32 * N * wpr) wpr *= 2;
+  while (wpr < 8 && K > kUnits * 32 * Piece<T>::N * wpr) wpr *= 2;
+  return wpr;
+}
+
+template <typename T, int WPR, int VPT>
+int run_routed(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* scale, const float* logits, int E, int k,
+               int renorm, float* weights, int32_t* ids, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((M + 7) / 8 + (static_cast<int64_t>(M) * WPR + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, route_quantize_kernel<T, WPR, VPT>, static_cast<const T*>(x), M, K, q, q_stride, scale,
+                         logits, E, k, renorm, weights, ids) != cudaSuccess) {
+    cudaGetLastError();
+    return MTP_ERR_LAUNCH;
+  }
+  return MTP_OK;
+}
+
+template <typename T, int WPR>
+int by_experts(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* scale, const float* logits, int E, int k,
+               int renorm, float* weights, int32_t* ids, cudaStream_t st) {
+  return E <= 256 ? run_routed<T, WPR, 8>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st)
+                  : run_routed<T, WPR, 32>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+}
+
+template <typename T>
+int route_and_quantize(const void* x, int dtype, int M, int K, int8_t* q, int64_t q_stride, float* scale,
+                       const float* logits, int E, int k, int renorm, float* weights, int32_t* ids, cudaStream_t st) {
+  if (!wide_rows<T>(x, K, K, q, q_stride)) {
+    const int rc = launch_router_topk(logits, M, E, k, renorm, weights, ids, nullptr, st);
+    return rc != MTP_OK ? rc : launch_quantize_int8(x, K, dtype, M, K, q, q_stride, scale, st);
+  }
+  return warps_per_row<T>(M, K) == 1
+             ? by_experts<T, 1>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st)
+             : by_experts<T, 8>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+}
+
+template <typename T>
+int run(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale, cudaStream_t st) {
+  const bool wide = wide_rows<T>(x, x_stride, K, q, q_stride);
+  const int wpr = warps_per_row<T>(M, K);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -179,6 +263,19 @@ int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int 
     case MTP_DTYPE_BF16: return run<__nv_bfloat16>(x, x_stride, M, K, q, q_stride, scale, st);
     case MTP_DTYPE_FP16: return run<__half>(x, x_stride, M, K, q, q_stride, scale, st);
     default: return run<float>(x, x_stride, M, K, q, q_stride, scale, st);
+  }
+}
+
+int launch_route_quantize(const void* x, int dtype, int M, int K, int8_t* q, int64_t q_stride, float* scale,
+                          const float* logits, int E, int k, int renorm, float* weights, int32_t* ids,
+                          cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16:
+      return route_and_quantize<__nv_bfloat16>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+    case MTP_DTYPE_FP16:
+      return route_and_quantize<__half>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+    default:
+      return route_and_quantize<float>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
   }
 }
 

@@ -329,14 +329,15 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
 
   const float* weights = p.topk_weights;
   const int32_t* ids = p.topk_ids;
+  int8_t* xq = reinterpret_cast<int8_t*>(ws + w.xq);
   if (p.router_logits) {
-    rc = launch_router_topk(p.router_logits, M, E, k, p.renormalize ? 1 : 0, f32(w.tw), i32(w.tid), nullptr, st);
-    if (rc != MTP_OK) return rc;
+    rc = launch_route_quantize(p.hidden_states, p.dtype, M, H, xq, w.hp, f32(w.xs), p.router_logits, E, k,
+                               p.renormalize ? 1 : 0, f32(w.tw), i32(w.tid), st);
     weights = f32(w.tw);
     ids = i32(w.tid);
+  } else {
+    rc = launch_quantize_int8(p.hidden_states, H, p.dtype, M, H, xq, w.hp, f32(w.xs), st);
   }
-  rc = launch_quantize_int8(p.hidden_states, H, p.dtype, M, H, reinterpret_cast<int8_t*>(ws + w.xq), w.hp, f32(w.xs),
-                            st);
   if (rc != MTP_OK) return rc;
 
   SortArgs s = {};
