@@ -98,7 +98,7 @@ def train(args, g) -> tuple[float, float]:
         optimizer.zero_grad()
         loss.backward()
         optimizer.step()
-        losses.append(float(loss))
+        losses.append(loss.item())
     print(f"training {args.steps} steps: loss {losses[0]:.4f} -> {losses[-1]:.4f}")
     return losses[0], losses[-1]
 

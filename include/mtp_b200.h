@@ -322,8 +322,9 @@ enum MtpActivation {
  * exact in int32, scales in fp32, rounded once to out_dtype.
  * offsets NULL: one product, b [n, k]. With offsets [num_groups + 1]: rows
  * offsets[g] .. offsets[g + 1] use b[g] of [num_groups, n, k] and b_scale[g];
- * rows from offsets[num_groups] on are written as zeros (offsets[0] = 0, as
- * mtp_sort_tokens gives them).
+ * rows before offsets[0] and from offsets[num_groups] on are written as zeros.
+ * The offsets ascend (mtp_sort_tokens gives them, from 0); values outside
+ * [0, rows] are clamped.
  * a_dtype int8: a [rows, k] with a_scale [rows]. Else a is bf16, fp16 or fp32
  * and is quantised as mtp_quantize_int8 does, in the workspace; a_scale NULL.
  * k < 131072; num_groups <= 1024. Rows of a (int8) or b that are not 16-byte

@@ -77,9 +77,9 @@ __device__ __forceinline__ void build_row_blocks(const Int8Args& a, RowBlocks& b
   for (int x = threadIdx.x; x < min(b.pre[a.E], kBlockTable); x += threads) b.table[x] = b.find(x, a.E);
 }
 
-// Rows behind the last group's are zero: the bytes [from, to) of the output,
+// Rows of no group are zero: the bytes [from, to) of the output,
 // shared out over the first `threads` threads of every CTA.
-__device__ __forceinline__ void zero_tail(uint8_t* from, uint8_t* to, int threads) {
+__device__ __forceinline__ void zero_rows(uint8_t* from, uint8_t* to, int threads) {
   const int64_t tid = static_cast<int64_t>(blockIdx.x) * threads + threadIdx.x;
   const int64_t all = static_cast<int64_t>(gridDim.x) * threads;
   uint8_t* lo = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(from) + 15) & ~static_cast<uintptr_t>(15));

@@ -414,8 +414,11 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
   const int quad = warp & 3, part = warp >> 2;
   const int width = GATED ? a.N / 2 : a.N;  // columns of the output
   T* out = static_cast<T*>(a.out);
+  if (cb.rows.first[0] > 0)
+    zero_rows(reinterpret_cast<uint8_t*>(out),
+              reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.rows.first[0]) * width), kTEpiWarps * 32);
   if (cb.rows.routed < a.P)
-    zero_tail(reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.rows.routed) * width),
+    zero_rows(reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(cb.rows.routed) * width),
               reinterpret_cast<uint8_t*>(out + static_cast<int64_t>(a.P) * width), kTEpiWarps * 32);
   const int64_t pitch = static_cast<int64_t>(width) * sizeof(T);
   const bool wide = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
@@ -703,20 +706,21 @@ int run_tiles(Int8Args& a, const void* ap, int64_t a_stride, const void* bp, int
               cudaStream_t st) {
   auto* kernel = tile_kernel<NT, PAIR, GATED, T>;
   constexpr size_t smem = tile_smem<NT, PAIR>();
-  static int configured_device = -1, slots = 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
-  if (configured_device != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) !=
-        cudaSuccess)
-      return MTP_ERR_CUDA;
-    slots = PAIR ? pair_slots(kernel, smem, sms) : sms;
+  static DeviceRecord record;
+  int rc = allow_shared(record, kernel, smem);
+  if (rc != MTP_OK) return rc;
+  int slots = sms;
+  if (PAIR) {
+    static int pairs[64] = {};  // by device, 0 before the first call
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MTP_ERR_CUDA;
+    if (!pairs[dev]) pairs[dev] = pair_slots(kernel, smem, sms);
+    slots = pairs[dev];
     if (slots < 1) return MTP_ERR_CUDA;
-    configured_device = dev;
   }
   Maps maps;
   maps.blocks = GATED && a.N % 32 == 0;
-  int rc = encode_rows(&maps.rows, ap, a.P, a.K, a_stride, Ring<NT, PAIR>::kRows);
+  rc = encode_rows(&maps.rows, ap, a.P, a.K, a_stride, Ring<NT, PAIR>::kRows);
   if (rc == MTP_OK) rc = encode_rows(&maps.few, ap, a.P, a.K, a_stride, kTBox);
   if (rc == MTP_OK)
     rc = maps.blocks ? encode_gated(&maps.weights, bp, a.E, a.N / 2, a.K, b_stride)

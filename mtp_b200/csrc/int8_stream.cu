@@ -206,14 +206,9 @@ int run(const Int8Args& a, StreamArgs p, cudaStream_t st) {
   auto* kernel = stream_kernel<QUANT, T>;
   const int sms = device_sm_count();
   if (!sms) return MTP_ERR_CUDA;
-  static int configured_device = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
-  if (configured_device != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSRowBytes) != cudaSuccess)
-      return MTP_ERR_CUDA;
-    configured_device = dev;
-  }
+  static DeviceRecord record;
+  const int rc = allow_shared(record, kernel, kSRowBytes);
+  if (rc != MTP_OK) return rc;
   p.kp = (a.K + 15) / 16 * 16;
   p.strips = (a.N + 15) / 16;
   // Warps of a unit: as many as it takes to give every warp of the GPU work.

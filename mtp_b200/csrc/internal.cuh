@@ -146,6 +146,26 @@ inline int device_sm_count() {
   return sms[dev];
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device; `done` is
+// the caller's record (static, one per kernel). Setting it twice does no harm.
+struct DeviceRecord {
+  bool done[64];
+};
+template <typename F>
+int allow_shared(DeviceRecord& r, F* kernel, size_t bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MTP_ERR_CUDA;
+  if (!r.done[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) !=
+        cudaSuccess) {
+      cudaGetLastError();
+      return MTP_ERR_CUDA;
+    }
+    r.done[dev] = true;
+  }
+  return MTP_OK;
+}
+
 // Token sort and unsort (token_sort.cu). Strides and row sizes in bytes.
 struct SortArgs {
   int M, k, E, E_map, numel;

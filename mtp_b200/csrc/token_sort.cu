@@ -687,16 +687,10 @@ int sort_run(const SortArgs& a, cudaStream_t st) {
   if (a.numel <= kSmallPairs)
     return launch(sort_small_kernel<V>, dim3(std::max(a.M, 1)), dim3(kSmallThreads),
                   static_cast<size_t>((a.numel + 127) / 128 * 128 + a.k) * sizeof(int), st, a);
-  static int configured_device = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
-  if (configured_device != dev) {
-    if (cudaFuncSetAttribute(sort_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(rank_smem(1024))) != cudaSuccess)
-      return MTP_ERR_CUDA;
-    configured_device = dev;
-  }
-  const int rc = launch(sort_rank_kernel, dim3(kRankCtas), dim3(kRankThreads), rank_smem(a.E), st, a);
+  static DeviceRecord record;
+  int rc = allow_shared(record, sort_rank_kernel, rank_smem(1024));
+  if (rc != MTP_OK) return rc;
+  rc = launch(sort_rank_kernel, dim3(kRankCtas), dim3(kRankThreads), rank_smem(a.E), st, a);
   if (rc != MTP_OK) return rc;
   const dim3 block = row_block(a.row_bytes / static_cast<int64_t>(sizeof(V)), 8);
   return launch(sort_copy_kernel<V>, dim3((a.M + block.y - 1) / block.y), block, 0, st, a);
@@ -705,16 +699,9 @@ int sort_run(const SortArgs& a, cudaStream_t st) {
 template <typename T, int NP, bool BACKWARD>
 int bulk_run(const UnsortArgs& a, int slots, int sms, cudaStream_t st) {
   auto* kernel = unsort_bulk_kernel<T, NP, BACKWARD>;
-  static int configured_device = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
-  if (configured_device != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBulkSmem)) !=
-        cudaSuccess)
-      return MTP_ERR_CUDA;
-    configured_device = dev;
-  }
-  return launch(kernel, dim3(sms), dim3(kBulkWarps * 32), kBulkSmem, st, a, slots);
+  static DeviceRecord record;
+  const int rc = allow_shared(record, kernel, kBulkSmem);
+  return rc != MTP_OK ? rc : launch(kernel, dim3(sms), dim3(kBulkWarps * 32), kBulkSmem, st, a, slots);
 }
 
 template <typename T>

@@ -417,18 +417,11 @@ template <int VPT, typename T>
 int run(const DecodeArgs& a, cudaStream_t st) {
   const int sms = device_sm_count();
   if (!sms) return MTP_ERR_CUDA;
-  static int configured_device = -1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return MTP_ERR_CUDA;
-  if (configured_device != dev) {
-    if (cudaFuncSetAttribute(decode_up_kernel<VPT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDCodes) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(decode_down_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDCodes) !=
-            cudaSuccess)
-      return MTP_ERR_CUDA;
-    configured_device = dev;
-  }
-  const int rc = launch(decode_up_kernel<VPT, T>, a, sms, static_cast<size_t>(a.M) * decode_pitch(a.H), st);
+  static DeviceRecord up, down;
+  int rc = allow_shared(up, decode_up_kernel<VPT, T>, kDCodes);
+  if (rc == MTP_OK) rc = allow_shared(down, decode_down_kernel<T>, kDCodes);
+  if (rc != MTP_OK) return rc;
+  rc = launch(decode_up_kernel<VPT, T>, a, sms, static_cast<size_t>(a.M) * decode_pitch(a.H), st);
   return rc != MTP_OK ? rc : launch(decode_down_kernel<T>, a, sms, kDRows * decode_pitch(a.I), st);
 }
 

@@ -342,8 +342,8 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
                         activation: str | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Rows ``offsets[g] .. offsets[g + 1]`` of int8 ``a`` [P, K] times ``b[g]`` of
     [G, N, K], scaled as in :func:`int8_matmul` by ``a_scale`` [P] and ``b_scale``
-    [G, N]. ``offsets`` [G + 1] int32 ascend from 0 (those of
-    :func:`sort_tokens`); rows behind ``offsets[G]`` are zeros.
+    [G, N]. ``offsets`` [G + 1] int32 ascend (those of :func:`sort_tokens`, from
+    0); rows before ``offsets[0]`` and from ``offsets[G]`` on are zeros.
     ``activation="silu_mul"``: the first N / 2 channels are gates, and the
     result [P, N / 2] is silu(gate) * up."""
     _check_rows(a, a_scale)

@@ -241,6 +241,21 @@ def test_int8_grouped_matmul_silu_mul(cuda_device, counts, n, k, dtype):
     assert not out[routed:].any()
 
 
+@pytest.mark.parametrize("rows", [12, 900])
+def test_grouped_rows_of_no_group(cuda_device, rows):
+    """Rows before offsets[0] are zeros, offsets past the rows are clamped."""
+    import mtp_b200
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    a, b = codes(g, rows, 64, dev=cuda_device), codes(g, 3, 40, 64, dev=cuda_device)
+    sa, sb = scales(g, rows, dev=cuda_device), scales(g, 3, 40, dev=cuda_device)
+    mid = rows // 2
+    offsets = torch.tensor([5, mid, mid, rows + 7], dtype=torch.int32, device=cuda_device)
+    out = mtp_b200.int8_grouped_matmul(a, sa, b, sb, offsets, out_dtype=torch.float32)
+    assert not out[:5].any()
+    for e, part in ((0, slice(5, mid)), (2, slice(mid, rows))):
+        check_product(out[part], a[part].double() @ b[e].double().T, sa[part], sb[e], None, torch.float32)
+
+
 def test_grouped_many_experts_and_64_bit_offsets(cuda_device):
     """1024 groups; weights of 2.1e9 bytes, so that their byte offsets pass 2^31."""
     import mtp_b200
@@ -356,6 +371,22 @@ def test_layer_with_many_pairs_of_one_expert(cuda_device, m):
     out = mtp_b200.moe_layer_w8a8(c["x"], None, c["w13"], c["s13"], c["w2"], c["s2"], 7, topk_weights=w, topk_ids=ids)
     check_layer(out, plain_layer(c, w, ids))
     assert not out[m // 2].any()
+
+
+@pytest.mark.parametrize("m", [4, 60, 700])
+def test_layer_keeps_a_bad_token_to_itself(cuda_device, m):
+    """An infinity or a NaN in one token's row makes that token's output NaN and no other's."""
+    import mtp_b200
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    c = layer_case(g, m, 8, 128, 64, torch.bfloat16, cuda_device)
+    args = (c["logits"], c["w13"], c["s13"], c["w2"], c["s2"], 2)
+    good = mtp_b200.moe_layer_w8a8(c["x"], *args)
+    x = c["x"].clone()
+    x[1, 7], x[m - 1, 0] = float("nan"), float("inf")
+    out = mtp_b200.moe_layer_w8a8(x, *args)
+    bad = torch.zeros(m, dtype=torch.bool, device=cuda_device)
+    bad[1] = bad[m - 1] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], good[~bad])
 
 
 def test_layer_in_a_graph_and_on_a_side_stream(cuda_device):
