@@ -69,6 +69,8 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 def _row_stride(name: str, t: torch.Tensor) -> int:
     """Elements between the rows of a 2-D tensor whose rows are contiguous and do not overlap."""
+    if t.is_contiguous():
+        return t.shape[1]
     if t.shape[0] <= 1:
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError(f"the rows of {name} must be contiguous")
@@ -98,7 +100,7 @@ class SortedTokens(NamedTuple):
 def _sort(x, ids, num_experts, expert_map, row_scales):
     m, k = ids.shape
     h = x.shape[1]
-    rows = x.new_empty((m * k, h))
+    rows = x.new_empty(m * k, h)
     positions = torch.empty_like(ids)
     offsets = ids.new_empty(num_experts + 1)
     scales = None if row_scales is None else row_scales.new_empty(m * k)
@@ -113,7 +115,7 @@ def _sort(x, ids, num_experts, expert_map, row_scales):
 def _unsort(rows, positions, weights):
     m, k = positions.shape
     r, h = rows.shape
-    out = rows.new_empty((m, h))
+    out = rows.new_empty(m, h)
     _unsort_entry(rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
                   None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr(),
                   _stream(rows.get_device()))
@@ -152,7 +154,7 @@ class _UnsortTokens(torch.autograd.Function):
         grad = grad.contiguous()
         (m, k), h = positions.shape, grad.shape[1]
         need_rows, _, need_weights = ctx.needs_input_grad
-        grad_rows = grad.new_empty((ctx.num_rows, h)) if need_rows else None
+        grad_rows = grad.new_empty(ctx.num_rows, h) if need_rows else None
         grad_weights = torch.empty_like(weights) if need_weights else None
         _unsort_backward_entry(grad.data_ptr(), None if rows is None else rows.data_ptr(), ctx.num_rows,
                                DTYPES[grad.dtype], positions.data_ptr(),
@@ -235,7 +237,7 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if k < 1:
         raise ValueError("x must have at least one column")
     kp = (k + 15) // 16 * 16
-    codes = x.new_empty((m, kp), dtype=torch.int8)
+    codes = x.new_empty(m, kp, dtype=torch.int8)
     scale = x.new_empty(m, dtype=torch.float32)
     _quantize_entry(x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(), kp, scale.data_ptr(),
                     _stream(x.get_device()))
@@ -255,7 +257,8 @@ def _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, a_off, b_off) -> in
 def _product(a, a_scale, b, b_scale, bias, offsets, out_dtype, activation, status):
     rows, k = a.shape
     n, groups = b.shape[-2], b.shape[0] if b.dim() == 3 else 1
-    out = a.new_empty((rows, n // 2 if activation else n), dtype=out_dtype)
+    cols = n // 2 if activation else n
+    out = a.new_empty(rows, cols) if out_dtype is a.dtype else a.new_empty(rows, cols, dtype=out_dtype)
     a_dtype, a_stride = DTYPES.get(a.dtype, _INT8), _row_stride("a", a)
     ap, bp = a.data_ptr(), b.data_ptr()
     size = _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, ap & 255, bp & 255)
