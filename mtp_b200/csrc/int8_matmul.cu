@@ -594,44 +594,6 @@ __global__ void __launch_bounds__(kTThreads, 1) tile_kernel(const __grid_constan
   }
 }
 
-// ---------------------------------------------------------------------------
-// rows into a layout that TMA and 16-byte loads take (aligned base and stride),
-// zeros behind each row
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) pad_rows_kernel(const int8_t* __restrict__ src, int64_t stride, int64_t rows,
-                                                       int K, int8_t* __restrict__ dst, int64_t dst_stride) {
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows;
-       r += static_cast<int64_t>(gridDim.x) * 8)
-    for (int c = (threadIdx.x & 31) * 4; c < dst_stride; c += 128) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (c + q < K) w |= static_cast<uint32_t>(static_cast<uint8_t>(src[r * stride + c + q])) << (8 * q);
-      *reinterpret_cast<uint32_t*>(dst + r * dst_stride + c) = w;
-    }
-}
-
-template <typename F, typename... A>
-int launch(F* kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
-    cudaGetLastError();
-    return MTP_ERR_LAUNCH;
-  }
-  return MTP_OK;
-}
-
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -774,13 +736,6 @@ int by_rows(Int8Args& a, int nt, int out_dtype, const void* ap, int64_t as, cons
 }  // namespace
 
 bool tma_rows_ok(const void* base, int64_t stride) { return aligned(base, 16) && stride % 16 == 0; }
-
-int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* dst, int64_t dst_stride,
-                    cudaStream_t st) {
-  const int64_t grid = std::min<int64_t>((rows + 7) / 8, 148 * 16);
-  return launch(pad_rows_kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, st, static_cast<const int8_t*>(src),
-                stride, rows, K, static_cast<int8_t*>(dst), dst_stride);
-}
 
 int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, bool a_padded,
                        const void* bp, int64_t b_stride, cudaStream_t st) {

@@ -214,8 +214,19 @@ struct Int8Args {
   int32_t* status;             // [1] or NULL: bit 0 set when a wait ran out
 };
 bool tma_rows_ok(const void* base, int64_t stride);
-int launch_pad_rows(const void* src, int64_t stride, int64_t rows, int K, void* dst, int64_t dst_stride,
-                    cudaStream_t st);
+// Rows into a layout that TMA and 16-byte loads take (quantize.cu): zeros from K
+// to dst_stride, a multiple of 16. rows 0: nothing.
+struct PadJob {
+  const int8_t* src;
+  int64_t stride, rows;
+  int K;
+  int8_t* dst;
+  int64_t dst_stride;
+};
+int launch_pad_rows(const PadJob& a, const PadJob& b, cudaStream_t st);
+// Rows to int8 as launch_quantize_int8, and other rows padded.
+int launch_quantize_and_pad(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
+                            float* scale, const PadJob& pad, cudaStream_t st);
 // a_padded: ap is a workspace whose rows may be read up to a multiple of 16.
 int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, int64_t a_stride, bool a_padded,
                        const void* bp, int64_t b_stride, cudaStream_t st);

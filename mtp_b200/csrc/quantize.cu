@@ -14,6 +14,7 @@
 #include "quantize.cuh"
 #include "w8a8_common.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mtp {
@@ -153,18 +154,14 @@ __global__ void __launch_bounds__(256) route_quantize_kernel(const T* __restrict
 
 // Any alignment: a row per CTA, read twice.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__ x, int64_t x_stride, int K,
-                                                           int8_t* __restrict__ q, int64_t q_stride,
-                                                           float* __restrict__ scale) {
+__device__ __forceinline__ void quantize_any(int64_t m, const T* __restrict__ x, int64_t x_stride, int K,
+                                             int8_t* __restrict__ q, int64_t q_stride, float* __restrict__ scale) {
   __shared__ uint32_t red[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t m = blockIdx.x;
   const T* row = x + m * x_stride;
   uint32_t most = 0;
   for (int c = threadIdx.x; c < K; c += 256) most = max(most, __float_as_uint(one(row + c)) & 0x7fffffffu);
   most = cta_max(__reduce_max_sync(kFullMask, most), red);
-  RowScale r = row_scale(most);
+  const RowScale r = row_scale(most);
   if (threadIdx.x == 0) scale[m] = __fdiv_rn(__uint_as_float(most), 127.f);
   for (int c = threadIdx.x; c < K; c += 256) {
     float v[4] = {one(row + c), 0.f, 0.f, 0.f};
@@ -172,6 +169,88 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__
     codes_of<4>(v, r, &w);
     q[m * q_stride + c] = static_cast<int8_t>(w);
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_any_kernel(const T* __restrict__ x, int64_t x_stride, int K,
+                                                           int8_t* __restrict__ q, int64_t q_stride,
+                                                           float* __restrict__ scale) {
+  pdl_launch_dependents();
+  pdl_wait();
+  quantize_any(blockIdx.x, x, x_stride, K, q, q_stride, scale);
+}
+
+// Padded copies by the warps of `blocks` CTAs, 16 bytes a lane: five aligned
+// words that hold them wherever the row starts (none past the last row's end,
+// none without a byte of the row), shifted into place.
+__device__ __forceinline__ void pad_rows(const PadJob& j, int block, int blocks) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = static_cast<int64_t>(block) * 8 + (threadIdx.x >> 5); r < j.rows;
+       r += static_cast<int64_t>(blocks) * 8) {
+    const int8_t* row = j.src + r * j.stride;
+    for (int c = lane * 16; c < j.dst_stride; c += 512) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+      const uint32_t* word = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+      const uint32_t* end = reinterpret_cast<const uint32_t*>(row + j.K);
+      const int shift = 8 * static_cast<int>(at & 3);
+      uint32_t w[5], o[4];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = c < j.K && word + i < end && (i < 4 || shift) ? word[i] : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = __funnelshift_r(w[i], w[i + 1], shift);
+        const int left = j.K - c - 4 * i;  // bytes of the row in this word
+        if (left < 4) o[i] = left > 0 ? o[i] & (0xffffffffu >> (32 - 8 * left)) : 0u;
+      }
+      *reinterpret_cast<uint4*>(j.dst + r * j.dst_stride + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ PadJob a, int blocks_a,
+                                                       const __grid_constant__ PadJob b) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (static_cast<int>(blockIdx.x) < blocks_a)
+    pad_rows(a, blockIdx.x, blocks_a);
+  else
+    pad_rows(b, blockIdx.x - blocks_a, gridDim.x - blocks_a);
+}
+
+// The first M CTAs quantise a row each, the others pad.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_and_pad_kernel(const T* __restrict__ x, int64_t x_stride, int M, int K,
+                                                               int8_t* __restrict__ q, int64_t q_stride,
+                                                               float* __restrict__ scale, int wide,
+                                                               const __grid_constant__ PadJob pad) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (static_cast<int>(blockIdx.x) >= M)
+    pad_rows(pad, blockIdx.x - M, gridDim.x - M);
+  else if (wide)
+    quantize_rows<T, 8>(blockIdx.x, x, x_stride, M, K, q, q_stride, scale);
+  else
+    quantize_any(blockIdx.x, x, x_stride, K, q, q_stride, scale);
+}
+
+int pad_blocks(const PadJob& j) { return static_cast<int>(std::min<int64_t>((j.rows + 7) / 8, 148 * 8)); }
+
+template <typename F, typename... A>
+int launch(F* kernel, int64_t grid, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return MTP_ERR_LAUNCH;
+  }
+  return MTP_OK;
 }
 
 template <typename T>
@@ -192,21 +271,8 @@ int warps_per_row(int M, int K) {
 template <typename T, int WPR, int VPT>
 int run_routed(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* scale, const float* logits, int E, int k,
                int renorm, float* weights, int32_t* ids, cudaStream_t st) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((M + 7) / 8 + (static_cast<int64_t>(M) * WPR + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, route_quantize_kernel<T, WPR, VPT>, static_cast<const T*>(x), M, K, q, q_stride, scale,
-                         logits, E, k, renorm, weights, ids) != cudaSuccess) {
-    cudaGetLastError();
-    return MTP_ERR_LAUNCH;
-  }
-  return MTP_OK;
+  return launch(route_quantize_kernel<T, WPR, VPT>, (M + 7) / 8 + (static_cast<int64_t>(M) * WPR + 7) / 8, st,
+                static_cast<const T*>(x), M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids);
 }
 
 template <typename T, int WPR>
@@ -232,27 +298,20 @@ template <typename T>
 int run(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale, cudaStream_t st) {
   const bool wide = wide_rows<T>(x, x_stride, K, q, q_stride);
   const int wpr = warps_per_row<T>(M, K);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(wide ? static_cast<unsigned>((static_cast<int64_t>(M) * wpr + 7) / 8) : M);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   const T* p = static_cast<const T*>(x);
+  if (!wide) return launch(quantize_any_kernel<T>, M, st, p, x_stride, K, q, q_stride, scale);
   auto* kernel = wpr == 1   ? quantize_kernel<T, 1>
                  : wpr == 2 ? quantize_kernel<T, 2>
                  : wpr == 4 ? quantize_kernel<T, 4>
                             : quantize_kernel<T, 8>;
-  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, kernel, p, x_stride, M, K, q, q_stride, scale)
-                             : cudaLaunchKernelEx(&cfg, quantize_any_kernel<T>, p, x_stride, K, q, q_stride, scale);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return MTP_ERR_LAUNCH;
-  }
-  return MTP_OK;
+  return launch(kernel, (static_cast<int64_t>(M) * wpr + 7) / 8, st, p, x_stride, M, K, q, q_stride, scale);
+}
+
+template <typename T>
+int run_padded(const void* x, int64_t x_stride, int M, int K, int8_t* q, int64_t q_stride, float* scale,
+               const PadJob& pad, cudaStream_t st) {
+  return launch(quantize_and_pad_kernel<T>, static_cast<int64_t>(M) + pad_blocks(pad), st, static_cast<const T*>(x),
+                x_stride, M, K, q, q_stride, scale, wide_rows<T>(x, x_stride, K, q, q_stride) ? 1 : 0, pad);
 }
 
 }  // namespace
@@ -276,6 +335,25 @@ int launch_route_quantize(const void* x, int dtype, int M, int K, int8_t* q, int
       return route_and_quantize<__half>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
     default:
       return route_and_quantize<float>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+  }
+}
+
+int launch_pad_rows(const PadJob& a, const PadJob& b, cudaStream_t st) {
+  const int blocks = pad_blocks(a) + pad_blocks(b);
+  return blocks ? launch(pad_rows_kernel, blocks, st, a, pad_blocks(a), b) : MTP_OK;
+}
+
+int launch_quantize_and_pad(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
+                            float* scale, const PadJob& pad, cudaStream_t st) {
+  // one launch where there are few rows; many are worth their own kernel
+  if (!pad.rows || M >= 148 * 8) {
+    const int rc = launch_pad_rows(pad, PadJob{}, st);
+    return rc != MTP_OK ? rc : launch_quantize_int8(x, x_stride, dtype, M, K, q, q_stride, scale, st);
+  }
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return run_padded<__nv_bfloat16>(x, x_stride, M, K, q, q_stride, scale, pad, st);
+    case MTP_DTYPE_FP16: return run_padded<__half>(x, x_stride, M, K, q, q_stride, scale, pad, st);
+    default: return run_padded<float>(x, x_stride, M, K, q, q_stride, scale, pad, st);
   }
 }
 

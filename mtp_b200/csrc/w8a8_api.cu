@@ -173,26 +173,28 @@ int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream) {
   const void* bp = p.b;
   int64_t a_stride = p.rows > 1 ? p.a_stride : w.kp, b_stride = p.k;
   const float* a_scale = p.a_scale;
-  if (quantise && !w.fused) {
-    int8_t* codes = reinterpret_cast<int8_t*>(ws + w.codes);
-    float* scales = reinterpret_cast<float*>(ws + w.scales);
-    rc = launch_quantize_int8(p.a, p.a_stride, p.a_dtype, p.rows, p.k, codes, w.kp, scales, st);
-    if (rc != MTP_OK) return rc;
-    ap = codes;
-    a_stride = w.kp;
-    a_scale = scales;
-  } else if (w.codes >= 0) {
-    rc = launch_pad_rows(p.a, p.a_stride, p.rows, p.k, ws + w.codes, w.kp, st);
-    if (rc != MTP_OK) return rc;
-    ap = ws + w.codes;
-    a_stride = w.kp;
-  }
+  PadJob pad_a = {}, pad_b = {};
   if (w.b >= 0) {
-    rc = launch_pad_rows(p.b, p.k, static_cast<int64_t>(p.num_groups) * p.n, p.k, ws + w.b, w.kp, st);
-    if (rc != MTP_OK) return rc;
+    pad_b = {p.b, p.k, static_cast<int64_t>(p.num_groups) * p.n, p.k, reinterpret_cast<int8_t*>(ws + w.b), w.kp};
     bp = ws + w.b;
     b_stride = w.kp;
   }
+  if (w.codes >= 0) {
+    int8_t* codes = reinterpret_cast<int8_t*>(ws + w.codes);
+    if (quantise) {
+      float* scales = reinterpret_cast<float*>(ws + w.scales);
+      rc = launch_quantize_and_pad(p.a, p.a_stride, p.a_dtype, p.rows, p.k, codes, w.kp, scales, pad_b, st);
+      if (rc != MTP_OK) return rc;
+      pad_b.rows = 0;
+      a_scale = scales;
+    } else {
+      pad_a = {static_cast<const int8_t*>(p.a), a_stride, p.rows, p.k, codes, w.kp};
+    }
+    ap = codes;
+    a_stride = w.kp;
+  }
+  rc = launch_pad_rows(pad_a, pad_b, st);
+  if (rc != MTP_OK) return rc;
   Int8Args a = {};
   a.P = p.rows;
   a.N = p.n;
@@ -361,18 +363,19 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   const void* w13 = p.w13;
   const void* w2 = p.w2;
   int64_t w13_stride = H, w2_stride = I;
+  PadJob pad13 = {}, pad2 = {};
   if (w.w13 >= 0) {
-    rc = launch_pad_rows(p.w13, H, 2ll * E * I, H, ws + w.w13, w.hp, st);
-    if (rc != MTP_OK) return rc;
+    pad13 = {p.w13, H, 2ll * E * I, H, reinterpret_cast<int8_t*>(ws + w.w13), w.hp};
     w13 = ws + w.w13;
     w13_stride = w.hp;
   }
   if (w.w2 >= 0) {
-    rc = launch_pad_rows(p.w2, I, static_cast<int64_t>(E) * H, I, ws + w.w2, w.ip, st);
-    if (rc != MTP_OK) return rc;
+    pad2 = {p.w2, I, static_cast<int64_t>(E) * H, I, reinterpret_cast<int8_t*>(ws + w.w2), w.ip};
     w2 = ws + w.w2;
     w2_stride = w.ip;
   }
+  rc = launch_pad_rows(pad13, pad2, st);
+  if (rc != MTP_OK) return rc;
 
   Int8Args g = {};
   g.P = P;
