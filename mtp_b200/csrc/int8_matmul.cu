@@ -49,7 +49,7 @@ constexpr uint32_t kTIdesc = (2u << 4) | (1u << 7) | (1u << 10);  // D s32, A an
 template <int NT, bool PAIR>
 struct Ring {
   static constexpr int kRows = PAIR ? NT / 2 : NT;
-  static constexpr int kStages = kRows >= 128 ? 5 : kRows == 64 ? 6 : 8;
+  static constexpr int kStages = kRows >= 128 ? 5 : kRows == 64 ? 7 : 8;
   static constexpr uint32_t kBytes = kTWBytes + kRows * kTK;
 };
 
@@ -67,7 +67,7 @@ template <int NT, bool PAIR>
 constexpr size_t tile_smem() {
   return 1024 + static_cast<size_t>(Ring<NT, PAIR>::kStages) * Ring<NT, PAIR>::kBytes + kTEpiWarps * kTStagingBytes + kTCtrl;
 }
-static_assert(tile_smem<256, true>() <= 227 * 1024 && tile_smem<128, false>() <= 227 * 1024 &&
+static_assert(tile_smem<256, true>() <= 227 * 1024 && tile_smem<128, true>() <= 227 * 1024 &&
                   tile_smem<64, false>() <= 227 * 1024 && tile_smem<32, false>() <= 227 * 1024,
               "shared memory");
 
@@ -728,7 +728,7 @@ template <bool GATED>
 int by_rows(Int8Args& a, int nt, int out_dtype, const void* ap, int64_t as, const void* bp, int64_t bs, int sms,
             cudaStream_t st) {
   if (nt == 256) return by_out<256, true, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
-  if (nt == 128) return by_out<128, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
+  if (nt == 128) return by_out<128, true, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
   if (nt == 64) return by_out<64, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
   return by_out<32, false, GATED>(a, out_dtype, ap, as, bp, bs, sms, st);
 }
@@ -744,12 +744,14 @@ int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, in
   if (!a.offsets && !gated && int8_stream_takes(a.P) && (a.K % 16 == 0 || a_padded))
     return launch_int8_stream(a, out_dtype, ap, a_stride, bp, b_stride, st);
   // Rows of a tile: enough for the average group, fewer while the tiles do not
-  // fill the SMs.
+  // fill the SMs. CTA pairs from 128 rows on: at 64 rows a group (16384 rows over
+  // 256 experts) 98.3 us gated and 59.9 us for 2048 x 512, one CTA a tile 101.3
+  // and 58.5; below, a pair's two halves of the rows are too small a box.
   const int per_group = (a.P + a.E - 1) / a.E, width = gated ? a.N / 2 : a.N;
   auto ctas = [&](int nt) {
-    const int channels = (gated ? 64 : kTM) * (nt == 256 ? 2 : 1);
+    const int pair = nt >= 128 ? 2 : 1, channels = (gated ? 64 : kTM) * pair;
     return static_cast<int64_t>((width + channels - 1) / channels) * ((per_group + nt - 1) / nt) *
-           std::min(a.P, a.E) * (nt == 256 ? 2 : 1);
+           std::min(a.P, a.E) * pair;
   };
   int nt = per_group <= 24 ? 32 : per_group <= 48 ? 64 : per_group <= 96 ? 128 : 256;
   while (nt > 32 && ctas(nt) < sms) nt /= 2;
