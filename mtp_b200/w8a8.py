@@ -124,20 +124,18 @@ def _unsort(rows, positions, weights):
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, ids, num_experts, expert_map, row_scales):
-        rows, positions, offsets, scales = _sort(x, ids, num_experts, expert_map, row_scales)
-        ctx.save_for_backward(positions)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(positions, offsets, *([] if scales is None else [scales]))
-        return rows, positions, offsets, scales
+    def forward(ctx, x, ids, num_experts, expert_map, row_scales, rest):
+        # positions, offsets and scales are not differentiable: they go around autograd, in `rest`
+        rows, *others = _sort(x, ids, num_experts, expert_map, row_scales)
+        ctx.save_for_backward(others[0])
+        rest.extend(others)
+        return rows
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_rows, *_):
+    def backward(ctx, grad_rows):
         (positions,) = ctx.saved_tensors
-        if grad_rows is None:
-            return None, None, None, None, None
-        return _unsort(grad_rows.contiguous(), positions, None), None, None, None, None
+        return _unsort(grad_rows.contiguous(), positions, None), None, None, None, None, None
 
 
 class _UnsortTokens(torch.autograd.Function):
@@ -196,7 +194,8 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
         if row_scales.numel() != m:
             raise ValueError(f"row_scales must have {m} entries")
     if hidden_states.requires_grad and torch.is_grad_enabled():
-        return SortedTokens(*_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales))
+        rest = []
+        return SortedTokens(_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales, rest), *rest)
     return SortedTokens(*_sort(hidden_states, topk_ids, num_experts, expert_map, row_scales))
 
 
