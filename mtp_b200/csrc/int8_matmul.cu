@@ -12,7 +12,7 @@
 //             rows (a few of 32 where the tile has few), 128-byte swizzle;
 //             columns past K and rows past the end arrive as zeros. Few large
 //             boxes: with boxes of 32 rows throughout, 8192^2 x 2048 took 113 us
-//             against 98;
+//             against 102;
 //   warp 9    one thread issues tcgen05.mma kind::i8 (K = 32) into one of two
 //             accumulators of NT columns in tensor memory;
 //   warps 0-7 epilogue: each warp takes its 32 channels of every other 32 rows on

@@ -253,9 +253,8 @@ def _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, a_off, b_off) -> in
     return out.value
 
 
-def _product(a, a_scale, b, b_scale, bias, offsets, out_dtype, activation, status):
-    rows, k = a.shape
-    n, groups = b.shape[-2], b.shape[0] if b.dim() == 3 else 1
+def _product(a, a_scale, b, b_scale, bias, offsets, shape, out_dtype, activation, status):
+    rows, k, groups, n = shape
     cols = n // 2 if activation else n
     out = a.new_empty(rows, cols) if out_dtype is a.dtype else a.new_empty(rows, cols, dtype=out_dtype)
     a_dtype, a_stride = DTYPES.get(a.dtype, _INT8), _row_stride("a", a)
@@ -273,18 +272,22 @@ def _product(a, a_scale, b, b_scale, bias, offsets, out_dtype, activation, statu
 
 
 def _check_weight(name, b, scale, ndim, device, k):
+    """Checks weights [(groups,) n, k] and their scales; returns (groups, n)."""
     _tensor(name, b, ndim, _I8, device)
     _tensor(name + "_scale", scale, ndim - 1, _F32, device)
-    if b.shape[-1] != k:
+    *lead, cols = b.shape
+    if cols != k:
         raise ValueError(f"{name} must have {k} columns, got shape {tuple(b.shape)}")
-    if scale.shape != b.shape[:-1]:
-        raise ValueError(f"{name}_scale must be {tuple(b.shape[:-1])}, got {tuple(scale.shape)}")
+    if list(scale.shape) != lead:
+        raise ValueError(f"{name}_scale must be {tuple(lead)}, got {tuple(scale.shape)}")
+    groups, n = lead if ndim == 3 else (1, lead[0])
     if not 1 <= k <= MAX_K:
         raise ValueError(f"1 to {MAX_K} columns are supported, got {k}")
-    if not b.shape[-2] or (ndim == 3 and not b.shape[0]):
+    if not groups or not n:
         raise ValueError(f"{name} must not be empty, got shape {tuple(b.shape)}")
-    if b.numel() // k >= 2 ** 31:
+    if groups * n >= 2 ** 31:
         raise ValueError(f"{name} has 2^31 or more rows")
+    return groups, n
 
 
 def _check_bias(bias, n, device):
@@ -304,10 +307,14 @@ def _check_out(out_dtype, status, device):
 
 
 def _check_rows(a, a_scale):
+    """Checks int8 rows and their scales; returns (rows, k, device)."""
     _tensor("a", a, 2, _I8, contiguous=False)
-    _tensor("a_scale", a_scale, 1, _F32, a.device)
-    if a_scale.numel() != a.shape[0]:
-        raise ValueError(f"a_scale must have {a.shape[0]} entries, got {a_scale.numel()}")
+    device = a.device
+    _tensor("a_scale", a_scale, 1, _F32, device)
+    rows, k = a.shape
+    if a_scale.numel() != rows:
+        raise ValueError(f"a_scale must have {rows} entries, got {a_scale.numel()}")
+    return rows, k, device
 
 
 def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
@@ -318,11 +325,11 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     [N]. The sum is exact in int32; the result is rounded once to ``out_dtype``.
     ``status`` [1] int32 (zeroed by the caller) gets bit 0 if a bounded wait of
     the kernel ran out, in which case the output is wrong."""
-    _check_rows(a, a_scale)
-    _check_weight("b", b, b_scale, 2, a.device, a.shape[1])
-    _check_bias(bias, b.shape[0], a.device)
-    _check_out(out_dtype, status, a.device)
-    return _product(a, a_scale, b, b_scale, bias, None, out_dtype, 0, status)
+    rows, k, device = _check_rows(a, a_scale)
+    _, n = _check_weight("b", b, b_scale, 2, device, k)
+    _check_bias(bias, n, device)
+    _check_out(out_dtype, status, device)
+    return _product(a, a_scale, b, b_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -332,11 +339,12 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     quantised as :func:`quantize_int8` does, in one call; the result has the
     type of ``x`` unless ``out_dtype`` is given."""
     _tensor("x", x, 2, _FLOATS, contiguous=False)
-    _check_weight("weight", weight, weight_scale, 2, x.device, x.shape[1])
-    _check_bias(bias, weight.shape[0], x.device)
+    (rows, k), device = x.shape, x.device
+    _, n = _check_weight("weight", weight, weight_scale, 2, device, k)
+    _check_bias(bias, n, device)
     out_dtype = out_dtype or x.dtype
-    _check_out(out_dtype, status, x.device)
-    return _product(x, None, weight, weight_scale, bias, None, out_dtype, 0, status)
+    _check_out(out_dtype, status, device)
+    return _product(x, None, weight, weight_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
 
 
 def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -348,10 +356,9 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     0); rows before ``offsets[0]`` and from ``offsets[G]`` on are zeros.
     ``activation="silu_mul"``: the first N / 2 channels are gates, and the
     result [P, N / 2] is silu(gate) * up."""
-    _check_rows(a, a_scale)
-    _check_weight("b", b, b_scale, 3, a.device, a.shape[1])
-    _tensor("offsets", offsets, 1, _I32, a.device)
-    groups, n = b.shape[0], b.shape[1]
+    rows, k, device = _check_rows(a, a_scale)
+    groups, n = _check_weight("b", b, b_scale, 3, device, k)
+    _tensor("offsets", offsets, 1, _I32, device)
     if groups > 1024:
         raise ValueError(f"at most 1024 groups are supported, got {groups}")
     if offsets.numel() != groups + 1:
@@ -360,8 +367,9 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
         raise ValueError(f'activation must be None or "silu_mul", got {activation!r}')
     if activation and n % 2:
         raise ValueError(f"silu_mul needs an even number of channels, got {n}")
-    _check_out(out_dtype, status, a.device)
-    return _product(a, a_scale, b, b_scale, None, offsets, out_dtype, _SILU_MUL if activation else 0, status)
+    _check_out(out_dtype, status, device)
+    return _product(a, a_scale, b, b_scale, None, offsets, (rows, k, groups, n), out_dtype,
+                    _SILU_MUL if activation else 0, status)
 
 
 # ---------------------------------------------------------------------------
@@ -394,12 +402,11 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
     _tensor("hidden_states", hidden_states, 2, _FLOATS)
     dev = hidden_states.device
     m, h = hidden_states.shape
-    _check_weight("w13", w13, w13_scale, 3, dev, h)
-    e, i = w13.shape[0], w13.shape[1] // 2
-    if w13.shape[1] != 2 * i:
-        raise ValueError(f"w13 must have gate and up rows, got {w13.shape[1]}")
-    _check_weight("w2", w2, w2_scale, 3, dev, i)
-    if w2.shape != (e, h, i):
+    e, n13 = _check_weight("w13", w13, w13_scale, 3, dev, h)
+    i = n13 // 2
+    if n13 != 2 * i:
+        raise ValueError(f"w13 must have gate and up rows, got {n13}")
+    if _check_weight("w2", w2, w2_scale, 3, dev, i) != (e, h):
         raise ValueError(f"w2 must be {(e, h, i)}, got {tuple(w2.shape)}")
     if e > 1024:
         raise ValueError(f"at most 1024 experts are supported, got {e}")
