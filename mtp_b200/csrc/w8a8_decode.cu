@@ -224,12 +224,9 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, DecodeShared&
     else
       __syncwarp();
   };
-  __threadfence();
   together();
-  if (part == 0 && lane == 0) {
-    d.last[team] = atomicAdd(a.done + s, 1) == d.l.blocks - 1;
-    __threadfence();
-  }
+  // releases what the team wrote and, for the last, acquires what the others did
+  if (part == 0 && lane == 0) d.last[team] = atom_acq_rel_gpu_add(a.done + s, 1) == d.l.blocks - 1;
   together();
   if (!d.last[team]) return;
   T* out = static_cast<T*>(a.out);
