@@ -15,7 +15,10 @@
 //
 // QUANT: the rows come as bf16, fp16 or fp32 and every CTA quantises them itself
 // into shared memory, while its first weights are on their way: a second launch
-// for so few rows costs more than quantising them again in every CTA.
+// for so few rows costs more than quantising them again in every CTA. One row of
+// 2048 to 1024 channels takes 3.8 us, the two kernels of the tile path 8.0; both
+// are latency (2 MB of weights are 0.3 us of HBM). 8192 x 8192 at one row 17 us,
+// 3.9 TB/s.
 #include "quantize.cuh"
 #include "w8a8_common.cuh"
 
