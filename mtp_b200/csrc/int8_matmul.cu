@@ -35,6 +35,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 
 namespace mtp {
 namespace {
@@ -748,18 +749,26 @@ int launch_int8_matmul(Int8Args a, bool gated, int out_dtype, const void* ap, in
   if (!sms) return MTP_ERR_CUDA;
   if (!a.offsets && !gated && int8_stream_takes(a.P) && (a.K % 16 == 0 || a_padded))
     return launch_int8_stream(a, out_dtype, ap, a_stride, bp, b_stride, st);
-  // Rows of a tile: enough for the average group, fewer while the tiles do not
-  // fill the SMs. CTA pairs from 128 rows on: at 64 rows a group (16384 rows over
-  // 256 experts) 98.3 us gated and 59.9 us for 2048 x 512, one CTA a tile 101.3
-  // and 58.5; below, a pair's two halves of the rows are too small a box.
-  const int per_group = (a.P + a.E - 1) / a.E, width = gated ? a.N / 2 : a.N;
-  auto ctas = [&](int nt) {
-    const int pair = nt >= 128 ? 2 : 1, channels = (gated ? 64 : kTM) * pair;
-    return static_cast<int64_t>((width + channels - 1) / channels) * ((per_group + nt - 1) / nt) *
-           std::min(a.P, a.E) * pair;
-  };
-  int nt = per_group <= 24 ? 32 : per_group <= 48 ? 64 : per_group <= 96 ? 128 : 256;
-  while (nt > 32 && ctas(nt) < sms) nt /= 2;
+  // Rows of a tile: the choice of the least time, rounds of tiles over the SMs
+  // times the time of a stage. A stage takes about 0.21, 0.22, 0.235 and 0.35 us
+  // with 32, 64, 128 (CTA pair) and 256 (pair) rows: most of it is issue and
+  // latency until there are 256. So more, smaller tiles only pay while they fit
+  // into one round: 256 x 4096 x 8192 takes 27.9 us with tiles of 32 rows (two
+  // rounds), 16.9 with 64, 17.5 with 128, 24.9 with 256; 512 x 4096 x 2048 16.5,
+  // 10.6, 8.4 and 11.3. Groups differ in size, so on average half a tile of
+  // each is empty: 64 rows a group want 128 (98.3 us; 64: 105.3).
+  const int width = gated ? a.N / 2 : a.N;
+  const double per_group = static_cast<double>(a.P) / a.E, used = std::min(a.P, a.E);
+  int nt = 0;
+  double best = 0;
+  for (int rows = 32, i = 0; rows <= 256; rows *= 2, ++i) {
+    constexpr double kStage[4] = {0.21, 0.22, 0.235, 0.35};
+    const int pair = rows >= 128 ? 2 : 1, channels = (gated ? 64 : kTM) * pair;
+    const double tiles = a.offsets ? used * std::max(1.0, per_group / rows + 0.5) : (a.P + rows - 1) / rows;
+    const double ctas = tiles * ((width + channels - 1) / channels) * pair;
+    const double time = std::ceil(ctas / sms) * kStage[i];
+    if (!nt || time < best) nt = rows, best = time;
+  }
   return gated ? by_rows<true>(a, nt, out_dtype, ap, a_stride, bp, b_stride, sms, st)
                : by_rows<false>(a, nt, out_dtype, ap, a_stride, bp, b_stride, sms, st);
 }
