@@ -241,6 +241,30 @@ def test_int8_grouped_matmul_silu_mul(cuda_device, counts, n, k, dtype):
     assert not out[routed:].any()
 
 
+@pytest.mark.parametrize("counts,n", [([3000, 2500, 2700], 512), ([900, 1, 1100], 520), ([300] * 40, 200)])
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("activation", [None, "silu_mul"])
+def test_grouped_large_groups(cuda_device, counts, n, dtype, activation):
+    """Groups of several tiles of the larger sizes, gated and not."""
+    import mtp_b200
+    g = torch.Generator(device=cuda_device).manual_seed(n + len(counts))
+    a, sa, b, sb, offsets = grouped_case(g, counts, 70, n, 400, cuda_device)
+    sa = sa / 5
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    out = mtp_b200.int8_grouped_matmul(a, sa, b, sb, offsets, out_dtype=dtype, activation=activation, status=status)
+    routed, e = sum(counts), row_group(counts, a.shape[0], cuda_device)
+    acc = grouped_acc(a, b, counts)
+    if activation is None:
+        check_product(out[:routed], acc[:routed], sa[:routed], sb[e][:routed], None, dtype)
+    else:
+        z = (acc * sa.double()[:, None] * sb.double()[e])[:routed]
+        gate, up = z[:, :n // 2], z[:, n // 2:]
+        ref = gate * torch.sigmoid(gate) * up
+        tol = (16 + 4 * gate.abs()) * 2.0 ** -23 * ref.abs() + rounding(ref, dtype) + 1e-30
+        assert ((out[:routed].double() - ref).abs() <= tol).all()
+    assert not out[routed:].any() and int(status) == 0
+
+
 @pytest.mark.parametrize("rows", [12, 900])
 def test_grouped_rows_of_no_group(cuda_device, rows):
     """Rows before offsets[0] are zeros, offsets past the rows are clamped."""
