@@ -353,9 +353,9 @@ MTP_API int mtp_int8_matmul(const MtpInt8MatmulArgs* args, void* stream);
 /* The W8A8 mixture-of-experts layer: router (softmax, top-k, renormalise) or
  * given topk_weights / topk_ids (with expert_map: global ids), rows of
  * hidden_states quantised and sorted by expert, h = silu(gate) * up of the
- * gate_up product kept in fp32, quantised per row, the down product rounded to
- * dtype per pair, and the weighted sum of each token's pairs in fp32 rounded
- * to dtype. w13 [E, 2I, H] (gate rows, then up rows), w2 [E, H, I] int8 with
+ * gate_up product kept in fp32, quantised per row, the down product kept in
+ * fp32, and the weighted sum of each token's pairs in fp32 rounded once to
+ * dtype. A token's result does not depend on the other tokens. w13 [E, 2I, H] (gate rows, then up rows), w2 [E, H, I] int8 with
  * scales [E, 2I] and [E, H].                                                */
 typedef struct MtpW8A8LayerArgs {
   int32_t num_tokens, hidden, inter, num_experts, top_k, renormalize;

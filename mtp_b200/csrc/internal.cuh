@@ -191,7 +191,9 @@ struct UnsortArgs {
   float* grad_weights;         // [M, k] or NULL
 };
 int launch_sort_tokens(const SortArgs& a, cudaStream_t st);
-int launch_unsort_tokens(const UnsortArgs& a, int dtype, bool backward, cudaStream_t st);
+int launch_unsort_tokens(const UnsortArgs& a, int dtype, cudaStream_t st);
+int launch_unsort_fp32_rows(const UnsortArgs& a, int out_dtype, cudaStream_t st);  // rows fp32, out of out_dtype
+int launch_unsort_backward(const UnsortArgs& a, int dtype, cudaStream_t st);
 
 // Rows to int8 (quantize.cu); strides in elements.
 int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,

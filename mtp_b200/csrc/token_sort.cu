@@ -322,7 +322,8 @@ __device__ __forceinline__ void from_floats(const float* f, Vec<__nv_bfloat16, N
 
 constexpr int kSlots = 8;  // slots whose rows a thread has in flight together
 
-template <typename T, int N>
+// T: the rows' type, O: the result's.
+template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
   using V = Vec<T, N>;
   pdl_launch_dependents();
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
   const int32_t* pos = a.positions + t * a.k;
   const float* wt = a.weights ? a.weights + t * a.k : nullptr;
   const T* rows = static_cast<const T*>(a.rows);
-  T* out = static_cast<T*>(a.out) + t * a.H;
+  O* out = static_cast<O*>(a.out) + t * a.H;
   for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
     float acc[N];
 #pragma unroll
@@ -357,9 +358,9 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
           for (int n = 0; n < N; ++n) acc[n] = fmaf(w[j], f[n], acc[n]);
         }
     }
-    V o;
+    Vec<O, N> o;
     from_floats(acc, o);
-    *reinterpret_cast<V*>(out + c) = o;
+    *reinterpret_cast<Vec<O, N>*>(out + c) = o;
   }
 }
 
@@ -466,7 +467,7 @@ __device__ __forceinline__ bool bulk_wait(uint32_t bar, uint32_t parity, bool pa
   return patient && mbar_wait(bar, parity, global_timer_ns() + kBulkTimeoutNs);
 }
 
-template <typename T, int NP, bool BACKWARD>
+template <typename T, typename O, int NP, bool BACKWARD>
 __global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const UnsortArgs a, int slots) {
   constexpr int N = 16 / sizeof(T);
   constexpr int kSeg = NP * 512;  // bytes
@@ -570,12 +571,12 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 1) unsort_bulk_kernel(const U
           for (int n = 0; n < N; ++n) acc[q][n] = fmaf(w, f[n], acc[q][n]);
         }
       }
-      uint8_t* out = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(use.t) * row_bytes + at;
+      O* out = static_cast<O*>(a.out) + static_cast<int64_t>(use.t) * a.H + at / static_cast<int>(sizeof(T));
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
-        V o;
+        Vec<O, N> o;
         from_floats(acc[q], o);
-        if ((q * 32 + lane) * 16 < bytes) *reinterpret_cast<V*>(out + (q * 32 + lane) * 16) = o;
+        if ((q * 32 + lane) * 16 < bytes) *reinterpret_cast<Vec<O, N>*>(out + (q * 32 + lane) * N) = o;
       }
     } else {
       float g[NP][N];
@@ -698,53 +699,75 @@ int sort_run(const SortArgs& a, cudaStream_t st) {
   return launch(sort_copy_kernel<V>, dim3((a.M + block.y - 1) / block.y), block, 0, st, a);
 }
 
-template <typename T, int NP, bool BACKWARD>
+template <typename T, typename O, int NP, bool BACKWARD>
 int bulk_run(const UnsortArgs& a, int slots, int sms, cudaStream_t st) {
-  auto* kernel = unsort_bulk_kernel<T, NP, BACKWARD>;
+  auto* kernel = unsort_bulk_kernel<T, O, NP, BACKWARD>;
   static DeviceRecord record;
   const int rc = allow_shared(record, kernel, kBulkSmem);
   return rc != MTP_OK ? rc : launch(kernel, dim3(sms), dim3(kBulkWarps * 32), kBulkSmem, st, a, slots);
 }
 
+// The widest vector that every row start and length allows.
 template <typename T>
-int unsort_run(const UnsortArgs& a, bool backward, cudaStream_t st) {
-  // the widest vector that every row start and length allows
+int unsort_vector(const UnsortArgs& a) {
   constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.out) |
                          reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.grad_rows) |
                          static_cast<uintptr_t>(static_cast<int64_t>(a.H) * sizeof(T));
-  const int n = (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
-  // Bulk copies where rows are wide (512 bytes: a segment) and there is enough
-  // to fill the rings; a small call is done before that (backward of 8 x 2048
-  // bf16: 512 tokens 11 us against 13 by bulk copies, 1024 tokens 28 against 17).
+  return (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
+}
+
+// Bulk copies where rows are wide (512 bytes: a segment) and there is enough
+// to fill the rings; a small call is done before that (backward of 8 x 2048
+// bf16: 512 tokens 11 us against 13 by bulk copies, 1024 tokens 28 against 17).
+// Returns whether this call is one, with its launch status in rc.
+template <typename T, typename O, bool BACKWARD>
+bool unsort_bulk(const UnsortArgs& a, cudaStream_t st, int& rc) {
   const int64_t row_bytes = static_cast<int64_t>(a.H) * sizeof(T);
-  const int parts = a.k + (backward ? 1 : 0);
-  if (n == kWide && row_bytes >= 512 && row_bytes < (1 << 30) && 2 * parts * 512 <= kBulkRing) {
-    // the widest segment of which a ring holds two tasks
-    int seg = 2048;
-    while (seg > 512 && (2 * parts * seg > kBulkRing || row_bytes < seg)) seg /= 2;
-    const int sms = device_sm_count();
-    if (!sms) return MTP_ERR_CUDA;
-    const int64_t tasks = a.M * (backward ? 1 : (row_bytes + seg - 1) / seg);
-    if (tasks >= (backward ? 4ll : 16ll) * sms) {
-      const int slots = std::min(kBulkSlots, kBulkRing / (parts * seg));
-      switch (seg / 512 * 2 + (backward ? 1 : 0)) {
-        case 8: return bulk_run<T, 4, false>(a, slots, sms, st);
-        case 9: return bulk_run<T, 4, true>(a, slots, sms, st);
-        case 4: return bulk_run<T, 2, false>(a, slots, sms, st);
-        case 5: return bulk_run<T, 2, true>(a, slots, sms, st);
-        case 2: return bulk_run<T, 1, false>(a, slots, sms, st);
-        default: return bulk_run<T, 1, true>(a, slots, sms, st);
-      }
-    }
+  const int parts = a.k + (BACKWARD ? 1 : 0);
+  if (row_bytes < 512 || row_bytes >= (1 << 30) || 2 * parts * 512 > kBulkRing) return false;
+  // the widest segment of which a ring holds two tasks
+  int seg = 2048;
+  while (seg > 512 && (2 * parts * seg > kBulkRing || row_bytes < seg)) seg /= 2;
+  const int sms = device_sm_count();
+  if (!sms) {
+    rc = MTP_ERR_CUDA;
+    return true;
   }
-  const dim3 block = row_block((a.H + n - 1) / n, backward ? 32 : 8);
+  const int64_t tasks = a.M * (BACKWARD ? 1 : (row_bytes + seg - 1) / seg);
+  if (tasks < (BACKWARD ? 4ll : 16ll) * sms) return false;
+  const int slots = std::min(kBulkSlots, kBulkRing / (parts * seg));
+  rc = seg == 2048   ? bulk_run<T, O, 4, BACKWARD>(a, slots, sms, st)
+       : seg == 1024 ? bulk_run<T, O, 2, BACKWARD>(a, slots, sms, st)
+                     : bulk_run<T, O, 1, BACKWARD>(a, slots, sms, st);
+  return true;
+}
+
+// Three kernels for the vectors that unsort_vector gives.
+template <typename F>
+int launch_rows(const UnsortArgs& a, int n, int wide_n, int least, F* wide, F* pair, F* one, cudaStream_t st) {
+  const dim3 block = row_block((a.H + n - 1) / n, least);
   const dim3 grid((a.M + block.y - 1) / block.y);
-  auto pick = [&](auto* wide, auto* pair, auto* one) { return n == kWide ? wide : n == kPair ? pair : one; };
-  if (backward)
-    return launch(pick(unsort_backward_kernel<T, kWide>, unsort_backward_kernel<T, kPair>, unsort_backward_kernel<T, 1>),
-                  grid, block, 0, st, a);
-  return launch(pick(unsort_kernel<T, kWide>, unsort_kernel<T, kPair>, unsort_kernel<T, 1>), grid, block, 0, st, a);
+  return launch(n == wide_n ? wide : n == 1 ? one : pair, grid, block, 0, st, a);
+}
+
+template <typename T, typename O>
+int unsort_forward(const UnsortArgs& a, cudaStream_t st) {
+  constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
+  const int n = unsort_vector<T>(a);
+  int rc;
+  if (n == kWide && unsort_bulk<T, O, false>(a, st, rc)) return rc;
+  return launch_rows(a, n, kWide, 8, unsort_kernel<T, O, kWide>, unsort_kernel<T, O, kPair>, unsort_kernel<T, O, 1>, st);
+}
+
+template <typename T>
+int unsort_backward(const UnsortArgs& a, cudaStream_t st) {
+  constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
+  const int n = unsort_vector<T>(a);
+  int rc;
+  if (n == kWide && unsort_bulk<T, T, true>(a, st, rc)) return rc;
+  return launch_rows(a, n, kWide, 32, unsort_backward_kernel<T, kWide>, unsort_backward_kernel<T, kPair>,
+                     unsort_backward_kernel<T, 1>, st);
 }
 
 }  // namespace
@@ -759,11 +782,27 @@ int launch_sort_tokens(const SortArgs& a, cudaStream_t st) {
   return sort_run<uint8_t>(a, st);
 }
 
-int launch_unsort_tokens(const UnsortArgs& a, int dtype, bool backward, cudaStream_t st) {
+int launch_unsort_tokens(const UnsortArgs& a, int dtype, cudaStream_t st) {
   switch (dtype) {
-    case MTP_DTYPE_BF16: return unsort_run<__nv_bfloat16>(a, backward, st);
-    case MTP_DTYPE_FP16: return unsort_run<__half>(a, backward, st);
-    default: return unsort_run<float>(a, backward, st);
+    case MTP_DTYPE_BF16: return unsort_forward<__nv_bfloat16, __nv_bfloat16>(a, st);
+    case MTP_DTYPE_FP16: return unsort_forward<__half, __half>(a, st);
+    default: return unsort_forward<float, float>(a, st);
+  }
+}
+
+int launch_unsort_fp32_rows(const UnsortArgs& a, int out_dtype, cudaStream_t st) {
+  switch (out_dtype) {
+    case MTP_DTYPE_BF16: return unsort_forward<float, __nv_bfloat16>(a, st);
+    case MTP_DTYPE_FP16: return unsort_forward<float, __half>(a, st);
+    default: return unsort_forward<float, float>(a, st);
+  }
+}
+
+int launch_unsort_backward(const UnsortArgs& a, int dtype, cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return unsort_backward<__nv_bfloat16>(a, st);
+    case MTP_DTYPE_FP16: return unsort_backward<__half>(a, st);
+    default: return unsort_backward<float>(a, st);
   }
 }
 

@@ -109,7 +109,7 @@ int mtp_unsort_tokens(const void* rows, int64_t num_rows, int32_t dtype, const i
   a.positions = positions;
   a.weights = weights;
   a.out = out;
-  return launch_unsort_tokens(a, dtype, false, static_cast<cudaStream_t>(stream));
+  return launch_unsort_tokens(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int mtp_unsort_tokens_backward(const void* grad, const void* rows, int64_t num_rows, int32_t dtype,
@@ -132,7 +132,7 @@ int mtp_unsort_tokens_backward(const void* grad, const void* rows, int64_t num_r
   a.grad = grad;
   a.grad_rows = grad_rows;
   a.grad_weights = grad_weights;
-  return launch_unsort_tokens(a, dtype, true, static_cast<cudaStream_t>(stream));
+  return launch_unsort_backward(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int mtp_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t K, int8_t* q,
@@ -264,7 +264,7 @@ LayerWs8 layer_ws8(const MtpW8A8LayerArgs& a) {
   w.h = c.take(4 * p * a.inter);
   w.hq = c.take(p * w.ip);
   w.hs = c.take(4 * p);
-  w.y = c.take(p * a.hidden * dtype_bytes(a.dtype));
+  w.y = c.take(4 * p * a.hidden);
   w.w13 = tma_rows_ok(a.w13, a.hidden) ? -1 : c.take(2ll * a.num_experts * a.inter * w.hp);
   w.w2 = tma_rows_ok(a.w2, a.inter) ? -1 : c.take(static_cast<int64_t>(a.num_experts) * a.hidden * w.ip);
   w.total = c.at;
@@ -397,7 +397,9 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   g.a_scale = f32(w.hs);
   g.b_scale = p.w2_scale;
   g.out = ws + w.y;
-  rc = launch_int8_matmul(g, false, p.dtype, ws + w.hq, w.ip, true, w2, w2_stride, st);
+  // y in fp32, as the few-token kernels hold it: an fp16 pair may pass 65504 where the weighted sum does
+  // not, and a token's result does not depend on the others of its call
+  rc = launch_int8_matmul(g, false, MTP_DTYPE_FP32, ws + w.hq, w.ip, true, w2, w2_stride, st);
   if (rc != MTP_OK) return rc;
 
   UnsortArgs u = {};
@@ -409,7 +411,7 @@ int mtp_w8a8_moe_layer(const MtpW8A8LayerArgs* args, void* stream) {
   u.positions = i32(w.positions);
   u.weights = weights;
   u.out = p.out;
-  return launch_unsort_tokens(u, p.dtype, false, st);
+  return launch_unsort_fp32_rows(u, p.dtype, st);
 }
 
 }  // extern "C"
