@@ -199,7 +199,7 @@ int launch_unsort_backward(const UnsortArgs& a, int dtype, cudaStream_t st);
 int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
                          float* scale, cudaStream_t st);
 
-// Contiguous rows to int8 and their tokens' top-k (as launch_router_topk).
+// Contiguous rows to int8 and their tokens' top-k (route_token).
 int launch_route_quantize(const void* x, int dtype, int M, int K, int8_t* q, int64_t q_stride, float* scale,
                           const float* logits, int E, int k, int renorm, float* weights, int32_t* ids,
                           cudaStream_t st);

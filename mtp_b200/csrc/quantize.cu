@@ -125,33 +125,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   quantize_rows<T, WPR>(blockIdx.x, x, x_stride, M, K, q, q_stride, scale);
 }
 
-// The rows of a layer quantised and its tokens routed, which do not depend on
-// each other, in one launch: the first CTAs route 8 tokens each (a warp a
-// token), the others quantise.
-template <typename T, int WPR, int VPT>
-__global__ void __launch_bounds__(256) route_quantize_kernel(const T* __restrict__ x, int M, int K,
-                                                             int8_t* __restrict__ q, int64_t q_stride,
-                                                             float* __restrict__ scale, const float* __restrict__ logits,
-                                                             int E, int k, int renorm, float* __restrict__ weights,
-                                                             int32_t* __restrict__ ids) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int routing = (M + 7) / 8;
-  if (static_cast<int>(blockIdx.x) >= routing) {
-    quantize_rows<T, WPR>(blockIdx.x - routing, x, K, M, K, q, q_stride, scale);
-    return;
-  }
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= M) return;
-  float w;
-  int id;
-  route_token<VPT>(logits + static_cast<int64_t>(t) * E, E, k, renorm, &w, &id);
-  if (lane < k) {
-    weights[static_cast<int64_t>(t) * k + lane] = w;
-    ids[static_cast<int64_t>(t) * k + lane] = id;
-  }
-}
-
 // Any alignment: a row per CTA, read twice.
 template <typename T>
 __device__ __forceinline__ void quantize_any(int64_t m, const T* __restrict__ x, int64_t x_stride, int K,
@@ -168,6 +141,36 @@ __device__ __forceinline__ void quantize_any(int64_t m, const T* __restrict__ x,
     uint32_t w;
     codes_of<4>(v, r, &w);
     q[m * q_stride + c] = static_cast<int8_t>(w);
+  }
+}
+
+// The rows of a layer quantised and its tokens routed, which do not depend on
+// each other, in one launch: the first CTAs route 8 tokens each (a warp a
+// token), the others quantise (WPR 0: rows of any alignment).
+template <typename T, int WPR, int VPT>
+__global__ void __launch_bounds__(256) route_quantize_kernel(const T* __restrict__ x, int M, int K,
+                                                             int8_t* __restrict__ q, int64_t q_stride,
+                                                             float* __restrict__ scale, const float* __restrict__ logits,
+                                                             int E, int k, int renorm, float* __restrict__ weights,
+                                                             int32_t* __restrict__ ids) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int routing = (M + 7) / 8;
+  if (static_cast<int>(blockIdx.x) >= routing) {
+    if constexpr (WPR == 0)
+      quantize_any(blockIdx.x - routing, x, K, K, q, q_stride, scale);
+    else
+      quantize_rows<T, WPR>(blockIdx.x - routing, x, K, M, K, q, q_stride, scale);
+    return;
+  }
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= M) return;
+  float w;
+  int id;
+  route_token<VPT>(logits + static_cast<int64_t>(t) * E, E, k, renorm, &w, &id);
+  if (lane < k) {
+    weights[static_cast<int64_t>(t) * k + lane] = w;
+    ids[static_cast<int64_t>(t) * k + lane] = id;
   }
 }
 
@@ -271,8 +274,9 @@ int warps_per_row(int M, int K) {
 template <typename T, int WPR, int VPT>
 int run_routed(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* scale, const float* logits, int E, int k,
                int renorm, float* weights, int32_t* ids, cudaStream_t st) {
-  return launch(route_quantize_kernel<T, WPR, VPT>, (M + 7) / 8 + (static_cast<int64_t>(M) * WPR + 7) / 8, st,
-                static_cast<const T*>(x), M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids);
+  const int64_t rows = WPR ? (static_cast<int64_t>(M) * WPR + 7) / 8 : M;
+  return launch(route_quantize_kernel<T, WPR, VPT>, (M + 7) / 8 + rows, st, static_cast<const T*>(x), M, K, q,
+                q_stride, scale, logits, E, k, renorm, weights, ids);
 }
 
 template <typename T, int WPR>
@@ -283,12 +287,10 @@ int by_experts(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* 
 }
 
 template <typename T>
-int route_and_quantize(const void* x, int dtype, int M, int K, int8_t* q, int64_t q_stride, float* scale,
+int route_and_quantize(const void* x, int M, int K, int8_t* q, int64_t q_stride, float* scale,
                        const float* logits, int E, int k, int renorm, float* weights, int32_t* ids, cudaStream_t st) {
-  if (!wide_rows<T>(x, K, K, q, q_stride)) {
-    const int rc = launch_router_topk(logits, M, E, k, renorm, weights, ids, nullptr, st);
-    return rc != MTP_OK ? rc : launch_quantize_int8(x, K, dtype, M, K, q, q_stride, scale, st);
-  }
+  if (!wide_rows<T>(x, K, K, q, q_stride))
+    return by_experts<T, 0>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
   return warps_per_row<T>(M, K) == 1
              ? by_experts<T, 1>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st)
              : by_experts<T, 8>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
@@ -330,11 +332,11 @@ int launch_route_quantize(const void* x, int dtype, int M, int K, int8_t* q, int
                           cudaStream_t st) {
   switch (dtype) {
     case MTP_DTYPE_BF16:
-      return route_and_quantize<__nv_bfloat16>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+      return route_and_quantize<__nv_bfloat16>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
     case MTP_DTYPE_FP16:
-      return route_and_quantize<__half>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+      return route_and_quantize<__half>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
     default:
-      return route_and_quantize<float>(x, dtype, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
+      return route_and_quantize<float>(x, M, K, q, q_stride, scale, logits, E, k, renorm, weights, ids, st);
   }
 }
 

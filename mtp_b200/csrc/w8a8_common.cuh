@@ -26,8 +26,10 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 out_cast(float v) { return __float2bfloat16_rn(v); }
 
 // One warp's top-k of a token: the operations of router_token (route.cuh), so
-// the same ids and weights, with each round's maximum and its lowest index as
-// warp reductions over integers that order like the logits.
+// the same ids and weights where the logits are numbers, with each round's
+// maximum and its lowest index as warp reductions over integers that order like
+// the logits. NaN logits are chosen last. A token with one has NaN weights and,
+// unlike there, always ids of experts, so that its result is NaN.
 template <int VPT>
 __device__ __forceinline__ void route_token(const float* __restrict__ row, int E, int k, int renorm, float* w_out,
                                             int* id_out) {
