@@ -507,7 +507,7 @@ __device__ void tile_epilogue(const Int8Args& a, TileCtrl& cb, uint8_t* staging,
               const float z1 = __int2float_rn(static_cast<int>(v[j + q + 1])) * s[q + 1] * sc.sb;
               const float got = __shfl_xor_sync(kFullMask, lane < 16 ? z1 : z0, 16);
               const float gate = lane < 16 ? z0 : got, up = lane < 16 ? got : z1;
-              o[q / 2] = silu_fast(gate) * up;
+              o[q / 2] = (sizeof(T) == 4 ? silu_fp32(gate) : silu_fast(gate)) * up;
             }
             put2(at + j * kRow, 2 * kRow, o[0], o[1], T());
           }

@@ -303,7 +303,7 @@ __device__ __forceinline__ void decode_units(const DecodeArgs& a, DecodeShared& 
         if (t % ks != part || ch0 >= width) continue;
         const float sa = d.scale[pair / a.k];
         const float gate = __int2float_rn(sum(t)) * sa * sb0, up = __int2float_rn(sum(2 + t)) * sa * sb1;
-        a.h[static_cast<int64_t>(pair) * a.I + ch0] = silu_fast(gate) * up;
+        a.h[static_cast<int64_t>(pair) * a.I + ch0] = silu_fp32(gate) * up;
       } else {
         const float sa = d.scale[8 * (blk - first) + col];
         float* o = a.y + static_cast<int64_t>(pair) * a.H;
