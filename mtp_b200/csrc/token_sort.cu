@@ -326,8 +326,12 @@ constexpr int kSlots = 8;  // slots whose rows a thread has in flight together
 template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a) {
   using V = Vec<T, N>;
-  pdl_launch_dependents();
+  // The next kernel only after the wait: launched before it, its CTAs (and those
+  // of the kernels behind it) take their places while the producer of the rows
+  // still runs. The W8A8 layer of 16 tokens 71.2 -> 66.6 us, sort and unsort of
+  // 64 tokens x 8 x 2048 bf16 7.4 -> 5.2 (unsort alone, 256 tokens: 2.4 -> 2.6).
   pdl_wait();
+  pdl_launch_dependents();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (t >= a.M) return;
   const int32_t* pos = a.positions + t * a.k;
