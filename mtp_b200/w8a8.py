@@ -15,7 +15,8 @@ Pair order, ``-1`` ids and ``expert_map`` follow :func:`mtp_b200.moe_align_block
 and :func:`mtp_b200.moe_layer_w4a16`. Shape, dtype and device errors raise
 ``ValueError`` before any launch; a non-zero C status raises
 :class:`mtp_b200.MtpError`. Every call is asynchronous on the current torch
-CUDA stream. There is no CPU path.
+stream of its tensors' GPU, which need not be the current one. There is no CPU
+path.
 """
 from __future__ import annotations
 
@@ -40,8 +41,19 @@ _quantize_entry = _lib.Entry("mtp_quantize_int8")
 _matmul_entry = _lib.Entry("mtp_int8_matmul")
 _layer_entry = _lib.Entry("mtp_w8a8_moe_layer")
 
-# The handle of the current stream of a device (torch.cuda.current_stream builds a Stream object around it).
-_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current device, and the handle of a device's current stream (torch.cuda.current_stream builds a Stream object around it).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+           or (lambda device: torch.cuda.current_stream(device).cuda_stream))
+
+
+def _launch(entry: _lib.Entry, device: int, *args) -> None:
+    """``entry(*args, stream)`` with ``device`` current, as the C side launches on the current device."""
+    if device == _current_device():
+        entry(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            entry(*args, _stream(device))
 
 
 def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None, contiguous: bool = True):
@@ -104,11 +116,11 @@ def _sort(x, ids, num_experts, expert_map, row_scales):
     positions = torch.empty_like(ids)
     offsets = ids.new_empty(num_experts + 1)
     scales = None if row_scales is None else row_scales.new_empty(m * k)
-    _sort_entry(x.data_ptr() or None, _row_stride("hidden_states", x), DTYPES.get(x.dtype, _INT8), m, h,
-              ids.data_ptr(), k, num_experts, None if expert_map is None else expert_map.data_ptr(),
-              0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
-              rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(),
-              offsets.data_ptr(), _stream(x.get_device()))
+    _launch(_sort_entry, x.get_device(), x.data_ptr() or None, _row_stride("hidden_states", x),
+            DTYPES.get(x.dtype, _INT8), m, h, ids.data_ptr(), k, num_experts,
+            None if expert_map is None else expert_map.data_ptr(),
+            0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
+            rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(), offsets.data_ptr())
     return rows, positions, offsets, scales
 
 
@@ -116,10 +128,20 @@ def _unsort(rows, positions, weights):
     m, k = positions.shape
     r, h = rows.shape
     out = rows.new_empty(m, h)
-    _unsort_entry(rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
-                  None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr(),
-                  _stream(rows.get_device()))
+    _launch(_unsort_entry, rows.get_device(), rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
+            None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr())
     return out
+
+
+def _unsort_backward(grad, rows, num_rows, positions, weights, need_rows, need_weights):
+    (m, k), h = positions.shape, grad.shape[1]
+    grad_rows = grad.new_empty(num_rows, h) if need_rows else None
+    grad_weights = torch.empty_like(weights) if need_weights else None
+    _launch(_unsort_backward_entry, grad.get_device(), grad.data_ptr(), None if rows is None else rows.data_ptr(),
+            num_rows, DTYPES[grad.dtype], positions.data_ptr(), None if weights is None else weights.data_ptr(), m, k, h,
+            None if grad_rows is None else grad_rows.data_ptr(),
+            None if grad_weights is None else grad_weights.data_ptr())
+    return grad_rows, grad_weights
 
 
 class _SortTokens(torch.autograd.Function):
@@ -149,16 +171,9 @@ class _UnsortTokens(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         rows, positions, weights = ctx.saved_tensors
-        grad = grad.contiguous()
-        (m, k), h = positions.shape, grad.shape[1]
         need_rows, _, need_weights = ctx.needs_input_grad
-        grad_rows = grad.new_empty(ctx.num_rows, h) if need_rows else None
-        grad_weights = torch.empty_like(weights) if need_weights else None
-        _unsort_backward_entry(grad.data_ptr(), None if rows is None else rows.data_ptr(), ctx.num_rows,
-                               DTYPES[grad.dtype], positions.data_ptr(),
-                               None if weights is None else weights.data_ptr(), m, k, h,
-                               None if grad_rows is None else grad_rows.data_ptr(),
-                               None if grad_weights is None else grad_weights.data_ptr(), _stream(grad.get_device()))
+        grad_rows, grad_weights = _unsort_backward(grad.contiguous(), rows, ctx.num_rows, positions, weights, need_rows,
+                                                   need_weights)
         return grad_rows, None, grad_weights
 
 
@@ -238,8 +253,8 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     kp = (k + 15) // 16 * 16
     codes = x.new_empty(m, kp, dtype=torch.int8)
     scale = x.new_empty(m, dtype=torch.float32)
-    _quantize_entry(x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(), kp, scale.data_ptr(),
-                    _stream(x.get_device()))
+    _launch(_quantize_entry, x.get_device(), x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k,
+            codes.data_ptr(), kp, scale.data_ptr())
     return codes if kp == k else codes[:, :k], scale
 
 
@@ -267,7 +282,7 @@ def _product(a, a_scale, b, b_scale, bias, offsets, shape, out_dtype, activation
                                   None if offsets is None else offsets.data_ptr(), out.data_ptr(),
                                   None if status is None else status.data_ptr(),
                                   None if ws is None else ws.data_ptr(), size)
-    _matmul_entry(C.byref(args), _stream(a.get_device()))
+    _launch(_matmul_entry, a.get_device(), C.byref(args))
     return out
 
 
@@ -449,5 +464,5 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
                                  None if expert_map is None else expert_map.data_ptr(), p13, w13_scale.data_ptr(), p2,
                                  w2_scale.data_ptr(), out.data_ptr(), None if status is None else status.data_ptr(),
                                  ws.data_ptr(), size)
-    _layer_entry(C.byref(args), _stream(hidden_states.get_device()))
+    _launch(_layer_entry, hidden_states.get_device(), C.byref(args))
     return out
