@@ -23,6 +23,8 @@ class Entries:
         monkeypatch.setattr(w8a8, "_current_device", lambda: self.current, raising=False)
         monkeypatch.setattr(w8a8, "_stream", lambda device: 1000 + device)
         monkeypatch.setattr(torch.cuda, "device", self.device)
+        # fake tensors of a GPU that is not there, wherever this runs
+        monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
 
     @contextlib.contextmanager
     def device(self, index):
@@ -45,7 +47,7 @@ def calls(z):
         ("quantize", lambda: mtp_b200.quantize_int8(x)),
         ("matmul", lambda: mtp_b200.int8_matmul(a, sa, b, sb)),
         ("matmul", lambda: mtp_b200.int8_linear(x, b, sb)),
-        ("matmul", lambda: mtp_b200.int8_grouped_matmul(a, sa, b[None], sb[None], z(2, dtype=I32))),
+        ("matmul", lambda: mtp_b200.int8_grouped_matmul(a, sa, z(2, 6, 16, dtype=I8), z(2, 6), z(3, dtype=I32))),
         ("layer", lambda: mtp_b200.moe_layer_w8a8(x, z(4, 3), w13, s13, w2, s2, 2)),
         ("layer", lambda: mtp_b200.moe_layer_w8a8(x, None, w13, s13, w2, s2, 2, topk_weights=w, topk_ids=ids)),
     ]
