@@ -282,7 +282,8 @@ enum MtpDtype {
  * x: any MtpDtype, rows x_stride elements apart; x and rows both NULL: positions
  * and offsets only. row_scales [M] (with sorted_scales [M*k]): one fp32 per
  * row, sorted along (0 for a pair without an expert). num_experts <= 1024,
- * k <= 32, M * k < 2^31. The gradient of x is mtp_unsort_tokens of the rows'
+ * k <= 32; H and M * k up to 2^31 - 65536, as are all counts of rows, columns
+ * and channels (num_groups * n) of this section and the next. The gradient of x is mtp_unsort_tokens of the rows'
  * gradient without weights. Same pair order as mtp_moe_align.              */
 MTP_API int mtp_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t H,
                             const int32_t* topk_ids, int32_t k, int32_t num_experts, const int32_t* expert_map,

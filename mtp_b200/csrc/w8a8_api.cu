@@ -19,6 +19,10 @@ struct Carver {
 };
 
 constexpr int kMaxK = 131071;  // 128 * 128 * k stays below 2^31
+// Rows, columns, pairs and channels of a call: the kernels index them in 32
+// bits, and their loops step past the last one by up to 32768.
+constexpr int64_t kMaxExtent = 0x7fffffffll - 0xffff;
+bool extent(int64_t n) { return n >= 0 && n <= kMaxExtent; }
 
 struct MatmulWs {
   int64_t codes, scales, b, total;  // -1: not needed
@@ -27,9 +31,9 @@ struct MatmulWs {
 };
 
 int matmul_shapes(const MtpInt8MatmulArgs& a) {
-  if (a.rows < 0 || a.n < 1 || a.k < 1 || a.k > kMaxK) return MTP_ERR_SHAPE;
+  if (!extent(a.rows) || a.n < 1 || a.k < 1 || a.k > kMaxK) return MTP_ERR_SHAPE;
   if (a.num_groups < 1 || a.num_groups > 1024 || (!a.offsets && a.num_groups != 1)) return MTP_ERR_SHAPE;
-  if (static_cast<int64_t>(a.num_groups) * a.n >= (1ll << 31) || a.a_stride < (a.rows > 1 ? a.k : 0))
+  if (!extent(static_cast<int64_t>(a.num_groups) * a.n) || a.a_stride < (a.rows > 1 ? a.k : 0))
     return MTP_ERR_SHAPE;
   if ((a.a_dtype != MTP_DTYPE_INT8 && !float_dtype(a.a_dtype)) || !float_dtype(a.out_dtype)) return MTP_ERR_ARG;
   if (a.activation != MTP_ACT_NONE && a.activation != MTP_ACT_SILU_MUL) return MTP_ERR_ARG;
@@ -61,8 +65,8 @@ int mtp_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, i
                     void* stream) {
   if (!offsets || (M > 0 && (!topk_ids || !positions)) || (x && M > 0 && !rows) || (row_scales && !sorted_scales))
     return MTP_ERR_NULL;
-  if (M < 0 || H < 0 || k < 1 || k > 32 || num_experts < 1 || num_experts > 1024 ||
-      static_cast<int64_t>(M) * k >= 0x7fffffffll || (expert_map && global_num_experts < 1) || (x && x_stride < 0))
+  if (M < 0 || !extent(H) || k < 1 || k > 32 || num_experts < 1 || num_experts > 1024 ||
+      !extent(static_cast<int64_t>(M) * k) || (expert_map && global_num_experts < 1) || (x && x_stride < 0))
     return MTP_ERR_SHAPE;
   if (!float_dtype(dtype) && dtype != MTP_DTYPE_INT8) return MTP_ERR_ARG;
   const int64_t size = dtype_bytes(dtype);
@@ -87,8 +91,7 @@ int mtp_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, i
 }
 
 static int unsort_shapes(int64_t num_rows, int32_t dtype, int32_t M, int32_t k, int32_t H) {
-  if (M < 0 || H < 0 || k < 1 || k > 32 || num_rows < 0 || num_rows >= 0x7fffffffll ||
-      static_cast<int64_t>(M) * k >= 0x7fffffffll)
+  if (M < 0 || !extent(H) || k < 1 || k > 32 || !extent(num_rows) || !extent(static_cast<int64_t>(M) * k))
     return MTP_ERR_SHAPE;
   return float_dtype(dtype) ? MTP_OK : MTP_ERR_ARG;
 }
@@ -137,7 +140,7 @@ int mtp_unsort_tokens_backward(const void* grad, const void* rows, int64_t num_r
 
 int mtp_quantize_int8(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t K, int8_t* q,
                       int64_t q_stride, float* scale, void* stream) {
-  if (M < 0 || K < 1 || x_stride < 0 || q_stride < (M > 1 ? K : 0)) return MTP_ERR_SHAPE;
+  if (!extent(M) || K < 1 || !extent(K) || x_stride < 0 || q_stride < (M > 1 ? K : 0)) return MTP_ERR_SHAPE;
   if (!float_dtype(dtype)) return MTP_ERR_ARG;
   if (M == 0) return MTP_OK;
   if (!x || !q || !scale) return MTP_ERR_NULL;
@@ -226,9 +229,8 @@ int layer_shapes(const MtpW8A8LayerArgs& a) {
       a.num_experts > 1024 || a.top_k < 1 || a.top_k > 32)
     return MTP_ERR_SHAPE;
   if (a.router_logits && a.top_k > a.num_experts) return MTP_ERR_SHAPE;
-  if (static_cast<int64_t>(a.num_tokens) * a.top_k >= 0x7fffffffll ||
-      static_cast<int64_t>(a.num_experts) * 2 * a.inter >= (1ll << 31) ||
-      static_cast<int64_t>(a.num_experts) * a.hidden >= (1ll << 31))
+  if (!extent(static_cast<int64_t>(a.num_tokens) * a.top_k) || !extent(static_cast<int64_t>(a.num_experts) * 2 * a.inter) ||
+      !extent(static_cast<int64_t>(a.num_experts) * a.hidden))
     return MTP_ERR_SHAPE;
   if (a.expert_map) {
     if (a.router_logits) return MTP_ERR_ARG;
