@@ -31,6 +31,7 @@ from . import _lib
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MtpDtype
 _INT8 = 3
 MAX_K = 131071  # 128 * 128 * K stays below 2^31
+MAX_EXTENT = 2 ** 31 - 65536  # rows, columns, pairs and channels of a call (ctypes would cut larger ones to 32 bits)
 _SILU_MUL = 1
 
 
@@ -70,6 +71,19 @@ def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None,
         raise ValueError(f"{name} must be {ndim}-D, got shape {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _extent(what: str, n: int):
+    if n > MAX_EXTENT:
+        raise ValueError(f"at most {MAX_EXTENT} {what} are supported, got {n}")
+
+
+def _check_map(expert_map: torch.Tensor | None, device: torch.device):
+    if expert_map is not None:
+        _tensor("expert_map", expert_map, 1, _I32, device)
+        if not expert_map.numel():
+            raise ValueError("expert_map is empty")
+        _extent("entries of expert_map", expert_map.numel())
 
 
 _F32 = (torch.float32,)
@@ -198,12 +212,9 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
         raise ValueError(f"topk_ids must have 1 to 32 columns, got {k}")
     if not 1 <= num_experts <= 1024:
         raise ValueError(f"num_experts must be in [1, 1024], got {num_experts}")
-    if m * k >= 2 ** 31 - 1:
-        raise ValueError(f"at most 2^31 - 2 pairs are supported, got {m * k}")
-    if expert_map is not None:
-        _tensor("expert_map", expert_map, 1, _I32, dev)
-        if not expert_map.numel():
-            raise ValueError("expert_map is empty")
+    _extent("pairs", m * k)
+    _extent("columns", hidden_states.shape[1])
+    _check_map(expert_map, dev)
     if row_scales is not None:
         _tensor("row_scales", row_scales, 1, _F32, dev)
         if row_scales.numel() != m:
@@ -228,6 +239,8 @@ def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
         raise ValueError(f"positions must have 1 to 32 columns, got {k}")
     if rows.shape[0] != m * k:
         raise ValueError(f"rows must have one row per pair, {m * k}, got {rows.shape[0]}")
+    _extent("pairs", m * k)
+    _extent("columns", rows.shape[1])
     if topk_weights is not None:
         _tensor("topk_weights", topk_weights, 2, _F32, rows.device)
         if topk_weights.shape != positions.shape:
@@ -250,6 +263,8 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     if k < 1:
         raise ValueError("x must have at least one column")
+    _extent("rows", m)
+    _extent("columns", k)
     kp = (k + 15) // 16 * 16
     codes = x.new_empty(m, kp, dtype=torch.int8)
     scale = x.new_empty(m, dtype=torch.float32)
@@ -300,8 +315,7 @@ def _check_weight(name, b, scale, ndim, device, k):
         raise ValueError(f"1 to {MAX_K} columns are supported, got {k}")
     if not groups or not n:
         raise ValueError(f"{name} must not be empty, got shape {tuple(b.shape)}")
-    if groups * n >= 2 ** 31:
-        raise ValueError(f"{name} has 2^31 or more rows")
+    _extent(f"rows of {name}", groups * n)
     return groups, n
 
 
@@ -329,6 +343,7 @@ def _check_rows(a, a_scale):
     rows, k = a.shape
     if a_scale.numel() != rows:
         raise ValueError(f"a_scale must have {rows} entries, got {a_scale.numel()}")
+    _extent("rows", rows)
     return rows, k, device
 
 
@@ -355,6 +370,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     type of ``x`` unless ``out_dtype`` is given."""
     _tensor("x", x, 2, _FLOATS, contiguous=False)
     (rows, k), device = x.shape, x.device
+    _extent("rows", rows)
     _, n = _check_weight("weight", weight, weight_scale, 2, device, k)
     _check_bias(bias, n, device)
     out_dtype = out_dtype or x.dtype
@@ -427,6 +443,7 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
         raise ValueError(f"at most 1024 experts are supported, got {e}")
     if not 1 <= top_k <= 32:
         raise ValueError(f"top_k must be in [1, 32], got {top_k}")
+    _extent("pairs", m * top_k)
     if router_logits is not None:
         _tensor("router_logits", router_logits, 2, _F32, dev)
         if router_logits.shape != (m, e):
@@ -442,10 +459,7 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
         _tensor("topk_ids", topk_ids, 2, _I32, dev)
         if topk_weights.shape != (m, top_k) or topk_ids.shape != (m, top_k):
             raise ValueError(f"topk_weights/topk_ids must be {(m, top_k)}")
-    if expert_map is not None:
-        _tensor("expert_map", expert_map, 1, _I32, dev)
-        if not expert_map.numel():
-            raise ValueError("expert_map is empty")
+    _check_map(expert_map, dev)
     if out is None:
         out = torch.empty_like(hidden_states)
     else:

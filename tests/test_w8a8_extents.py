@@ -1,8 +1,11 @@
 """Sizes that the kernels' 32-bit indexes do not hold are refused before a launch: at the C entries from
-2^31 - 65535 on (their loops step past the last element by up to 32768)."""
+2^31 - 65535 on (their loops step past the last element by up to 32768), and in Python, whose ctypes would cut
+2^32 + 8 to 8 without a word."""
 import ctypes as C
 
 import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 LIMIT = 2 ** 31 - 65536
 SHAPE, LAST = 2, 2 ** 31 - 1
@@ -68,3 +71,50 @@ def test_c_entries_take_the_largest_sizes(entries):
     assert entries["matmul_size"](n=2 ** 21 - 64, groups=1024) == 0
     assert entries["layer_size"](m=LIMIT, k=1) == 0
     assert entries["layer_size"](m=LIMIT // 8, k=8) == 0
+
+
+I32, I8, BF = torch.int32, torch.int8, torch.bfloat16
+
+
+def calls(z, n):
+    """Every public function with a size of n, on tensors that z makes."""
+    import mtp_b200 as p
+    ids = z(2, 1, dtype=I32)
+    layer = (z(3, 8, 16, dtype=I8), z(3, 8), z(3, 16, 4, dtype=I8), z(3, 16), 1)
+    return {
+        "sort columns": lambda: p.sort_tokens(z(2, n, dtype=BF), ids, 3),
+        "sort pairs": lambda: p.sort_tokens(z(n, 4, dtype=BF), z(n, 1, dtype=I32), 3),
+        "sort map": lambda: p.sort_tokens(z(2, 4), ids, 3, expert_map=z(n, dtype=I32)),
+        "unsort columns": lambda: p.unsort_tokens(z(2, n, dtype=BF), ids),
+        "unsort pairs": lambda: p.unsort_tokens(z(n, 4, dtype=BF), z(n, 1, dtype=I32)),
+        "quantize columns": lambda: p.quantize_int8(z(1, n, dtype=BF)),
+        "quantize rows": lambda: p.quantize_int8(z(n, 1, dtype=BF)),
+        "matmul rows": lambda: p.int8_matmul(z(n, 16, dtype=I8), z(n), z(4, 16, dtype=I8), z(4)),
+        "matmul channels": lambda: p.int8_matmul(z(2, 16, dtype=I8), z(2), z(n, 16, dtype=I8), z(n)),
+        "linear rows": lambda: p.int8_linear(z(n, 16), z(4, 16, dtype=I8), z(4)),
+        "grouped rows": lambda: p.int8_grouped_matmul(z(n, 16, dtype=I8), z(n), z(1, 4, 16, dtype=I8), z(1, 4), z(2, dtype=I32)),
+        "grouped channels": lambda: p.int8_grouped_matmul(z(2, 16, dtype=I8), z(2), z(4, n, 16, dtype=I8), z(4, n), z(5, dtype=I32)),
+        "layer tokens": lambda: p.moe_layer_w8a8(z(n, 16), z(n, 3), *layer),
+        "layer map": lambda: p.moe_layer_w8a8(z(2, 16), None, *layer, topk_weights=z(2, 1), topk_ids=ids, expert_map=z(n, dtype=I32)),
+    }
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+@pytest.mark.parametrize("n", [LIMIT + 1, 2 ** 31, 2 ** 32 + 8])
+def test_python_refuses_what_32_bits_do_not_index(built_lib, monkeypatch, n):
+    from mtp_b200 import w8a8
+    for entry in ("sort", "unsort", "quantize", "matmul", "layer"):
+        monkeypatch.setattr(w8a8, f"_{entry}_entry", lambda *args: None)
+    monkeypatch.setattr(w8a8, "_current_device", lambda: 0, raising=False)
+    monkeypatch.setattr(w8a8, "_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    taken = []
+    with FakeTensorMode():
+        z = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="cuda:0")
+        for name, call in calls(z, n).items():
+            try:
+                call()
+                taken.append(name)
+            except ValueError as e:
+                assert "supported" in str(e), name
+    assert not taken
