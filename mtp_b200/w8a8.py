@@ -25,6 +25,7 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -84,6 +85,17 @@ def _check_map(expert_map: torch.Tensor | None, device: torch.device):
         if not expert_map.numel():
             raise ValueError("expert_map is empty")
         _extent("entries of expert_map", expert_map.numel())
+
+
+def _differentiated(*tensors) -> bool:
+    """Whether a derivative of one of ``tensors`` is being recorded, backward or (dual tensors) forward."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside dual_level there are none (unpack_dual takes 0.3 us)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _F32 = (torch.float32,)
@@ -201,7 +213,7 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
     int32, if given - have no expert here: their rows come last, as zeros.
     ``row_scales`` [M] fp32 (the scales of int8 rows) are sorted along. The
     gradient of ``hidden_states`` sums the gradients of a token's routed rows
-    in fp32."""
+    in fp32. Forward-mode derivatives raise ``RuntimeError``."""
     _tensor("hidden_states", hidden_states, 2, _ROWS, contiguous=False)
     dev = hidden_states.device
     _tensor("topk_ids", topk_ids, 2, _I32, dev)
@@ -219,7 +231,7 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
         _tensor("row_scales", row_scales, 1, _F32, dev)
         if row_scales.numel() != m:
             raise ValueError(f"row_scales must have {m} entries")
-    if hidden_states.requires_grad and torch.is_grad_enabled():
+    if _differentiated(hidden_states):
         rest = []
         return SortedTokens(_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales, rest), *rest)
     return SortedTokens(*_sort(hidden_states, topk_ids, num_experts, expert_map, row_scales))
@@ -231,7 +243,8 @@ def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
     fp16 or fp32), in fp32 and rounded once. ``positions`` [M, k] int32 as
     :func:`sort_tokens` gives them; ``topk_weights`` [M, k] fp32 (None: 1). A
     token without routed pairs gets zeros. Gradients go to ``rows`` (zero for
-    rows of unrouted pairs) and ``topk_weights``."""
+    rows of unrouted pairs) and ``topk_weights``; forward-mode derivatives raise
+    ``RuntimeError``."""
     _tensor("rows", rows, 2, _FLOATS)
     _tensor("positions", positions, 2, _I32, rows.device)
     m, k = positions.shape
@@ -245,7 +258,7 @@ def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
         _tensor("topk_weights", topk_weights, 2, _F32, rows.device)
         if topk_weights.shape != positions.shape:
             raise ValueError(f"topk_weights must be {(m, k)}, got {tuple(topk_weights.shape)}")
-    if torch.is_grad_enabled() and (rows.requires_grad or (topk_weights is not None and topk_weights.requires_grad)):
+    if _differentiated(rows, topk_weights):
         return _UnsortTokens.apply(rows, positions, topk_weights)
     return _unsort(rows, positions, topk_weights)
 
