@@ -16,7 +16,8 @@ and :func:`mtp_b200.moe_layer_w4a16`. Shape, dtype and device errors raise
 ``ValueError`` before any launch; a non-zero C status raises
 :class:`mtp_b200.MtpError`. Every call is asynchronous on the current torch
 stream of its tensors' GPU, which need not be the current one. There is no CPU
-path.
+path. Only the token sort has gradients: the other functions work on inputs that
+require one, but a backward pass that reaches them raises ``NotImplementedError``.
 """
 from __future__ import annotations
 
@@ -93,9 +94,22 @@ def _differentiated(*tensors) -> bool:
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    if getattr(forward_ad, "_current_level", 0) < 0:  # outside dual_level there are none (unpack_dual takes 0.3 us)
+    if forward_ad._current_level < 0:  # outside dual_level there are no duals (unpack_dual takes 0.3 us)
         return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+class _NoGradient(torch.autograd.Function):
+    """call(), whose derivatives with respect to ``inputs`` are errors instead of missing."""
+
+    @staticmethod
+    def forward(ctx, name, call, *inputs):
+        ctx.name = name
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.name} has no gradient")
 
 
 _F32 = (torch.float32,)
@@ -233,8 +247,12 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
             raise ValueError(f"row_scales must have {m} entries")
     if _differentiated(hidden_states):
         rest = []
-        return SortedTokens(_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales, rest), *rest)
-    return SortedTokens(*_sort(hidden_states, topk_ids, num_experts, expert_map, row_scales))
+        r = SortedTokens(_SortTokens.apply(hidden_states, topk_ids, num_experts, expert_map, row_scales, rest), *rest)
+    else:
+        r = SortedTokens(*_sort(hidden_states, topk_ids, num_experts, expert_map, row_scales))
+    if row_scales is not None and _differentiated(row_scales):
+        r = r._replace(row_scales=_NoGradient.apply("row_scales of sort_tokens", lambda: r.row_scales, row_scales))
+    return r
 
 
 def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
@@ -278,6 +296,13 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError("x must have at least one column")
     _extent("rows", m)
     _extent("columns", k)
+    if _differentiated(x):
+        return _NoGradient.apply("quantize_int8", lambda: _quantize(x), x)
+    return _quantize(x)
+
+
+def _quantize(x):
+    m, k = x.shape
     kp = (k + 15) // 16 * 16
     codes = x.new_empty(m, kp, dtype=torch.int8)
     scale = x.new_empty(m, dtype=torch.float32)
@@ -372,7 +397,10 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     _, n = _check_weight("b", b, b_scale, 2, device, k)
     _check_bias(bias, n, device)
     _check_out(out_dtype, status, device)
-    return _product(a, a_scale, b, b_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
+    args = (a, a_scale, b, b_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
+    if _differentiated(a_scale, b_scale, bias):
+        return _NoGradient.apply("int8_matmul", lambda: _product(*args), a_scale, b_scale, bias)
+    return _product(*args)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -388,7 +416,10 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     _check_bias(bias, n, device)
     out_dtype = out_dtype or x.dtype
     _check_out(out_dtype, status, device)
-    return _product(x, None, weight, weight_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
+    args = (x, None, weight, weight_scale, bias, None, (rows, k, 1, n), out_dtype, 0, status)
+    if _differentiated(x, weight_scale, bias):
+        return _NoGradient.apply("int8_linear", lambda: _product(*args), x, weight_scale, bias)
+    return _product(*args)
 
 
 def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -412,8 +443,10 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     if activation and n % 2:
         raise ValueError(f"silu_mul needs an even number of channels, got {n}")
     _check_out(out_dtype, status, device)
-    return _product(a, a_scale, b, b_scale, None, offsets, (rows, k, groups, n), out_dtype,
-                    _SILU_MUL if activation else 0, status)
+    args = (a, a_scale, b, b_scale, None, offsets, (rows, k, groups, n), out_dtype, _SILU_MUL if activation else 0, status)
+    if _differentiated(a_scale, b_scale):
+        return _NoGradient.apply("int8_grouped_matmul", lambda: _product(*args), a_scale, b_scale)
+    return _product(*args)
 
 
 # ---------------------------------------------------------------------------
@@ -442,7 +475,9 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
     rows, then up rows) with ``w13_scale`` [E, 2I]; ``w2`` [E, H, I] int8 with
     ``w2_scale`` [E, H]. Ids outside [0, E) - after ``expert_map``, which takes
     global ids to local ones - contribute nothing. Returns ``out`` [M, H] in
-    the type of ``hidden_states``. ``status`` as in :func:`int8_matmul`."""
+    the type of ``hidden_states`` (a given ``out`` cannot be part of a graph: with
+    inputs that require a gradient it raises ``RuntimeError``). ``status`` as in
+    :func:`int8_matmul`."""
     _tensor("hidden_states", hidden_states, 2, _FLOATS)
     dev = hidden_states.device
     m, h = hidden_states.shape
@@ -473,13 +508,28 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
         if topk_weights.shape != (m, top_k) or topk_ids.shape != (m, top_k):
             raise ValueError(f"topk_weights/topk_ids must be {(m, top_k)}")
     _check_map(expert_map, dev)
-    if out is None:
-        out = torch.empty_like(hidden_states)
-    else:
+    if out is not None:
         _tensor("out", out, 2, (hidden_states.dtype,), dev)
         if out.shape != (m, h):
             raise ValueError(f"out must be {(m, h)}, got {tuple(out.shape)}")
     _check_out(hidden_states.dtype, status, dev)
+    if router_logits is not None:
+        topk_weights = topk_ids = None
+    args = (hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, topk_weights, topk_ids,
+            expert_map, out, status)
+    floats = (hidden_states, router_logits, topk_weights, w13_scale, w2_scale)
+    if _differentiated(*floats):
+        if out is not None:
+            raise RuntimeError("moe_layer_w8a8 has no gradient: give no out with inputs that require one")
+        return _NoGradient.apply("moe_layer_w8a8", lambda: _layer(*args), *floats)
+    return _layer(*args)
+
+
+def _layer(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, topk_weights, topk_ids,
+           expert_map, out, status):
+    (m, h), (e, _, i) = hidden_states.shape, w2.shape
+    if out is None:
+        out = torch.empty_like(hidden_states)
     given = router_logits is None
     dtype, px, p13, p2 = DTYPES[hidden_states.dtype], hidden_states.data_ptr(), w13.data_ptr(), w2.data_ptr()
     size = _layer_workspace(m, h, i, e, top_k, dtype, not given, px & 255, p13 & 255, p2 & 255)
