@@ -44,29 +44,22 @@ _quantize_entry = _lib.Entry("mtp_quantize_int8")
 _matmul_entry = _lib.Entry("mtp_int8_matmul")
 _layer_entry = _lib.Entry("mtp_w8a8_moe_layer")
 
-# The current device, and the handle of a device's current stream (torch.cuda.current_stream builds a Stream object around it).
+# The current device, on which the C side launches: the functions below that launch make their tensors' device
+# current first. And the handle of a device's current stream (torch.cuda.current_stream builds a Stream object around it).
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
            or (lambda device: torch.cuda.current_stream(device).cuda_stream))
-
-
-def _launch(entry: _lib.Entry, device: int, *args) -> None:
-    """``entry(*args, stream)`` with ``device`` current, as the C side launches on the current device."""
-    if device == _current_device():
-        entry(*args, _stream(device))
-    else:
-        with torch.cuda.device(device):
-            entry(*args, _stream(device))
 
 
 def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None, contiguous: bool = True):
     """``t`` is a CUDA tensor of one of ``dtypes`` and ``ndim`` dimensions on ``device``."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor, got device {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device is None or t.device != device:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor, got device {t.device}")
+        if device is not None:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
     if t.ndim != ndim:
@@ -75,17 +68,16 @@ def _tensor(name: str, t, ndim: int, dtypes, device: torch.device | None = None,
         raise ValueError(f"{name} must be contiguous")
 
 
-def _extent(what: str, n: int):
-    if n > MAX_EXTENT:
-        raise ValueError(f"at most {MAX_EXTENT} {what} are supported, got {n}")
+def _too_large(what: str, n: int):
+    raise ValueError(f"at most {MAX_EXTENT} {what} are supported, got {n}")
 
 
-def _check_map(expert_map: torch.Tensor | None, device: torch.device):
-    if expert_map is not None:
-        _tensor("expert_map", expert_map, 1, _I32, device)
-        if not expert_map.numel():
-            raise ValueError("expert_map is empty")
-        _extent("entries of expert_map", expert_map.numel())
+def _check_map(expert_map: torch.Tensor, device: torch.device):
+    _tensor("expert_map", expert_map, 1, _I32, device)
+    if not expert_map.numel():
+        raise ValueError("expert_map is empty")
+    if expert_map.numel() > MAX_EXTENT:
+        _too_large("entries of expert_map", expert_map.numel())
 
 
 def _differentiated(*tensors) -> bool:
@@ -150,37 +142,49 @@ class SortedTokens(NamedTuple):
 
 
 def _sort(x, ids, num_experts, expert_map, row_scales):
+    device = x.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _sort(x, ids, num_experts, expert_map, row_scales)
     m, k = ids.shape
     h = x.shape[1]
     rows = x.new_empty(m * k, h)
     positions = torch.empty_like(ids)
     offsets = ids.new_empty(num_experts + 1)
     scales = None if row_scales is None else row_scales.new_empty(m * k)
-    _launch(_sort_entry, x.get_device(), x.data_ptr() or None, _row_stride("hidden_states", x),
-            DTYPES.get(x.dtype, _INT8), m, h, ids.data_ptr(), k, num_experts,
-            None if expert_map is None else expert_map.data_ptr(),
-            0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
-            rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(), offsets.data_ptr())
+    _sort_entry(x.data_ptr() or None, _row_stride("hidden_states", x), DTYPES.get(x.dtype, _INT8), m, h,
+              ids.data_ptr(), k, num_experts, None if expert_map is None else expert_map.data_ptr(),
+              0 if expert_map is None else expert_map.numel(), None if scales is None else row_scales.data_ptr(),
+              rows.data_ptr(), None if scales is None else scales.data_ptr(), positions.data_ptr(),
+              offsets.data_ptr(), _stream(device))
     return rows, positions, offsets, scales
 
 
 def _unsort(rows, positions, weights):
+    device = rows.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _unsort(rows, positions, weights)
     m, k = positions.shape
     r, h = rows.shape
     out = rows.new_empty(m, h)
-    _launch(_unsort_entry, rows.get_device(), rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
-            None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr())
+    _unsort_entry(rows.data_ptr(), r, DTYPES[rows.dtype], positions.data_ptr(),
+                  None if weights is None else weights.data_ptr(), m, k, h, out.data_ptr(), _stream(device))
     return out
 
 
 def _unsort_backward(grad, rows, num_rows, positions, weights, need_rows, need_weights):
+    device = grad.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _unsort_backward(grad, rows, num_rows, positions, weights, need_rows, need_weights)
     (m, k), h = positions.shape, grad.shape[1]
     grad_rows = grad.new_empty(num_rows, h) if need_rows else None
     grad_weights = torch.empty_like(weights) if need_weights else None
-    _launch(_unsort_backward_entry, grad.get_device(), grad.data_ptr(), None if rows is None else rows.data_ptr(),
-            num_rows, DTYPES[grad.dtype], positions.data_ptr(), None if weights is None else weights.data_ptr(), m, k, h,
-            None if grad_rows is None else grad_rows.data_ptr(),
-            None if grad_weights is None else grad_weights.data_ptr())
+    _unsort_backward_entry(grad.data_ptr(), None if rows is None else rows.data_ptr(), num_rows, DTYPES[grad.dtype],
+                           positions.data_ptr(), None if weights is None else weights.data_ptr(), m, k, h,
+                           None if grad_rows is None else grad_rows.data_ptr(),
+                           None if grad_weights is None else grad_weights.data_ptr(), _stream(device))
     return grad_rows, grad_weights
 
 
@@ -231,16 +235,19 @@ def sort_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor, num_experts
     _tensor("hidden_states", hidden_states, 2, _ROWS, contiguous=False)
     dev = hidden_states.device
     _tensor("topk_ids", topk_ids, 2, _I32, dev)
-    m, k = topk_ids.shape
-    if m != hidden_states.shape[0]:
-        raise ValueError(f"topk_ids has {m} rows, hidden_states has {hidden_states.shape[0]}")
+    (m, k), (tokens, h) = topk_ids.shape, hidden_states.shape
+    if m != tokens:
+        raise ValueError(f"topk_ids has {m} rows, hidden_states has {tokens}")
     if not 1 <= k <= 32:
         raise ValueError(f"topk_ids must have 1 to 32 columns, got {k}")
     if not 1 <= num_experts <= 1024:
         raise ValueError(f"num_experts must be in [1, 1024], got {num_experts}")
-    _extent("pairs", m * k)
-    _extent("columns", hidden_states.shape[1])
-    _check_map(expert_map, dev)
+    if m * k > MAX_EXTENT:
+        _too_large("pairs", m * k)
+    if h > MAX_EXTENT:
+        _too_large("columns", h)
+    if expert_map is not None:
+        _check_map(expert_map, dev)
     if row_scales is not None:
         _tensor("row_scales", row_scales, 1, _F32, dev)
         if row_scales.numel() != m:
@@ -265,13 +272,15 @@ def unsort_tokens(rows: torch.Tensor, positions: torch.Tensor,
     ``RuntimeError``."""
     _tensor("rows", rows, 2, _FLOATS)
     _tensor("positions", positions, 2, _I32, rows.device)
-    m, k = positions.shape
+    (m, k), (pairs, h) = positions.shape, rows.shape
     if not 1 <= k <= 32:
         raise ValueError(f"positions must have 1 to 32 columns, got {k}")
-    if rows.shape[0] != m * k:
-        raise ValueError(f"rows must have one row per pair, {m * k}, got {rows.shape[0]}")
-    _extent("pairs", m * k)
-    _extent("columns", rows.shape[1])
+    if pairs != m * k:
+        raise ValueError(f"rows must have one row per pair, {m * k}, got {pairs}")
+    if pairs > MAX_EXTENT:
+        _too_large("pairs", pairs)
+    if h > MAX_EXTENT:
+        _too_large("columns", h)
     if topk_weights is not None:
         _tensor("topk_weights", topk_weights, 2, _F32, rows.device)
         if topk_weights.shape != positions.shape:
@@ -294,20 +303,26 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     if k < 1:
         raise ValueError("x must have at least one column")
-    _extent("rows", m)
-    _extent("columns", k)
+    if m > MAX_EXTENT:
+        _too_large("rows", m)
+    if k > MAX_EXTENT:
+        _too_large("columns", k)
     if _differentiated(x):
         return _NoGradient.apply("quantize_int8", lambda: _quantize(x), x)
     return _quantize(x)
 
 
 def _quantize(x):
+    device = x.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _quantize(x)
     m, k = x.shape
     kp = (k + 15) // 16 * 16
     codes = x.new_empty(m, kp, dtype=torch.int8)
     scale = x.new_empty(m, dtype=torch.float32)
-    _launch(_quantize_entry, x.get_device(), x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k,
-            codes.data_ptr(), kp, scale.data_ptr())
+    _quantize_entry(x.data_ptr(), _row_stride("x", x), DTYPES[x.dtype], m, k, codes.data_ptr(), kp, scale.data_ptr(),
+                    _stream(device))
     return codes if kp == k else codes[:, :k], scale
 
 
@@ -322,6 +337,10 @@ def _matmul_workspace(rows, n, k, groups, a_dtype, a_stride, a_off, b_off) -> in
 
 
 def _product(a, a_scale, b, b_scale, bias, offsets, shape, out_dtype, activation, status):
+    device = a.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _product(a, a_scale, b, b_scale, bias, offsets, shape, out_dtype, activation, status)
     rows, k, groups, n = shape
     cols = n // 2 if activation else n
     out = a.new_empty(rows, cols) if out_dtype is a.dtype else a.new_empty(rows, cols, dtype=out_dtype)
@@ -335,7 +354,7 @@ def _product(a, a_scale, b, b_scale, bias, offsets, shape, out_dtype, activation
                                   None if offsets is None else offsets.data_ptr(), out.data_ptr(),
                                   None if status is None else status.data_ptr(),
                                   None if ws is None else ws.data_ptr(), size)
-    _launch(_matmul_entry, a.get_device(), C.byref(args))
+    _matmul_entry(C.byref(args), _stream(device))
     return out
 
 
@@ -353,7 +372,8 @@ def _check_weight(name, b, scale, ndim, device, k):
         raise ValueError(f"1 to {MAX_K} columns are supported, got {k}")
     if not groups or not n:
         raise ValueError(f"{name} must not be empty, got shape {tuple(b.shape)}")
-    _extent(f"rows of {name}", groups * n)
+    if groups * n > MAX_EXTENT:
+        _too_large(f"rows of {name}", groups * n)
     return groups, n
 
 
@@ -381,7 +401,8 @@ def _check_rows(a, a_scale):
     rows, k = a.shape
     if a_scale.numel() != rows:
         raise ValueError(f"a_scale must have {rows} entries, got {a_scale.numel()}")
-    _extent("rows", rows)
+    if rows > MAX_EXTENT:
+        _too_large("rows", rows)
     return rows, k, device
 
 
@@ -411,7 +432,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     type of ``x`` unless ``out_dtype`` is given."""
     _tensor("x", x, 2, _FLOATS, contiguous=False)
     (rows, k), device = x.shape, x.device
-    _extent("rows", rows)
+    if rows > MAX_EXTENT:
+        _too_large("rows", rows)
     _, n = _check_weight("weight", weight, weight_scale, 2, device, k)
     _check_bias(bias, n, device)
     out_dtype = out_dtype or x.dtype
@@ -491,7 +513,8 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
         raise ValueError(f"at most 1024 experts are supported, got {e}")
     if not 1 <= top_k <= 32:
         raise ValueError(f"top_k must be in [1, 32], got {top_k}")
-    _extent("pairs", m * top_k)
+    if m * top_k > MAX_EXTENT:
+        _too_large("pairs", m * top_k)
     if router_logits is not None:
         _tensor("router_logits", router_logits, 2, _F32, dev)
         if router_logits.shape != (m, e):
@@ -507,7 +530,8 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
         _tensor("topk_ids", topk_ids, 2, _I32, dev)
         if topk_weights.shape != (m, top_k) or topk_ids.shape != (m, top_k):
             raise ValueError(f"topk_weights/topk_ids must be {(m, top_k)}")
-    _check_map(expert_map, dev)
+    if expert_map is not None:
+        _check_map(expert_map, dev)
     if out is not None:
         _tensor("out", out, 2, (hidden_states.dtype,), dev)
         if out.shape != (m, h):
@@ -515,8 +539,8 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
     _check_out(hidden_states.dtype, status, dev)
     if router_logits is not None:
         topk_weights = topk_ids = None
-    args = (hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, topk_weights, topk_ids,
-            expert_map, out, status)
+    args = (hidden_states, router_logits, w13, w13_scale, w2, w2_scale, (m, h, i, e, top_k), renormalize, topk_weights,
+            topk_ids, expert_map, out, status)
     floats = (hidden_states, router_logits, topk_weights, w13_scale, w2_scale)
     if _differentiated(*floats):
         if out is not None:
@@ -525,9 +549,14 @@ def moe_layer_w8a8(hidden_states: torch.Tensor, router_logits: torch.Tensor | No
     return _layer(*args)
 
 
-def _layer(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, renormalize, topk_weights, topk_ids,
+def _layer(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, shape, renormalize, topk_weights, topk_ids,
            expert_map, out, status):
-    (m, h), (e, _, i) = hidden_states.shape, w2.shape
+    device = hidden_states.get_device()
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _layer(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, shape, renormalize, topk_weights,
+                          topk_ids, expert_map, out, status)
+    m, h, i, e, top_k = shape
     if out is None:
         out = torch.empty_like(hidden_states)
     given = router_logits is None
@@ -541,5 +570,5 @@ def _layer(hidden_states, router_logits, w13, w13_scale, w2, w2_scale, top_k, re
                                  None if expert_map is None else expert_map.data_ptr(), p13, w13_scale.data_ptr(), p2,
                                  w2_scale.data_ptr(), out.data_ptr(), None if status is None else status.data_ptr(),
                                  ws.data_ptr(), size)
-    _launch(_layer_entry, hidden_states.get_device(), C.byref(args))
+    _layer_entry(C.byref(args), _stream(device))
     return out

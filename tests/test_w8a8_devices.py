@@ -81,9 +81,18 @@ def test_results_under_another_current_device(cuda_device, monkeypatch):
         return mtp_b200.unsort_tokens(y, r.positions)
 
     want = results()
-    entered, device = [], torch.cuda.device
-    monkeypatch.setattr(w8a8, "_current_device", lambda: 5)
-    monkeypatch.setattr(torch.cuda, "device", lambda index: entered.append(index) or device(index))
+    entered, current, device = [], [5], torch.cuda.device
+
+    @contextlib.contextmanager
+    def enter(index):
+        entered.append(index)
+        current.append(index)
+        with device(index):
+            yield
+        current.pop()
+
+    monkeypatch.setattr(w8a8, "_current_device", lambda: current[-1])
+    monkeypatch.setattr(torch.cuda, "device", enter)
     got = results()
     assert entered == [0] * 4
     assert torch.equal(got, want)
