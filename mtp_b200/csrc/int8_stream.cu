@@ -75,7 +75,7 @@ __device__ void quantise_rows(const StreamArgs& p, int M, int K, uint8_t* codes,
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      store_unit<true>(reinterpret_cast<int8_t*>(codes + m * p.pitch), c, p.kp, v, r);
+      store_unit(reinterpret_cast<int8_t*>(codes + m * p.pitch + c), v, r);
     }
   }
   __syncthreads();

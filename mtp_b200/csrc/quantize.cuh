@@ -85,15 +85,10 @@ __device__ __forceinline__ void codes_of(float* v, RowScale r, uint32_t* w) {
   for (int i = 0; i < N; i += 4) w[i / 4] = r.factor != 0.f ? four_codes(v + i, r.factor) : 0u;
 }
 
-template <bool WIDE>
-__device__ __forceinline__ void store_unit(int8_t* q, int c, int K, float* v, RowScale r) {
+__device__ __forceinline__ void store_unit(int8_t* q, float* v, RowScale r) {
   uint32_t w[2];
   codes_of<8>(v, r, w);
-  if (WIDE) {
-    *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
-  } else {
-    for (int i = 0; i < 8 && c + i < K; ++i) q[c + i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
-  }
+  *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
 }
 
 }  // namespace mtp

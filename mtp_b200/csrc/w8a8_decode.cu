@@ -96,7 +96,7 @@ __device__ __forceinline__ void quantise_into(F row, int rows, int K, uint8_t* c
         for (int i = 0; i < 8; ++i) v[i] = keep[i];
       else
         load_unit<X, true>(src, c, K, v);
-      store_unit<true>(reinterpret_cast<int8_t*>(codes + m * pitch), c, K, v, r);
+      store_unit(reinterpret_cast<int8_t*>(codes + m * pitch + c), v, r);
     }
   }
 }
