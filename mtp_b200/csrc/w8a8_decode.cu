@@ -12,8 +12,8 @@
 //         weights are on their way, and takes its share of the down units (16
 //         channels), y in fp32. The last unit of a strip of channels to finish
 //         sums it: out[t] = sum over the token's pairs, in order, of weight * y.
-// (One launch with grid barriers between these phases took 19 us to this one's
-// 15: a barrier over 148 SMs costs more than the end of a kernel.)
+// (One launch with grid barriers between these phases took 19.3 us a call, the
+// two take 17: a barrier over 148 SMs costs more than the end of a kernel.)
 // A unit's product is streamed as in int8_stream.cu: 16 bytes of K a lane from
 // global memory into mma.m16n8k32, ks warps a unit, int32 sums through shared
 // memory. A CTA's units are one range of (block, strip), so it touches few
@@ -431,10 +431,12 @@ int by_experts(const DecodeArgs& a, cudaStream_t st) {
 
 int64_t w8a8_decode_list_bytes() { return sizeof(DecodeLists); }
 
-// Up to the weights of about 32 experts of 3 MB: beyond, streaming them at HBM's
-// rate matters more than launches, and the tile kernels do that better (2048 x
-// 512, top-8 of 256: 1 token 17.7 us against 26.3, 4 tokens 31.0 against 39.0,
-// 8 tokens 54.2 against 53.6).
+// Up to 100 MB of weights: beyond, streaming them at HBM's rate matters more than
+// launches, and the tile kernels do that better. These kernels against those, us a
+// call in a graph over four layers' weights: 2048 x 512, top-8 of 256, 1 token 17.1
+// against 25.9, 4 tokens (96 MB at most) 30.2 and 35.2, 5 tokens 36.5 and 38.1, 6
+// tokens 47.1 and 42.8; 2048 x 768, top-8 of 128, 2 tokens (72 MB) 25.7 and 32.3,
+// 4 tokens (144 MB) 42.0 and 42.0, 5 tokens 47.0 and 45.0.
 bool w8a8_decode_takes(int M, int H, int I, int E, int k) {
   return M <= kDTokens && std::min<int64_t>(static_cast<int64_t>(M) * k, E) * 3 * H * I <= (100ll << 20) && M * k <= kDPairs && H % 16 == 0 && I % 16 == 0 &&
          static_cast<int64_t>(M) * decode_pitch(H) <= kDCodes && static_cast<int64_t>(kDRows) * decode_pitch(I) <= kDCodes;
