@@ -306,6 +306,63 @@ MTP_API int mtp_unsort_tokens_backward(const void* grad, const void* rows, int64
                                        const int32_t* positions, const float* weights, int32_t M, int32_t k,
                                        int32_t H, void* grad_rows, float* grad_weights, void* stream);
 
+/* ---- a training step around the token sort --------------------------------------- */
+/* The router with its losses, for logits [M, num_experts] (bf16, fp16 or fp32,
+ * rows logits_stride elements apart): p = softmax of a row in fp32; ids [M, k] =
+ * the k largest, descending (ties: the lower id; NaN logits last, always
+ * distinct experts); weights [M, k] = p there, divided by their sum with
+ * renormalize. Tokens count where token_mask [M] is not 0 (NULL: all); the
+ * others have ids -1 and weights 0. Over the n tokens that count:
+ * counts [num_experts] = pairs of each expert, balance_loss [1] =
+ * num_experts / (k n^2) * sum_e counts[e] * sum_t p[t, e] (1 where even),
+ * z_loss [1] = sum_t (log sum exp)^2 / n; both 0 for n = 0. pull
+ * [num_experts + 1] (or NULL) is for the gradient. num_experts <= 1024, k <= 32.
+ * Nothing depends on timing. workspace: 256-byte aligned, no zero fill needed. */
+MTP_API int mtp_route_tokens_workspace_size(int32_t M, int32_t num_experts, int64_t* bytes);
+MTP_API int mtp_route_tokens(const void* logits, int64_t logits_stride, int32_t dtype, int32_t M,
+                             int32_t num_experts, int32_t k, int32_t renormalize, const uint8_t* token_mask,
+                             float* weights, int32_t* ids, int32_t* counts, float* balance_loss, float* z_loss,
+                             float* pull, void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradient: grad_logits [M, num_experts] (contiguous) for the gradients of
+ * weights [M, k], balance_loss [1] and z_loss [1], each NULL where there is none;
+ * zeros for tokens that do not count. ids and pull as the forward call wrote
+ * them (ids outside the experts are no pair).                               */
+MTP_API int mtp_route_tokens_backward(const void* logits, int64_t logits_stride, int32_t dtype, int32_t M,
+                                      int32_t num_experts, int32_t k, int32_t renormalize,
+                                      const uint8_t* token_mask, const int32_t* ids, const float* pull,
+                                      const float* grad_weights, const float* grad_balance_loss,
+                                      const float* grad_z_loss, void* grad_logits, void* stream);
+
+/* y [M, H] = (x - mean) / sqrt(var + eps) * weight + bias per row of x (bf16,
+ * fp16 or fp32, rows x_stride elements apart), the variance over H, in fp32,
+ * rounded once. weight, bias [H] (NULL: 1 and 0): param_dtype, the type of x or
+ * fp32. stats [M, 2] (or NULL): mean and 1 / sqrt(var + eps) of each row, for
+ * the gradient.                                                             */
+MTP_API int mtp_layer_norm(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t H, const void* weight,
+                           const void* bias, int32_t param_dtype, float eps, void* y, float* stats, void* stream);
+/* Its gradients for grad [M, H] (contiguous): grad_x [M, H] in the type of x,
+ * grad_weight and grad_bias [H] in param_dtype, summed over the rows in fp32 in
+ * a fixed order; each may be NULL. workspace (256-byte aligned) only for the
+ * gradients of weight and bias.                                             */
+MTP_API int mtp_layer_norm_backward_workspace_size(int32_t M, int32_t H, int64_t* bytes);
+MTP_API int mtp_layer_norm_backward(const void* grad, const void* x, int64_t x_stride, int32_t dtype, int32_t M,
+                                    int32_t H, const void* weight, int32_t param_dtype, const float* stats,
+                                    void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+
+/* out [N, H] = scale * table[ids[t]] in fp32, rounded once, for a table [V, H] of
+ * bf16, fp16 or fp32 and ids of id_bytes 4 (int32) or 8 (int64); an id outside
+ * [0, V) gives a row of zeros.                                              */
+MTP_API int mtp_embed_tokens(const void* ids, int32_t id_bytes, int32_t N, const void* table, int32_t dtype,
+                             int32_t V, int32_t H, float scale, void* out, void* stream);
+/* Its gradient: grad_table [V, H] = scale * the sum of grad [N, H] over the
+ * tokens of each row, in fp32 in a fixed order, rounded once; every row is
+ * written. workspace: 256-byte aligned, no zero fill needed.                */
+MTP_API int mtp_embed_tokens_backward_workspace_size(int32_t N, int32_t H, int32_t dtype, int64_t* bytes);
+MTP_API int mtp_embed_tokens_backward(const void* ids, int32_t id_bytes, int32_t N, const void* grad, int32_t dtype,
+                                      int32_t V, int32_t H, float scale, void* grad_table, void* workspace,
+                                      int64_t workspace_bytes, void* stream);
+
 /* ---- int8 (W8A8) ------------------------------------------------------------- */
 /* One scale per row: scale = max|x| / 127, q = round(x * (127 / max|x|)), half
  * to even, in fp32. A row of zeros has scale 0; a row with an infinity or a NaN

@@ -24,6 +24,12 @@ from .ops import (  # noqa: F401
     topk_softmax,
     vllm_wna16_to_gptq,
 )
+from .training import (  # noqa: F401
+    RoutedTokens,
+    embed_tokens,
+    layer_norm,
+    route_tokens,
+)
 from .w8a8 import (  # noqa: F401
     SortedTokens,
     int8_grouped_matmul,
@@ -41,16 +47,19 @@ __all__ = [
     "MtpError",
     "MtpPredictor",
     "PrefetchSession",
+    "RoutedTokens",
     "load_library",
     "SharedExpert",
     "SortedTokens",
     "W4A16Experts",
     "dequantize_gptq_projection",
+    "embed_tokens",
     "experts_from_vllm_wna16",
     "fused_experts",
     "int8_grouped_matmul",
     "int8_linear",
     "int8_matmul",
+    "layer_norm",
     "layer_path",
     "layer_workspace",
     "moe_align_block_size",
@@ -59,6 +68,7 @@ __all__ = [
     "plan_dispatch",
     "prefill_workspace",
     "quantize_int8",
+    "route_tokens",
     "sort_tokens",
     "topk_softmax",
     "unsort_tokens",

@@ -34,6 +34,15 @@ EXPORTS = (
     "mtp_sort_tokens",
     "mtp_unsort_tokens",
     "mtp_unsort_tokens_backward",
+    "mtp_route_tokens_workspace_size",
+    "mtp_route_tokens",
+    "mtp_route_tokens_backward",
+    "mtp_layer_norm",
+    "mtp_layer_norm_backward_workspace_size",
+    "mtp_layer_norm_backward",
+    "mtp_embed_tokens",
+    "mtp_embed_tokens_backward_workspace_size",
+    "mtp_embed_tokens_backward",
     "mtp_quantize_int8",
     "mtp_int8_matmul_workspace_size",
     "mtp_int8_matmul",
@@ -136,6 +145,15 @@ _SIGS = {
     "mtp_sort_tokens": (C.c_int, [vp, i64, i32, i32, i32, vp, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp]),
     "mtp_unsort_tokens": (C.c_int, [vp, i64, i32, vp, vp, i32, i32, i32, vp, vp]),
     "mtp_unsort_tokens_backward": (C.c_int, [vp, vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp]),
+    "mtp_route_tokens_workspace_size": (C.c_int, [i32, i32, C.POINTER(i64)]),
+    "mtp_route_tokens": (C.c_int, [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+    "mtp_route_tokens_backward": (C.c_int, [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "mtp_layer_norm": (C.c_int, [vp, i64, i32, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp]),
+    "mtp_layer_norm_backward_workspace_size": (C.c_int, [i32, i32, C.POINTER(i64)]),
+    "mtp_layer_norm_backward": (C.c_int, [vp, vp, i64, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, i64, vp]),
+    "mtp_embed_tokens": (C.c_int, [vp, i32, i32, vp, i32, i32, i32, C.c_float, vp, vp]),
+    "mtp_embed_tokens_backward_workspace_size": (C.c_int, [i32, i32, i32, C.POINTER(i64)]),
+    "mtp_embed_tokens_backward": (C.c_int, [vp, i32, i32, vp, i32, i32, i32, C.c_float, vp, vp, i64, vp]),
     "mtp_quantize_int8": (C.c_int, [vp, i64, i32, i32, i32, vp, i64, vp, vp]),
     "mtp_int8_matmul_workspace_size": (C.c_int, [C.POINTER(MtpInt8MatmulArgs), C.POINTER(i64)]),
     "mtp_int8_matmul": (C.c_int, [C.POINTER(MtpInt8MatmulArgs), vp]),

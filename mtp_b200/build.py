@@ -26,9 +26,9 @@ STAMP = LIBDIR / "libmtp_b200.stamp"
 
 SOURCES = ["capi.cu", "router_align.cu", "gptq.cu", "moe_fused.cu", "moe_prefill.cu", "predictor.cu", "prefetch.cu",
            "noalloc.cu", "token_sort.cu", "quantize.cu", "int8_matmul.cu", "int8_stream.cu",
-           "w8a8_api.cu", "w8a8_decode.cu"]
+           "w8a8_api.cu", "w8a8_decode.cu", "route_loss.cu", "layer_norm.cu", "embedding.cu", "training_api.cu"]
 HEADERS = ["common.cuh", "internal.cuh", "int8_common.cuh", "quantize.cuh", "route.cuh",
-           "w8a8_common.cuh"]
+           "rows.cuh", "w8a8_common.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,0 +1,460 @@
+// Rows of a table by token ids, scaled, and the table's gradient.
+//
+// forward:  out[t] = scale * table[id[t]], zeros for an id outside [0, V).
+// gradient: grad_table[v] = scale * sum over the tokens t of v, ascending, of
+//           grad[t], in fp32, rounded once; zeros for rows without a token.
+//
+// The gradient sorts the tokens by id first, so that no sum depends on timing:
+// 1. embed_sort_kernel: a CTA takes a slice of the table's rows, finds the
+//    tokens of that slice among all, sorts them (stable) and writes zeros to
+//    the rows that have none. Where a slice's tokens go needs no word from the
+//    other CTAs: the tokens of smaller ids are counted on the way.
+// 2. embed_sum_kernel: a warp takes a chunk of the sorted tokens and a slice of
+//    the columns and sums row after row. So the work is even however uneven the
+//    rows' tokens are. Rows that lie inside a chunk are written, the others'
+//    sums go to `parts`: [chunk][0] of the row that reaches in from the chunk
+//    before, [chunk][1] of one that begins in the chunk and reaches out.
+// 3. embed_join_kernel: sums the parts of each row that reaches over chunks.
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace mtp {
+namespace {
+
+constexpr int kSms = 148;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSliceRows = 1 << 17;   // rows that a CTA takes at once: bits in shared memory
+constexpr int kCounted = 512;         // tokens of a slice that are sorted by counting
+constexpr int kDigitBits = 6;         // of a round of the radix sort
+constexpr int kJoinWarps = 8;
+
+template <typename ID>
+__device__ __forceinline__ int64_t id_at(const EmbedArgs& a, int i) {
+  return static_cast<const ID*>(a.ids)[i];
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+template <typename ID, typename T, int N>
+__global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
+  using V = Vec<T, N>;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= a.N) return;
+  const int64_t id = id_at<ID>(a, static_cast<int>(t));
+  const bool here = id >= 0 && id < a.V;
+  const T* row = static_cast<const T*>(a.table) + (here ? id : 0) * a.H;
+  T* out = static_cast<T*>(a.out) + t * a.H;
+  for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
+    float f[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = 0.f;
+    if (here) {
+      to_floats(*reinterpret_cast<const V*>(row + c), f);
+#pragma unroll
+      for (int n = 0; n < N; ++n) f[n] *= a.scale;
+    }
+    V o;
+    from_floats(f, o);
+    *reinterpret_cast<V*>(out + c) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// gradient: the sort
+// ---------------------------------------------------------------------------
+struct SortShared {
+  uint32_t present[kSliceRows / 32];
+  int count[kSortWarps][1 << kDigitBits];
+  int start[1 << kDigitBits];
+  __align__(16) uint32_t key[kCounted];  // row << 9 | number in the slice
+  int token[kCounted];
+  int warp_in[kSortWarps], warp_below[kSortWarps];
+};
+
+// One stable round of the radix sort: entries [0, n) of (key, token) by `bits`
+// bits of key - lo from `shift` on.
+__device__ void radix_round(SortShared& s, const int32_t* key, const int32_t* token, int32_t* key_out,
+                            int32_t* token_out, int n, int lo, int shift, int bits) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
+  for (int x = tid; x < kSortWarps * bins; x += kSortThreads) s.count[x / bins][x % bins] = 0;
+  __syncthreads();
+  const int span = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int begin = min(warp * span, n), end = min(begin + span, n);
+  auto ranked = [&](int i, int& digit, int& rank) {  // and how many of the round have this digit
+    digit = i < end ? (key[i] - lo) >> shift & (bins - 1) : bins;
+    unsigned same = kFullMask;
+    for (int b = 0; b <= bits; ++b) {
+      const bool one = digit >> b & 1;
+      const unsigned votes = __ballot_sync(kFullMask, one);
+      same &= one ? votes : ~votes;
+    }
+    rank = __popc(same & ((1u << lane) - 1u));
+    return __popc(same);
+  };
+  for (int i = begin; i < end; i += 32) {
+    int digit, rank;
+    const int equal = ranked(i + lane, digit, rank);
+    if (digit < bins && rank == 0) s.count[warp][digit] += equal;
+    __syncwarp();
+  }
+  __syncthreads();
+  if (tid < bins) {
+    int run = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int v = s.count[w][tid];
+      s.count[w][tid] = run;
+      run += v;
+    }
+    s.start[tid] = run;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int run = 0;
+    for (int b = 0; b < bins; ++b) {
+      const int v = s.start[b];
+      s.start[b] = run;
+      run += v;
+    }
+  }
+  __syncthreads();
+  for (int i = begin; i < end; i += 32) {
+    int digit, rank;
+    const int equal = ranked(i + lane, digit, rank);
+    int p = 0;
+    if (digit < bins) p = s.start[digit] + s.count[warp][digit] + rank;
+    __syncwarp();
+    if (digit < bins) {
+      key_out[p] = key[i + lane];
+      token_out[p] = token[i + lane];
+      if (rank == 0) s.count[warp][digit] += equal;
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+}
+
+template <typename ID, typename V>
+__global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const EmbedArgs a, int rows, int64_t row_vectors) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  SortShared& s = *reinterpret_cast<SortShared*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  if (blockIdx.x == 0 && tid == 0) a.valid[1] = 0;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * rows, last = min(first + rows, static_cast<int64_t>(a.V));
+  const int span = ((a.N + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int64_t begin64 = static_cast<int64_t>(warp) * span;
+  const int begin = static_cast<int>(min(begin64, static_cast<int64_t>(a.N)));
+  const int end = static_cast<int>(min(begin64 + span, static_cast<int64_t>(a.N)));
+  for (int64_t lo64 = first; lo64 < last; lo64 += kSliceRows) {
+    const int lo = static_cast<int>(lo64), have = static_cast<int>(min(static_cast<int64_t>(kSliceRows), last - lo64));
+    for (int x = tid; x < (have + 31) / 32; x += kSortThreads) s.present[x] = 0;
+    __syncthreads();
+    int in = 0, below = 0;
+#pragma unroll 4
+    for (int i = begin; i < end; i += 32) {
+      const int64_t id = i + lane < end ? id_at<ID>(a, i + lane) : -1;
+      below += id >= 0 && id < lo;
+      const bool mine = id >= lo && id < lo64 + have;
+      if (mine) {
+        const int row = static_cast<int>(id - lo);
+        atomicOr(&s.present[row >> 5], 1u << (row & 31));
+        ++in;
+      }
+    }
+    in = __reduce_add_sync(kFullMask, in);
+    below = __reduce_add_sync(kFullMask, below);
+    if (lane == 0) {
+      s.warp_in[warp] = in;
+      s.warp_below[warp] = below;
+    }
+    __syncthreads();
+    int base = 0, n = 0, at = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      at += w < warp ? s.warp_in[w] : 0;
+      n += s.warp_in[w];
+      base += s.warp_below[w];
+    }
+    if (tid == 0 && lo64 + have == a.V) a.valid[0] = base + n;
+    // the rounds of the radix sort go between the halves of keys and order, the last into the first half
+    const int bits = have > 1 ? 32 - __clz(have - 1) : 0;
+    const int rounds = n <= kCounted ? 0 : (bits + kDigitBits - 1) / kDigitBits;
+    int32_t* key = a.keys + base;
+    int32_t* token = a.order + base;
+    if (n > 0) {
+      const bool counted = n <= kCounted;
+      int32_t* key_to = rounds & 1 ? key + a.N : key;
+      int32_t* token_to = rounds & 1 ? token + a.N : token;
+      for (int i = begin; i < end; i += 32) {
+        const int64_t id = i + lane < end ? id_at<ID>(a, i + lane) : -1;
+        const bool mine = id >= lo && id < lo64 + have;
+        const unsigned votes = __ballot_sync(kFullMask, mine);
+        if (mine) {
+          const int p = at + __popc(votes & ((1u << lane) - 1u));
+          if (counted) {
+            s.key[p] = static_cast<uint32_t>(id - lo) << 9 | p;
+            s.token[p] = i + lane;
+          } else {
+            key_to[p] = static_cast<int>(id);
+            token_to[p] = i + lane;
+          }
+        }
+        at += __popc(votes);
+      }
+      if (counted)
+        for (int x = n + tid; x < (n + 3) / 4 * 4; x += kSortThreads) s.key[x] = 0xffffffffu;
+      __syncthreads();
+      if (counted && tid < n) {
+        const uint32_t k = s.key[tid];
+        int p = 0;
+        for (int x = 0; x < n; x += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(s.key + x);
+          p += (v.x < k) + (v.y < k) + (v.z < k) + (v.w < k);
+        }
+        key[p] = lo + static_cast<int>(k >> 9);
+        token[p] = s.token[tid];
+      }
+      const int each = rounds ? (bits + rounds - 1) / rounds : 0;
+      for (int r = 0; r < rounds; ++r) {
+        const int64_t from = (rounds - r) & 1 ? a.N : 0, to = a.N - from;
+        radix_round(s, key + from, token + from, key + to, token + to, n, lo, r * each, min(each, bits - r * each));
+      }
+    }
+    // zeros to the rows without a token: a warp a row
+    V zero;
+    memset(&zero, 0, sizeof(V));
+    for (int row = warp; row < have; row += kSortWarps) {
+      if (s.present[row >> 5] >> (row & 31) & 1) continue;
+      V* out = static_cast<V*>(a.grad_table) + (lo64 + row) * row_vectors;
+      for (int64_t c = lane; c < row_vectors; c += 32) out[c] = zero;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// gradient: the sums
+// ---------------------------------------------------------------------------
+constexpr int kAhead = 8;  // tokens whose rows a thread has in flight
+
+// blockDim (lanes of an item, items): an item is a chunk of the sorted tokens
+// and as many columns as its lanes hold.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int slices) {
+  using V = Vec<T, N>;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int chunk = static_cast<int>(item / slices), slice = static_cast<int>(item % slices);
+  const int valid = a.valid[0];
+  const int64_t begin64 = static_cast<int64_t>(chunk) * a.chunk;
+  if (begin64 >= valid) return;
+  const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.chunk, static_cast<int64_t>(valid)));
+  const int64_t c = (static_cast<int64_t>(slice) * blockDim.x + threadIdx.x) * N;
+  const int head = begin > 0 ? a.keys[begin - 1] : -1;   // a row that reaches in
+  const int tail = end < valid ? a.keys[end] : -1;       // or out
+  int row = a.keys[begin];
+  const int last = a.keys[end - 1];
+  const bool owner = last == tail && !(row == last && row == head);
+  if (owner && slice == 0 && threadIdx.x == 0) a.owners[atomicAdd(a.valid + 1, 1)] = chunk;
+  if (c >= a.H) return;
+  const T* grad = static_cast<const T*>(a.grad) + c;
+  float acc[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) acc[n] = 0.f;
+  auto write = [&] {  // the row's sum
+    const bool in = row == head, out = row == tail;
+    if (in || out) {
+      float* part = a.parts + (2ll * chunk + (in ? 0 : 1)) * a.H + c;
+#pragma unroll
+      for (int n = 0; n < N; ++n) part[n] = acc[n];
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) acc[n] *= a.scale;
+      V o;
+      from_floats(acc, o);
+      *reinterpret_cast<V*>(static_cast<T*>(a.grad_table) + static_cast<int64_t>(row) * a.H + c) = o;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] = 0.f;
+  };
+  for (int i0 = begin; i0 < end; i0 += kAhead) {
+    V v[kAhead];
+    int key[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u, end - 1);
+      key[u] = a.keys[i];
+      v[u] = *reinterpret_cast<const V*>(grad + static_cast<int64_t>(a.order[i]) * a.H);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u >= end) break;
+      if (key[u] != row) {
+        write();
+        row = key[u];
+      }
+      float f[N];
+      to_floats(v[u], f);
+#pragma unroll
+      for (int n = 0; n < N; ++n) acc[n] += f[n];
+    }
+  }
+  write();
+}
+
+// A CTA takes a row that reaches over chunks and 32 of its columns; its warps
+// share the chunks out evenly and in order.
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const EmbedArgs a) {
+  __shared__ float sums[kJoinWarps][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int valid = a.valid[0], owners = a.valid[1];
+  const int blocks = (a.H + 31) / 32;
+  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(owners) * blocks; item += gridDim.x) {
+    const int chunk = a.owners[item / blocks];
+    const int c = static_cast<int>(item % blocks) * 32 + lane;
+    const int row = a.keys[(chunk + 1ll) * a.chunk];
+    int more = 0;  // chunks that the row reaches into
+    for (;;) {
+      const int64_t i = (chunk + 1ll + more + lane) * a.chunk;
+      const unsigned votes = __ballot_sync(kFullMask, i < valid && a.keys[i] == row);
+      if (votes != kFullMask) {
+        more += __ffs(~votes) - 1;
+        break;
+      }
+      more += 32;
+    }
+    const int each = (more + kJoinWarps) / kJoinWarps;  // of more + 1 parts
+    const int from = warp * each, to = min(from + each, more + 1);
+    float s = 0.f;
+    if (c < a.H)
+#pragma unroll 8
+      for (int p = from; p < to; ++p) s += a.parts[(2ll * (chunk + p) + (p == 0 ? 1 : 0)) * a.H + c];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < a.H) {
+      s = 0.f;
+      for (int w = 0; w < kJoinWarps; ++w) s += sums[w][lane];
+      s *= a.scale;
+      Vec<T, 1> o;
+      from_floats(&s, o);
+      static_cast<Vec<T, 1>*>(a.grad_table)[static_cast<int64_t>(row) * a.H + c] = o;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+// The widest vector that the rows of both tensors allow.
+template <typename T>
+int vector_of(const void* x, const void* y, int H) {
+  constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) |
+                         static_cast<uintptr_t>(static_cast<int64_t>(H) * sizeof(T));
+  return (bits & 15) == 0 ? kWide : (bits & 3) == 0 ? kPair : 1;
+}
+
+template <typename ID, typename T, int N>
+int forward_run(const EmbedArgs& a, cudaStream_t st) {
+  const dim3 block = row_block((a.H + N - 1) / N, 8);
+  return launch(embed_kernel<ID, T, N>, dim3((a.N + block.y - 1) / block.y), block, 0, st, a);
+}
+
+template <typename ID, typename V>
+int sort_run(const EmbedArgs& a, int64_t row_bytes, cudaStream_t st) {
+  static DeviceRecord record;
+  auto* kernel = embed_sort_kernel<ID, V>;
+  const int rc = allow_shared(record, kernel, sizeof(SortShared));
+  if (rc != MTP_OK) return rc;
+  const int rows = (a.V - 1) / kSms + 1;
+  return launch(kernel, dim3((a.V - 1) / rows + 1), dim3(kSortThreads), sizeof(SortShared), st, a, rows,
+                row_bytes / static_cast<int64_t>(sizeof(V)));
+}
+
+template <typename ID>
+int sort_run(const EmbedArgs& a, int64_t row_bytes, cudaStream_t st) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.grad_table) | static_cast<uintptr_t>(row_bytes);
+  if ((bits & 15) == 0) return sort_run<ID, uint4>(a, row_bytes, st);
+  if ((bits & 3) == 0) return sort_run<ID, uint32_t>(a, row_bytes, st);
+  return sort_run<ID, uint16_t>(a, row_bytes, st);
+}
+
+template <typename T, int N>
+int sum_run(const EmbedArgs& a, cudaStream_t st) {
+  const int64_t vectors = a.H / N, chunks = (static_cast<int64_t>(a.N) + a.chunk - 1) / a.chunk;
+  int lanes = 4;
+  while (lanes < vectors && lanes < 32) lanes *= 2;
+  const int64_t slices = (vectors + lanes - 1) / lanes, items = chunks * slices;
+  const int per = 256 / lanes;
+  if ((items + per - 1) / per > 0x7fffffff) return MTP_ERR_SHAPE;
+  int rc = launch(embed_sum_kernel<T, N>, dim3(static_cast<unsigned>((items + per - 1) / per)), dim3(lanes, per), 0, st,
+                  a, static_cast<int>(slices));
+  if (rc != MTP_OK || chunks == 1) return rc;
+  return launch(embed_join_kernel<T>, dim3(8 * kSms), dim3(kJoinWarps * 32), 0, st, a);
+}
+
+template <typename T>
+int run(const EmbedArgs& a, bool backward, cudaStream_t st) {
+  constexpr int kWide = 16 / sizeof(T), kPair = 4 / sizeof(T);
+  if (!backward) {
+    const int n = vector_of<T>(a.table, a.out, a.H);
+    if (a.wide_ids)
+      return n == kWide ? forward_run<int64_t, T, kWide>(a, st)
+             : n == 1   ? forward_run<int64_t, T, 1>(a, st)
+                        : forward_run<int64_t, T, kPair>(a, st);
+    return n == kWide ? forward_run<int32_t, T, kWide>(a, st)
+           : n == 1   ? forward_run<int32_t, T, 1>(a, st)
+                      : forward_run<int32_t, T, kPair>(a, st);
+  }
+  const int64_t row_bytes = static_cast<int64_t>(a.H) * sizeof(T);
+  const int rc = a.wide_ids ? sort_run<int64_t>(a, row_bytes, st) : sort_run<int32_t>(a, row_bytes, st);
+  if (rc != MTP_OK || a.N == 0) return rc;
+  const int n = vector_of<T>(a.grad, a.grad_table, a.H);
+  return n == kWide ? sum_run<T, kWide>(a, st) : n == 1 ? sum_run<T, 1>(a, st) : sum_run<T, kPair>(a, st);
+}
+
+int run(const EmbedArgs& a, int dtype, bool backward, cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return run<__nv_bfloat16>(a, backward, st);
+    case MTP_DTYPE_FP16: return run<__half>(a, backward, st);
+    default: return run<float>(a, backward, st);
+  }
+}
+
+}  // namespace
+
+EmbedWs embed_workspace(int N, int H, int dtype) {
+  EmbedWs w;
+  // chunks so long that the items (a warp for 512 bytes of a row) fill the GPU once
+  const int64_t slices = (static_cast<int64_t>(H) * (dtype == MTP_DTYPE_FP32 ? 4 : 2) + 511) / 512;
+  w.chunk = 16;
+  while (w.chunk < 256 && static_cast<int64_t>(N) * slices > 32ll * kSms * w.chunk) w.chunk *= 2;
+  const int64_t chunks = (static_cast<int64_t>(N) + w.chunk - 1) / w.chunk;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = round_up(at + bytes, 256);
+    return o;
+  };
+  w.valid = take(8);
+  w.owners = take(4 * chunks);
+  w.keys = take(8ll * N);
+  w.order = take(8ll * N);
+  w.parts = take(chunks > 1 ? 8 * chunks * H : 0);
+  w.total = at;
+  return w;
+}
+int launch_embed(const EmbedArgs& a, int dtype, cudaStream_t st) { return run(a, dtype, false, st); }
+int launch_embed_backward(const EmbedArgs& a, int dtype, cudaStream_t st) { return run(a, dtype, true, st); }
+
+}  // namespace mtp

@@ -195,6 +195,77 @@ int launch_unsort_tokens(const UnsortArgs& a, int dtype, cudaStream_t st);
 int launch_unsort_fp32_rows(const UnsortArgs& a, int out_dtype, cudaStream_t st);  // rows fp32, out of out_dtype
 int launch_unsort_backward(const UnsortArgs& a, int dtype, cudaStream_t st);
 
+// The router with its losses (route_loss.cu).
+struct RouteLossArgs {
+  int M, E, k, renorm;
+  int64_t stride;              // elements between the rows of logits
+  const void* logits;          // [M, E]
+  const uint8_t* mask;         // [M] or NULL: tokens that count
+  float* weights;              // [M, k]
+  int32_t* ids;                // [M, k]
+  int32_t* counts;             // [E]
+  float* balance;
+  float* z_loss;
+  float* pull;                 // [E + 1] for the gradient (or NULL): E counts[e] / (k n^2), then 2 / n
+  float* part_load;            // [parts, E]
+  int32_t* part_count;         // [parts, E]
+  double* part_sums;           // [parts, 2]: lse^2, tokens
+  const int32_t* ids_in;       // backward: [M, k]
+  const float* grad_weights;   // [M, k] or NULL
+  const float* grad_balance;   // [1] or NULL
+  const float* grad_z_loss;    // [1] or NULL
+  void* grad_logits;           // [M, E]
+};
+int64_t route_loss_parts(int M, int E);
+int launch_route_loss(const RouteLossArgs& a, int dtype, cudaStream_t st);
+int launch_route_loss_backward(const RouteLossArgs& a, int dtype, cudaStream_t st);
+
+// Layer norm (layer_norm.cu). param_fp32: weight, bias and their gradients are fp32, else of the rows' type.
+struct NormArgs {
+  int M, H;
+  bool param_fp32;
+  float eps;
+  int64_t stride;              // elements between the rows of x
+  const void* x;               // [M, H]
+  const void* weight;          // [H] or NULL (= 1)
+  const void* bias;            // [H] or NULL (= 0)
+  void* y;                     // [M, H]
+  float* stats;                // [M, 2] mean, 1 / sqrt(var + eps); forward: or NULL
+  const void* grad;            // [M, H]
+  void* grad_x;                // [M, H] or NULL
+  void* grad_weight;           // [H] or NULL
+  void* grad_bias;             // [H] or NULL
+  float* parts;                // [layer_norm_parts, 2, H]
+};
+int64_t layer_norm_parts(int M, int H);
+int launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t st);
+int launch_layer_norm_backward(const NormArgs& a, int dtype, cudaStream_t st);
+
+// Embedding (embedding.cu).
+struct EmbedArgs {
+  int N, V, H;
+  bool wide_ids;               // int64 ids, else int32
+  float scale;
+  const void* ids;             // [N]
+  const void* table;           // [V, H]
+  void* out;                   // [N, H]
+  const void* grad;            // [N, H]
+  void* grad_table;            // [V, H]
+  int chunk;                   // sorted tokens that a warp sums, and what embed_workspace lays out:
+  int32_t* valid;              // [2] tokens whose id is a row; entries of owners
+  int32_t* owners;             // [chunks] chunks in which a row begins that reaches over chunks
+  int32_t* keys;               // [2][N] their ids in order, and a buffer
+  int32_t* order;              // [2][N] their tokens
+  float* parts;                // [chunks][2][H] sums of rows that reach over chunks
+};
+struct EmbedWs {
+  int chunk;
+  int64_t valid, owners, keys, order, parts, total;
+};
+EmbedWs embed_workspace(int N, int H, int dtype);
+int launch_embed(const EmbedArgs& a, int dtype, cudaStream_t st);
+int launch_embed_backward(const EmbedArgs& a, int dtype, cudaStream_t st);
+
 // Rows to int8 (quantize.cu); strides in elements.
 int launch_quantize_int8(const void* x, int64_t x_stride, int dtype, int M, int K, int8_t* q, int64_t q_stride,
                          float* scale, cudaStream_t st);

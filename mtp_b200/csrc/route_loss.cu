@@ -1,0 +1,379 @@
+// The router of a training step: top-k weights with their gradient, the pairs
+// of every expert, the balance loss and the z loss.
+//
+// forward:  p = softmax(z[t]), ids = the k largest (ties: lowest id), w = p[ids],
+//           divided by their sum if renormalised. Over the n counted tokens:
+//           counts[e] = #{pairs of e}, load[e] = sum_t p[t, e],
+//           balance = sum_e pull[e] load[e] with pull[e] = E counts[e] / (k n^2),
+//           z_loss = sum_t lse(z[t])^2 / n.
+// gradient: with gb, gz of the losses and g of the weights, a[e] = gb pull[e],
+//           dz[e] = p[e] (a[e] - sum_i a[i] p[i] + gz 2/n lse)
+//                   + (e = ids[j]) w[j] (g[j] - sum_i g[i] w[i])   renormalised;
+//           without, g[j] is added to a[ids[j]] instead.
+//           counts have no gradient.
+//
+// A warp takes a token, its logits stay in registers. The sums over tokens go
+// warp by warp in registers, then over the warps, then over the CTAs, always in
+// the same order; the counts are integers. So results do not depend on timing.
+#include "rows.cuh"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace mtp {
+namespace {
+
+constexpr int kFinishCtas = 8;  // one cluster
+constexpr int kFinishThreads = 1024;
+constexpr int kOneCtaTokens = 64;  // up to here one CTA does all
+constexpr int kSms = 148;
+
+int loss_threads(int E) { return E <= 256 ? 512 : 256; }
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T, int VPT>
+__device__ __forceinline__ void load_row(const RouteLossArgs& a, int t, int lane, float (&v)[VPT]) {
+  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) v[i] = lane + 32 * i < a.E ? as_float(row[lane + 32 * i]) : -INFINITY;
+}
+
+// v -> exp(v - max) (0 past the last expert); returns max and sum.
+template <int VPT>
+__device__ __forceinline__ float2 softmax_row(int E, int lane, float (&v)[VPT]) {
+  float mx = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) mx = fmaxf(mx, v[i]);
+  mx = warp_max(mx);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    v[i] = lane + 32 * i < E ? expf(v[i] - mx) : 0.f;
+    s += v[i];
+  }
+  return make_float2(mx, warp_sum(s));
+}
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  return v;
+}
+
+// pull[e] of an expert, 0 without counted tokens.
+__device__ __forceinline__ float pull_of(const RouteLossArgs& a, int count, double n) {
+  return n > 0 ? static_cast<float>(static_cast<double>(a.E) * count / (static_cast<double>(a.k) * n * n)) : 0.f;
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const RouteLossArgs a) {
+  extern __shared__ __align__(16) float sm[];  // [warps][E] loads, then [E] counts
+  __shared__ double red[16][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int* hist = reinterpret_cast<int*>(sm + warps * a.E);
+  for (int e = tid; e < a.E; e += blockDim.x) hist[e] = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  float load[VPT], squares = 0.f;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) load[i] = 0.f;
+  for (int t = blockIdx.x * warps + warp; t < a.M; t += gridDim.x * warps) {
+    const int64_t o = static_cast<int64_t>(t) * a.k + lane;
+    if (a.mask && !a.mask[t]) {
+      if (lane < a.k) {
+        a.weights[o] = 0.f;
+        a.ids[o] = -1;
+      }
+      continue;
+    }
+    float v[VPT];
+    load_row<T>(a, t, lane, v);
+    // keys order like the logits: 0 is taken or absent, NaN comes last
+    uint32_t key[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const uint32_t bits = __float_as_uint(v[i] == 0.f ? 0.f : v[i]);  // -0 ties with 0
+      key[i] = lane + 32 * i >= a.E ? 0u : v[i] != v[i] ? 1u : bits >> 31 ? ~bits : bits | 0x80000000u;
+    }
+    const float2 ms = softmax_row<VPT>(a.E, lane, v);
+    float my_w = 0.f, wsum = 0.f;
+    int my_id = 0;
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = 0;
+      int at = 0;
+#pragma unroll
+      for (int i = VPT - 1; i >= 0; --i)
+        if (key[i] >= best) best = key[i], at = i;
+      const uint32_t top = __reduce_max_sync(kFullMask, best);
+      const int id = __reduce_min_sync(kFullMask, best == top ? static_cast<unsigned>(lane + 32 * at) : 0xffffu);
+      float p = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (lane + 32 * i == id) {
+          key[i] = 0;
+          p = v[i] / ms.y;
+        }
+      p = __shfl_sync(kFullMask, p, id & 31);
+      wsum += p;
+      if (lane == j) {
+        my_w = p;
+        my_id = id;
+      }
+    }
+    if (a.renorm) my_w = my_w / fmaxf(wsum, 1e-20f);
+    if (lane < a.k) {
+      a.weights[o] = my_w;
+      a.ids[o] = my_id;
+      atomicAdd(&hist[my_id], 1);
+    }
+    const float inv = 1.f / ms.y;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) load[i] = fmaf(v[i], inv, load[i]);
+    const float lse = ms.x + logf(ms.y);
+    squares = fmaf(lse, lse, squares);
+    ++n;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+    if (lane + 32 * i < a.E) sm[warp * a.E + lane + 32 * i] = load[i];
+  if (lane == 0) {
+    red[warp][0] = squares;
+    red[warp][1] = n;
+  }
+  __syncthreads();
+  double squares_all = 0, n_all = 0;
+  for (int w = 0; w < warps; ++w) {
+    squares_all += red[w][0];
+    n_all += red[w][1];
+  }
+  if (gridDim.x > 1) {  // route_finish_kernel sums over the CTAs
+    for (int e = tid; e < a.E; e += blockDim.x) {
+      float s = 0.f;
+      for (int w = 0; w < warps; ++w) s += sm[w * a.E + e];
+      a.part_load[static_cast<int64_t>(blockIdx.x) * a.E + e] = s;
+      a.part_count[static_cast<int64_t>(blockIdx.x) * a.E + e] = hist[e];
+    }
+    if (tid == 0) {
+      a.part_sums[2 * blockIdx.x] = squares_all;
+      a.part_sums[2 * blockIdx.x + 1] = n_all;
+    }
+    return;
+  }
+  double balance = 0;
+  for (int e = tid; e < a.E; e += blockDim.x) {
+    float s = 0.f;
+    for (int w = 0; w < warps; ++w) s += sm[w * a.E + e];
+    const float pull = pull_of(a, hist[e], n_all);
+    balance += static_cast<double>(pull) * s;
+    a.counts[e] = hist[e];
+    if (a.pull) a.pull[e] = pull;
+  }
+  balance = warp_sum64(balance);
+  __syncthreads();
+  if (lane == 0) red[warp][0] = balance;
+  __syncthreads();
+  if (tid == 0) {
+    balance = 0;
+    for (int w = 0; w < warps; ++w) balance += red[w][0];
+    *a.balance = static_cast<float>(balance);
+    *a.z_loss = n_all > 0 ? static_cast<float>(squares_all / n_all) : 0.f;
+    if (a.pull) a.pull[a.E] = n_all > 0 ? static_cast<float>(2. / n_all) : 0.f;
+  }
+}
+
+// The sums over the CTAs of route_loss_kernel: CTA r takes the experts
+// [128 r, 128 r + 128), eight threads each.
+__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads, 1)
+    route_finish_kernel(const RouteLossArgs a, int parts) {
+  __shared__ float loads[8][128];
+  __shared__ int counts[8][128];
+  __shared__ double sums[32][2];
+  __shared__ double balances[kFinishCtas];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x;
+  const int col = tid & 127, row = tid >> 7, e = rank * 128 + col;
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // this CTA runs: its shared memory may be written
+  pdl_launch_dependents();
+  pdl_wait();
+  float load = 0.f;
+  int count = 0;
+  if (e < a.E)
+#pragma unroll 4
+    for (int g = row; g < parts; g += 8) {
+      load += a.part_load[static_cast<int64_t>(g) * a.E + e];
+      count += a.part_count[static_cast<int64_t>(g) * a.E + e];
+    }
+  loads[row][col] = load;
+  counts[row][col] = count;
+  double squares = 0, n = 0;
+  for (int g = tid; g < parts; g += kFinishThreads) {
+    squares += a.part_sums[2 * g];
+    n += a.part_sums[2 * g + 1];
+  }
+  squares = warp_sum64(squares);
+  n = warp_sum64(n);
+  if (lane == 0) {
+    sums[warp][0] = squares;
+    sums[warp][1] = n;
+  }
+  __syncthreads();
+  squares = n = 0;
+  for (int w = 0; w < 32; ++w) {
+    squares += sums[w][0];
+    n += sums[w][1];
+  }
+  double balance = 0;
+  if (tid < 128 && e < a.E) {
+    load = 0.f;
+    count = 0;
+    for (int r = 0; r < 8; ++r) {
+      load += loads[r][col];
+      count += counts[r][col];
+    }
+    const float pull = pull_of(a, count, n);
+    balance = static_cast<double>(pull) * load;
+    a.counts[e] = count;
+    if (a.pull) a.pull[e] = pull;
+  }
+  __syncthreads();
+  balance = warp_sum64(balance);
+  if (lane == 0) sums[warp][0] = balance;
+  __syncthreads();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (tid == 0) {
+    balance = sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0];
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(smem_u32(&balances[rank])));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(balance) : "memory");
+  }
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+  if (rank == 0 && tid == 0) {
+    balance = 0;
+    for (int r = 0; r < kFinishCtas; ++r) balance += balances[r];
+    *a.balance = static_cast<float>(balance);
+    *a.z_loss = n > 0 ? static_cast<float>(squares / n) : 0.f;
+    if (a.pull) a.pull[a.E] = n > 0 ? static_cast<float>(2. / n) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T rounded(float v) {
+  Vec<T, 1> o;
+  from_floats(&v, o);
+  return o.v[0];
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const float gb = a.grad_balance ? *a.grad_balance : 0.f;
+  const float cz = a.grad_z_loss ? *a.grad_z_loss * a.pull[a.E] : 0.f;
+  float pull[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) pull[i] = a.grad_balance && lane + 32 * i < a.E ? gb * a.pull[lane + 32 * i] : 0.f;
+  for (int t = blockIdx.x * warps + warp; t < a.M; t += gridDim.x * warps) {
+    T* out = static_cast<T*>(a.grad_logits) + static_cast<int64_t>(t) * a.E;
+    if (a.mask && !a.mask[t]) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (lane + 32 * i < a.E) out[lane + 32 * i] = rounded<T>(0.f);
+      continue;
+    }
+    float v[VPT];
+    load_row<T>(a, t, lane, v);
+    int id = -1;
+    float g = 0.f, zj = 0.f;
+    if (a.grad_weights && lane < a.k) {
+      const int64_t o = static_cast<int64_t>(t) * a.k + lane;
+      id = a.ids_in[o];
+      g = a.grad_weights[o];
+      if (id < 0 || id >= a.E) id = -1;
+      if (id >= 0) zj = as_float((static_cast<const T*>(a.logits) + t * a.stride)[id]);
+    }
+    const float2 ms = softmax_row<VPT>(a.E, lane, v);
+    const float inv = 1.f / ms.y;
+    float mean = 0.f;  // sum_i a[i] p[i]
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      v[i] *= inv;
+      mean = fmaf(pull[i], v[i], mean);
+    }
+    float direct = 0.f, pj = 0.f;
+    if (a.grad_weights) {
+      pj = id >= 0 ? expf(zj - ms.x) * inv : 0.f;
+      if (a.renorm) {
+        const float w = pj / fmaxf(warp_sum(pj), 1e-20f);
+        const float wg = id >= 0 ? w * g : 0.f;
+        direct = w * (g - warp_sum(wg));
+      } else {
+        direct = id >= 0 ? pj * g : 0.f;
+        mean += direct;
+      }
+    }
+    mean = warp_sum(mean);
+    const float shift = (a.grad_z_loss ? cz * (ms.x + logf(ms.y)) : 0.f) - mean;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (lane + 32 * i < a.E) out[lane + 32 * i] = rounded<T>(v[i] * (pull[i] + shift));
+    if (a.grad_weights) {
+      __syncwarp();  // the chosen experts' entries once more, over the row's
+      if (id >= 0) out[id] = rounded<T>(fmaf(pj, (a.grad_balance ? gb * a.pull[id] : 0.f) + shift, direct));
+    }
+  }
+}
+
+}  // namespace
+
+// CTAs of route_loss_kernel whose sums route_finish_kernel takes, 0: none.
+int64_t route_loss_parts(int M, int E) {
+  if (M <= kOneCtaTokens) return 0;
+  const int warps = loss_threads(E) / 32;
+  return std::min<int64_t>((static_cast<int64_t>(M) + warps - 1) / warps, kSms * (16 / warps));
+}
+
+namespace {
+
+template <typename T, int VPT>
+int forward_run(const RouteLossArgs& a, cudaStream_t st) {
+  const int threads = loss_threads(a.E), ctas = static_cast<int>(std::max<int64_t>(route_loss_parts(a.M, a.E), 1));
+  const size_t smem = static_cast<size_t>(threads / 32 + 1) * a.E * sizeof(float);
+  const int rc = launch(route_loss_kernel<T, VPT>, dim3(ctas), dim3(threads), smem, st, a);
+  if (rc != MTP_OK || ctas == 1) return rc;
+  return launch(route_finish_kernel, dim3(kFinishCtas), dim3(kFinishThreads), 0, st, a, ctas);
+}
+
+template <typename T, int VPT>
+int backward_run(const RouteLossArgs& a, cudaStream_t st) {
+  return launch(route_backward_kernel<T, VPT>, dim3(std::min((a.M + 7) / 8, 8 * kSms)), dim3(256), 0, st, a);
+}
+
+template <typename T>
+int run(const RouteLossArgs& a, bool backward, cudaStream_t st) {
+  const int vpt = (a.E + 31) / 32;
+#define MTP_VPT(n)                                                                       \
+  if (vpt <= n) return backward ? backward_run<T, n>(a, st) : forward_run<T, n>(a, st);
+  MTP_VPT(1) MTP_VPT(2) MTP_VPT(4) MTP_VPT(8) MTP_VPT(16)
+#undef MTP_VPT
+  return backward ? backward_run<T, 32>(a, st) : forward_run<T, 32>(a, st);
+}
+
+int run(const RouteLossArgs& a, int dtype, bool backward, cudaStream_t st) {
+  switch (dtype) {
+    case MTP_DTYPE_BF16: return run<__nv_bfloat16>(a, backward, st);
+    case MTP_DTYPE_FP16: return run<__half>(a, backward, st);
+    default: return run<float>(a, backward, st);
+  }
+}
+
+}  // namespace
+
+int launch_route_loss(const RouteLossArgs& a, int dtype, cudaStream_t st) { return run(a, dtype, false, st); }
+int launch_route_loss_backward(const RouteLossArgs& a, int dtype, cudaStream_t st) { return run(a, dtype, true, st); }
+
+}  // namespace mtp
