@@ -4,10 +4,14 @@
 
 #include "internal.cuh"
 
+#include <string.h>
+
 namespace mtp {
 
-// N values of a row as fp32 and back. Conversions to 16 bits go in pairs: one
-// at a time they run at 16 a cycle and SM, below what HBM delivers.
+// N values of a row as fp32 and back, rounded to nearest even. Two 16-bit values
+// at a time: that is one instruction a value on the way in and one for both on
+// the way out (one value at a time, the conversions run at 16 a cycle and SM,
+// below what HBM delivers).
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
@@ -20,12 +24,24 @@ __device__ __forceinline__ void to_floats(const Vec<float, N>& x, float* f) {
 template <int N>
 __device__ __forceinline__ void to_floats(const Vec<__half, N>& x, float* f) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) f[n] = __half2float(x.v[n]);
+  for (int n = 0; n + 1 < N; n += 2) {
+    const float2 v = __half22float2(__halves2half2(x.v[n], x.v[n + 1]));
+    f[n] = v.x;
+    f[n + 1] = v.y;
+  }
+  if (N % 2) f[N - 1] = __half2float(x.v[N - 1]);
 }
 template <int N>
 __device__ __forceinline__ void to_floats(const Vec<__nv_bfloat16, N>& x, float* f) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) f[n] = __bfloat162float(x.v[n]);
+  for (int n = 0; n + 1 < N; n += 2) {
+    const __nv_bfloat162 h = __halves2bfloat162(x.v[n], x.v[n + 1]);
+    uint32_t bits;
+    memcpy(&bits, &h, 4);
+    f[n] = __uint_as_float(bits << 16);
+    f[n + 1] = __uint_as_float(bits & 0xffff0000u);
+  }
+  if (N % 2) f[N - 1] = __bfloat162float(x.v[N - 1]);
 }
 template <int N>
 __device__ __forceinline__ void from_floats(const float* f, Vec<float, N>& x) {
@@ -37,8 +53,7 @@ __device__ __forceinline__ void from_floats(const float* f, Vec<__half, N>& x) {
 #pragma unroll
   for (int n = 0; n + 1 < N; n += 2) {
     const __half2 h = __floats2half2_rn(f[n], f[n + 1]);
-    x.v[n] = __low2half(h);
-    x.v[n + 1] = __high2half(h);
+    memcpy(&x.v[n], &h, 4);
   }
   if (N % 2) x.v[N - 1] = __float2half_rn(f[N - 1]);
 }
@@ -47,8 +62,7 @@ __device__ __forceinline__ void from_floats(const float* f, Vec<__nv_bfloat16, N
 #pragma unroll
   for (int n = 0; n + 1 < N; n += 2) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(f[n], f[n + 1]);
-    x.v[n] = __low2bfloat16(h);
-    x.v[n + 1] = __high2bfloat16(h);
+    memcpy(&x.v[n], &h, 4);
   }
   if (N % 2) x.v[N - 1] = __float2bfloat16_rn(f[N - 1]);
 }
