@@ -28,7 +28,9 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSliceRows = 1 << 17;   // rows that a CTA takes at once: bits in shared memory
 constexpr int kCounted = 512;         // tokens of a slice that are sorted by counting
 constexpr int kDigitBits = 6;         // of a round of the radix sort
-constexpr int kJoinWarps = 8;
+constexpr int kBatch = 8;             // ids that a lane has in flight
+constexpr int kKept = 128;            // tokens of a warp's range that it keeps while it counts them
+constexpr int kJoinWarps = 16;
 
 template <typename ID>
 __device__ __forceinline__ int64_t id_at(const EmbedArgs& a, int i) {
@@ -38,6 +40,8 @@ __device__ __forceinline__ int64_t id_at(const EmbedArgs& a, int i) {
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
+constexpr int kVectors = 4;  // of a row that a thread has in flight
+
 template <typename ID, typename T, int N>
 __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
   using V = Vec<T, N>;
@@ -49,18 +53,27 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
   const bool here = id >= 0 && id < a.V;
   const T* row = static_cast<const T*>(a.table) + (here ? id : 0) * a.H;
   T* out = static_cast<T*>(a.out) + t * a.H;
-  for (int c = threadIdx.x * N; c < a.H; c += blockDim.x * N) {
-    float f[N];
+  const int step = blockDim.x * N;
+  for (int64_t c0 = threadIdx.x * N; c0 < a.H; c0 += kVectors * step) {
+    V v[kVectors];
 #pragma unroll
-    for (int n = 0; n < N; ++n) f[n] = 0.f;
-    if (here) {
-      to_floats(*reinterpret_cast<const V*>(row + c), f);
+    for (int i = 0; i < kVectors; ++i)
+      if (here && c0 + i * step < a.H) v[i] = *reinterpret_cast<const V*>(row + c0 + i * step);
 #pragma unroll
-      for (int n = 0; n < N; ++n) f[n] *= a.scale;
+    for (int i = 0; i < kVectors; ++i) {
+      if (c0 + i * step >= a.H) break;
+      float f[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) f[n] = 0.f;
+      if (here) {
+        to_floats(v[i], f);
+#pragma unroll
+        for (int n = 0; n < N; ++n) f[n] *= a.scale;
+      }
+      V o;
+      from_floats(f, o);
+      *reinterpret_cast<V*>(out + c0 + i * step) = o;
     }
-    V o;
-    from_floats(f, o);
-    *reinterpret_cast<V*>(out + c) = o;
   }
 }
 
@@ -74,6 +87,7 @@ struct SortShared {
   __align__(16) uint32_t key[kCounted];  // row << 9 | number in the slice
   int token[kCounted];
   int warp_in[kSortWarps], warp_below[kSortWarps];
+  int kept_row[kSortWarps][kKept], kept_token[kSortWarps][kKept];
 };
 
 // One stable round of the radix sort: entries [0, n) of (key, token) by `bits`
@@ -156,18 +170,30 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     for (int x = tid; x < (have + 31) / 32; x += kSortThreads) s.present[x] = 0;
     __syncthreads();
     int in = 0, below = 0;
-#pragma unroll 4
-    for (int i = begin; i < end; i += 32) {
-      const int64_t id = i + lane < end ? id_at<ID>(a, i + lane) : -1;
-      below += id >= 0 && id < lo;
-      const bool mine = id >= lo && id < lo64 + have;
-      if (mine) {
-        const int row = static_cast<int>(id - lo);
-        atomicOr(&s.present[row >> 5], 1u << (row & 31));
-        ++in;
+    // fn(i, id, whether it is of this slice) for this lane's ids, 32 of the warp at a time in order
+    auto walk = [&](auto fn) {
+      for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
+        int64_t id[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) id[u] = i0 + 32 * u + lane < end ? id_at<ID>(a, i0 + 32 * u + lane) : -1;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) fn(i0 + 32 * u + lane, id[u], id[u] >= lo && id[u] < lo64 + have);
       }
-    }
-    in = __reduce_add_sync(kFullMask, in);
+    };
+    walk([&](int i, int64_t id, bool mine) {
+      below += id >= 0 && id < lo;
+      const unsigned votes = __ballot_sync(kFullMask, mine);
+      if (votes == 0) return;
+      if (mine) {
+        const int row = static_cast<int>(id - lo), p = in + __popc(votes & ((1u << lane) - 1u));
+        atomicOr(&s.present[row >> 5], 1u << (row & 31));
+        if (p < kKept) {
+          s.kept_row[warp][p] = row;
+          s.kept_token[warp][p] = i;
+        }
+      }
+      in += __popc(votes);
+    });
     below = __reduce_add_sync(kFullMask, below);
     if (lane == 0) {
       s.warp_in[warp] = in;
@@ -190,21 +216,23 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
       const bool counted = n <= kCounted;
       int32_t* key_to = rounds & 1 ? key + a.N : key;
       int32_t* token_to = rounds & 1 ? token + a.N : token;
-      for (int i = begin; i < end; i += 32) {
-        const int64_t id = i + lane < end ? id_at<ID>(a, i + lane) : -1;
-        const bool mine = id >= lo && id < lo64 + have;
-        const unsigned votes = __ballot_sync(kFullMask, mine);
-        if (mine) {
-          const int p = at + __popc(votes & ((1u << lane) - 1u));
-          if (counted) {
-            s.key[p] = static_cast<uint32_t>(id - lo) << 9 | p;
-            s.token[p] = i + lane;
-          } else {
-            key_to[p] = static_cast<int>(id);
-            token_to[p] = i + lane;
-          }
+      auto put = [&](int p, int row, int t) {
+        if (counted) {
+          s.key[p] = static_cast<uint32_t>(row) << 9 | p;
+          s.token[p] = t;
+        } else {
+          key_to[p] = lo + row;
+          token_to[p] = t;
         }
-        at += __popc(votes);
+      };
+      if (in <= kKept) {
+        for (int x = lane; x < in; x += 32) put(at + x, s.kept_row[warp][x], s.kept_token[warp][x]);
+      } else {
+        walk([&](int i, int64_t id, bool mine) {
+          const unsigned votes = __ballot_sync(kFullMask, mine);
+          if (mine) put(at + __popc(votes & ((1u << lane) - 1u)), static_cast<int>(id - lo), i);
+          at += __popc(votes);
+        });
       }
       if (counted)
         for (int x = n + tid; x < (n + 3) / 4 * 4; x += kSortThreads) s.key[x] = 0xffffffffu;
@@ -242,6 +270,10 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
 // ---------------------------------------------------------------------------
 constexpr int kAhead = 8;  // tokens whose rows a thread has in flight
 
+// A row whose tokens reach over chunks is summed whole, by the item in whose
+// chunk it begins, if it has at most kWhole of them; so most rows need no parts.
+constexpr int kWhole = 64;
+
 // blockDim (lanes of an item, items): an item is a chunk of the sorted tokens
 // and as many columns as its lanes hold.
 template <typename T, int N>
@@ -254,14 +286,44 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int s
   const int valid = a.valid[0];
   const int64_t begin64 = static_cast<int64_t>(chunk) * a.chunk;
   if (begin64 >= valid) return;
-  const int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.chunk, static_cast<int64_t>(valid)));
-  const int64_t c = (static_cast<int64_t>(slice) * blockDim.x + threadIdx.x) * N;
-  const int head = begin > 0 ? a.keys[begin - 1] : -1;   // a row that reaches in
-  const int tail = end < valid ? a.keys[end] : -1;       // or out
+  int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.chunk, static_cast<int64_t>(valid)));
+  // the item's lanes count the equal keys from position i on, forwards or backwards, up to kWhole + 1
+  const unsigned lanes = (blockDim.x == 32 ? kFullMask : (1u << blockDim.x) - 1u)
+                         << ((threadIdx.y * blockDim.x) & 31);
+  const int first_lane = (threadIdx.y * blockDim.x) & 31;
+  auto run = [&](int i, int direction, int key) {
+    for (int n = 0; n <= kWhole; n += blockDim.x) {
+      const int64_t p = i + static_cast<int64_t>(direction) * (n + static_cast<int>(threadIdx.x));
+      const unsigned other = __ballot_sync(lanes, p < 0 || p >= valid || a.keys[p] != key) >> first_lane;
+      if (other) return n + __ffs(other) - 1;
+    }
+    return kWhole + 1;
+  };
   int row = a.keys[begin];
   const int last = a.keys[end - 1];
-  const bool owner = last == tail && !(row == last && row == head);
+  int head = begin > 0 && a.keys[begin - 1] == row ? row : -1;  // a row that reaches in
+  int tail = end < valid && a.keys[end] == last ? last : -1;    // or out
+  bool owner = false;
+  if (head >= 0) {
+    const int before = run(begin - 1, -1, row), behind = run(begin, 1, row);
+    if (before + behind <= kWhole) {  // whole, by another item
+      begin += behind;
+      head = -1;
+      if (begin >= end) return;
+      row = a.keys[begin];
+    }
+  }
+  if (tail >= 0 && !(head == tail)) {
+    const int before = run(end - 1, -1, last), behind = run(end, 1, last);
+    if (before + behind <= kWhole) {
+      end += behind;
+      tail = -1;
+    } else {
+      owner = true;
+    }
+  }
   if (owner && slice == 0 && threadIdx.x == 0) a.owners[atomicAdd(a.valid + 1, 1)] = chunk;
+  const int64_t c = (static_cast<int64_t>(slice) * blockDim.x + threadIdx.x) * N;
   if (c >= a.H) return;
   const T* grad = static_cast<const T*>(a.grad) + c;
   float acc[N];
@@ -322,15 +384,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const Embed
     const int chunk = a.owners[item / blocks];
     const int c = static_cast<int>(item % blocks) * 32 + lane;
     const int row = a.keys[(chunk + 1ll) * a.chunk];
-    int more = 0;  // chunks that the row reaches into
-    for (;;) {
-      const int64_t i = (chunk + 1ll + more + lane) * a.chunk;
-      const unsigned votes = __ballot_sync(kFullMask, i < valid && a.keys[i] == row);
-      if (votes != kFullMask) {
-        more += __ffs(~votes) - 1;
-        break;
+    // chunks that the row reaches into: a search among the chunks' first keys, 32 at a time
+    int more = 1;
+    for (int64_t left = (valid - 1) / a.chunk - chunk; more < left;) {  // the row has `more`, at most `left`
+      const int64_t stride = (left - more + 31) / 32;
+      const int64_t q = min(more + stride * (lane + 1), left);
+      const unsigned votes = __ballot_sync(kFullMask, a.keys[(chunk + q) * a.chunk] == row);
+      const int n = __popc(votes);  // the first n of them are the row's
+      if (n == 32) {
+        more = static_cast<int>(left);
+      } else {
+        left = min(more + stride * (n + 1), left) - 1;
+        more = static_cast<int>(min(more + stride * n, left));
       }
-      more += 32;
     }
     const int each = (more + kJoinWarps) / kJoinWarps;  // of more + 1 parts
     const int from = warp * each, to = min(from + each, more + 1);
@@ -366,7 +432,9 @@ int vector_of(const void* x, const void* y, int H) {
 
 template <typename ID, typename T, int N>
 int forward_run(const EmbedArgs& a, cudaStream_t st) {
-  const dim3 block = row_block((a.H + N - 1) / N, 8);
+  // a few tokens take all lanes at once
+  const int64_t vectors = (a.H + N - 1) / N;
+  const dim3 block = row_block(a.N > 2 * kSms ? (vectors + kVectors - 1) / kVectors : vectors, 8);
   return launch(embed_kernel<ID, T, N>, dim3((a.N + block.y - 1) / block.y), block, 0, st, a);
 }
 
@@ -437,7 +505,7 @@ EmbedWs embed_workspace(int N, int H, int dtype) {
   EmbedWs w;
   // chunks so long that the items (a warp for 512 bytes of a row) fill the GPU once
   const int64_t slices = (static_cast<int64_t>(H) * (dtype == MTP_DTYPE_FP32 ? 4 : 2) + 511) / 512;
-  w.chunk = 16;
+  w.chunk = 32;
   while (w.chunk < 256 && static_cast<int64_t>(N) * slices > 32ll * kSms * w.chunk) w.chunk *= 2;
   const int64_t chunks = (static_cast<int64_t>(N) + w.chunk - 1) / w.chunk;
   int64_t at = 0;

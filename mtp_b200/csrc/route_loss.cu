@@ -26,8 +26,9 @@ namespace {
 
 constexpr int kFinishCtas = 8;  // one cluster
 constexpr int kFinishThreads = 1024;
-constexpr int kOneCtaTokens = 64;  // up to here one CTA does all
+constexpr int kOneCtaTokens = 16;  // up to here one CTA does all
 constexpr int kSms = 148;
+constexpr int kTogether = 19;  // parts of a column that a thread has in flight: all of 148
 
 int loss_threads(int E) { return E <= 256 ? 512 : 256; }
 
@@ -68,10 +69,122 @@ __device__ __forceinline__ float pull_of(const RouteLossArgs& a, int count, doub
   return n > 0 ? static_cast<float>(static_cast<double>(a.E) * count / (static_cast<double>(a.k) * n * n)) : 0.f;
 }
 
+// Integers that order like numbers do (0 below all of them, NaN below -inf).
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t bits = __float_as_uint(v == 0.f ? 0.f : v);  // -0 ties with 0
+  return v != v ? 1u : bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+
+// What a warp's chosen experts give: lane j has the j-th, wsum is their
+// probabilities' sum in this order.
+__device__ __forceinline__ void write_choice(const RouteLossArgs& a, float p, int id, float wsum, int64_t o, int* hist) {
+  if (a.renorm) p = p / fmaxf(wsum, 1e-20f);
+  if ((threadIdx.x & 31) < a.k) {
+    a.weights[o] = p;
+    a.ids[o] = id;
+    atomicAdd(&hist[id], 1);
+  }
+}
+
+// The k largest, one after the other: a maximum over the warp each.
+template <typename T, int VPT>
+__device__ __noinline__ void choose_one_by_one(const RouteLossArgs& a, int t, float2 ms, int64_t o, int* hist) {
+  const int lane = threadIdx.x & 31;
+  float z[VPT];
+  load_row<T>(a, t, lane, z);
+  uint32_t key[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) key[i] = lane + 32 * i < a.E ? order_key(z[i]) : 0u;
+  float my_p = 0.f, wsum = 0.f;
+  int my_id = 0;
+  for (int j = 0; j < a.k; ++j) {
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = VPT - 1; i >= 0; --i)
+      if (key[i] >= best) best = key[i], at = i;
+    const uint32_t top = __reduce_max_sync(kFullMask, best);
+    const int id = __reduce_min_sync(kFullMask, best == top ? static_cast<unsigned>(lane + 32 * at) : 0xffffu);
+    float p = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (lane + 32 * i == id) {
+        key[i] = 0;
+        p = expf(z[i] - ms.x) / ms.y;
+      }
+    p = __shfl_sync(kFullMask, p, id & 31);
+    wsum += p;
+    if (lane == j) {
+      my_p = p;
+      my_id = id;
+    }
+  }
+  write_choice(a, my_p, my_id, wsum, o, hist);
+}
+
+struct Chosen {
+  float z[32];
+  int id[32];
+};
+
+// The same with less work: the k-th largest of the lanes' own maxima is no more
+// than the k-th largest of all, so that few values (the k, and those that share
+// a lane with one of them) are left to rank. Gives false, and does nothing,
+// where they are more than 32 or the row has a NaN.
+// 65536 tokens of 512 experts, top-8: one by one 192 us.
+template <int VPT>
+__device__ __forceinline__ bool choose(const RouteLossArgs& a, const float (&z)[VPT], float best, float2 ms, int64_t o,
+                                       Chosen& c, int* hist) {
+  const int lane = threadIdx.x & 31;
+  if (!(ms.y < INFINITY)) return false;
+  uint32_t mine = lane < a.E ? order_key(best) : 0u, least = 0;
+  for (int j = 0; j < a.k; ++j) {
+    least = __reduce_max_sync(kFullMask, mine);
+    const unsigned at = __ballot_sync(kFullMask, mine == least);
+    if (lane == __ffs(at) - 1) mine = 0;
+  }
+  // the number of that order; -inf where there are fewer lanes than choices
+  const float bound = least == 0 ? -INFINITY : __uint_as_float(least >> 31 ? least & 0x7fffffffu : ~least);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const bool in = z[i] >= bound && lane + 32 * i < a.E;
+    const unsigned votes = __ballot_sync(kFullMask, in);
+    if (votes == 0) continue;
+    const int at = n + __popc(votes & ((1u << lane) - 1u));
+    if (in && at < 32) {
+      c.z[at] = z[i];
+      c.id[at] = lane + 32 * i;
+    }
+    n += __popc(votes);
+  }
+  if (n > 32) return false;
+  __syncwarp();
+  const float my_z = lane < n ? c.z[lane] : -INFINITY;
+  const int my_id = lane < n ? c.id[lane] : 0x7fffffff;
+  int rank = 0;
+  for (int x = 0; x < n; ++x) {
+    const float other = c.z[x];
+    rank += other > my_z || (other == my_z && c.id[x] < my_id);
+  }
+  __syncwarp();
+  if (lane < n && rank < a.k) {
+    c.z[rank] = expf(my_z - ms.x) / ms.y;
+    c.id[rank] = my_id;
+  }
+  __syncwarp();
+  float wsum = 0.f;
+  for (int j = 0; j < a.k; ++j) wsum += c.z[j];
+  write_choice(a, c.z[lane], c.id[lane], wsum, o, hist);
+  __syncwarp();
+  return true;
+}
+
 template <typename T, int VPT>
 __global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const RouteLossArgs a) {
   extern __shared__ __align__(16) float sm[];  // [warps][E] loads, then [E] counts
   __shared__ double red[16][2];
+  __shared__ Chosen chosen[16];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   int* hist = reinterpret_cast<int*>(sm + warps * a.E);
   for (int e = tid; e < a.E; e += blockDim.x) hist[e] = 0;
@@ -91,46 +204,16 @@ __global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const 
       }
       continue;
     }
-    float v[VPT];
-    load_row<T>(a, t, lane, v);
-    // keys order like the logits: 0 is taken or absent, NaN comes last
-    uint32_t key[VPT];
+    float z[VPT], v[VPT];
+    load_row<T>(a, t, lane, z);
+    float best = -INFINITY;  // of this lane
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const uint32_t bits = __float_as_uint(v[i] == 0.f ? 0.f : v[i]);  // -0 ties with 0
-      key[i] = lane + 32 * i >= a.E ? 0u : v[i] != v[i] ? 1u : bits >> 31 ? ~bits : bits | 0x80000000u;
+      v[i] = z[i];
+      best = fmaxf(best, z[i]);
     }
     const float2 ms = softmax_row<VPT>(a.E, lane, v);
-    float my_w = 0.f, wsum = 0.f;
-    int my_id = 0;
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = 0;
-      int at = 0;
-#pragma unroll
-      for (int i = VPT - 1; i >= 0; --i)
-        if (key[i] >= best) best = key[i], at = i;
-      const uint32_t top = __reduce_max_sync(kFullMask, best);
-      const int id = __reduce_min_sync(kFullMask, best == top ? static_cast<unsigned>(lane + 32 * at) : 0xffffu);
-      float p = 0.f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (lane + 32 * i == id) {
-          key[i] = 0;
-          p = v[i] / ms.y;
-        }
-      p = __shfl_sync(kFullMask, p, id & 31);
-      wsum += p;
-      if (lane == j) {
-        my_w = p;
-        my_id = id;
-      }
-    }
-    if (a.renorm) my_w = my_w / fmaxf(wsum, 1e-20f);
-    if (lane < a.k) {
-      a.weights[o] = my_w;
-      a.ids[o] = my_id;
-      atomicAdd(&hist[my_id], 1);
-    }
+    if (!choose<VPT>(a, z, best, ms, o, chosen[warp], hist)) choose_one_by_one<T, VPT>(a, t, ms, o, hist);
     const float inv = 1.f / ms.y;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) load[i] = fmaf(v[i], inv, load[i]);
@@ -202,10 +285,21 @@ __global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThr
   float load = 0.f;
   int count = 0;
   if (e < a.E)
-#pragma unroll 4
-    for (int g = row; g < parts; g += 8) {
-      load += a.part_load[static_cast<int64_t>(g) * a.E + e];
-      count += a.part_count[static_cast<int64_t>(g) * a.E + e];
+    for (int g0 = row; g0 < parts; g0 += 8 * kTogether) {
+      float l[kTogether];
+      int n[kTogether];
+#pragma unroll
+      for (int x = 0; x < kTogether; ++x) {
+        const int64_t at = static_cast<int64_t>(g0 + 8 * x) * a.E + e;
+        const bool in = g0 + 8 * x < parts;
+        l[x] = in ? a.part_load[at] : 0.f;
+        n[x] = in ? a.part_count[at] : 0;
+      }
+#pragma unroll
+      for (int x = 0; x < kTogether; ++x) {
+        load += l[x];
+        count += n[x];
+      }
     }
   loads[row][col] = load;
   counts[row][col] = count;
