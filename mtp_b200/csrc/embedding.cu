@@ -33,9 +33,12 @@ constexpr int kKept = 128;            // tokens of a warp's range that it keeps 
 constexpr int kJoinWarps = 16;
 
 template <typename ID>
-__device__ __forceinline__ int64_t id_at(const EmbedArgs& a, int i) {
+__device__ __forceinline__ ID id_at(const EmbedArgs& a, int i) {
   return static_cast<const ID*>(a.ids)[i];
 }
+// An id as a number without sign: negative ones lie behind all rows.
+__device__ __forceinline__ uint32_t unsigned_id(int32_t id) { return static_cast<uint32_t>(id); }
+__device__ __forceinline__ uint64_t unsigned_id(int64_t id) { return static_cast<uint64_t>(id); }
 
 // ---------------------------------------------------------------------------
 // forward
@@ -173,15 +176,19 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     // fn(i, id, whether it is of this slice) for this lane's ids, 32 of the warp at a time in order
     auto walk = [&](auto fn) {
       for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
-        int64_t id[kBatch];
+        ID id[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) id[u] = i0 + 32 * u + lane < end ? id_at<ID>(a, i0 + 32 * u + lane) : -1;
+        for (int u = 0; u < kBatch; ++u) id[u] = i0 + 32 * u + lane < end ? id_at<ID>(a, i0 + 32 * u + lane) : ID(-1);
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) fn(i0 + 32 * u + lane, id[u], id[u] >= lo && id[u] < lo64 + have);
+        for (int u = 0; u < kBatch; ++u) {
+          const auto x = unsigned_id(id[u]);
+          using U = decltype(unsigned_id(id[u]));
+          fn(i0 + 32 * u + lane, x, x - static_cast<U>(lo) < static_cast<U>(have));
+        }
       }
     };
-    walk([&](int i, int64_t id, bool mine) {
-      below += id >= 0 && id < lo;
+    walk([&](int i, auto id, bool mine) {
+      below += id < static_cast<decltype(id)>(lo);
       const unsigned votes = __ballot_sync(kFullMask, mine);
       if (votes == 0) return;
       if (mine) {
@@ -228,7 +235,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
       if (in <= kKept) {
         for (int x = lane; x < in; x += 32) put(at + x, s.kept_row[warp][x], s.kept_token[warp][x]);
       } else {
-        walk([&](int i, int64_t id, bool mine) {
+        walk([&](int i, auto id, bool mine) {
           const unsigned votes = __ballot_sync(kFullMask, mine);
           if (mine) put(at + __popc(votes & ((1u << lane) - 1u)), static_cast<int>(id - lo), i);
           at += __popc(votes);
@@ -270,9 +277,10 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
 // ---------------------------------------------------------------------------
 constexpr int kAhead = 8;  // tokens whose rows a thread has in flight
 
-// A row whose tokens reach over chunks is summed whole, by the item in whose
-// chunk it begins, if it has at most kWhole of them; so most rows need no parts.
-constexpr int kWhole = 64;
+// A row that reaches over one border of chunks with fewer than kWhole tokens
+// behind it is summed whole by the item in whose chunk it begins; so most rows
+// need no parts. Chunks have at least kWhole tokens.
+constexpr int kWhole = 32;
 
 // blockDim (lanes of an item, items): an item is a chunk of the sorted tokens
 // and as many columns as its lanes hold.
@@ -287,17 +295,13 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int s
   const int64_t begin64 = static_cast<int64_t>(chunk) * a.chunk;
   if (begin64 >= valid) return;
   int begin = static_cast<int>(begin64), end = static_cast<int>(min(begin64 + a.chunk, static_cast<int64_t>(valid)));
-  // the item's lanes count the equal keys from position i on, forwards or backwards, up to kWhole + 1
-  const unsigned lanes = (blockDim.x == 32 ? kFullMask : (1u << blockDim.x) - 1u)
-                         << ((threadIdx.y * blockDim.x) & 31);
-  const int first_lane = (threadIdx.y * blockDim.x) & 31;
-  auto run = [&](int i, int direction, int key) {
-    for (int n = 0; n <= kWhole; n += blockDim.x) {
-      const int64_t p = i + static_cast<int64_t>(direction) * (n + static_cast<int>(threadIdx.x));
-      const unsigned other = __ballot_sync(lanes, p < 0 || p >= valid || a.keys[p] != key) >> first_lane;
-      if (other) return n + __ffs(other) - 1;
-    }
-    return kWhole + 1;
+  // the item's lanes count the keys equal to `key` among the kWhole from position i on
+  const unsigned lanes = (blockDim.x == 32 ? kFullMask : (1u << blockDim.x) - 1u) << ((threadIdx.y * blockDim.x) & 31);
+  auto run = [&](int i, int key) {
+    int n = 0;
+    for (int x = threadIdx.x; x < kWhole; x += blockDim.x)
+      n += static_cast<int64_t>(i) + x < valid && a.keys[static_cast<int64_t>(i) + x] == key;
+    return __reduce_add_sync(lanes, n);
   };
   int row = a.keys[begin];
   const int last = a.keys[end - 1];
@@ -305,18 +309,18 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int s
   int tail = end < valid && a.keys[end] == last ? last : -1;    // or out
   bool owner = false;
   if (head >= 0) {
-    const int before = run(begin - 1, -1, row), behind = run(begin, 1, row);
-    if (before + behind <= kWhole) {  // whole, by another item
-      begin += behind;
+    const int n = run(begin, row);
+    if (n < kWhole && !(begin > a.chunk && a.keys[begin - a.chunk - 1] == row)) {  // whole, by the item before
+      begin += n;
       head = -1;
       if (begin >= end) return;
       row = a.keys[begin];
     }
   }
-  if (tail >= 0 && !(head == tail)) {
-    const int before = run(end - 1, -1, last), behind = run(end, 1, last);
-    if (before + behind <= kWhole) {
-      end += behind;
+  if (tail >= 0 && head != tail) {
+    const int n = run(end, last);
+    if (n < kWhole) {
+      end += n;
       tail = -1;
     } else {
       owner = true;
@@ -370,19 +374,19 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int s
   write();
 }
 
-// A CTA takes a row that reaches over chunks and 32 of its columns; its warps
+// A CTA takes a row that reaches over chunks and 32 * N of its columns; its warps
 // share the chunks out evenly and in order.
-template <typename T>
+template <typename T, int N>
 __global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const EmbedArgs a) {
-  __shared__ float sums[kJoinWarps][32];
+  __shared__ Vec<float, N> sums[kJoinWarps][32];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int valid = a.valid[0], owners = a.valid[1];
-  const int blocks = (a.H + 31) / 32;
+  const int blocks = (a.H + 32 * N - 1) / (32 * N);
   for (int64_t item = blockIdx.x; item < static_cast<int64_t>(owners) * blocks; item += gridDim.x) {
     const int chunk = a.owners[item / blocks];
-    const int c = static_cast<int>(item % blocks) * 32 + lane;
+    const int64_t c = item % blocks * (32 * N) + lane * N;
     const int row = a.keys[(chunk + 1ll) * a.chunk];
     // chunks that the row reaches into: a search among the chunks' first keys, 32 at a time
     int more = 1;
@@ -400,19 +404,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const Embed
     }
     const int each = (more + kJoinWarps) / kJoinWarps;  // of more + 1 parts
     const int from = warp * each, to = min(from + each, more + 1);
-    float s = 0.f;
+    Vec<float, N> s = {};
     if (c < a.H)
 #pragma unroll 8
-      for (int p = from; p < to; ++p) s += a.parts[(2ll * (chunk + p) + (p == 0 ? 1 : 0)) * a.H + c];
+      for (int p = from; p < to; ++p) {
+        const Vec<float, N> v = *reinterpret_cast<const Vec<float, N>*>(a.parts + (2ll * (chunk + p) + (p == 0 ? 1 : 0)) * a.H + c);
+#pragma unroll
+        for (int n = 0; n < N; ++n) s.v[n] += v.v[n];
+      }
     sums[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && c < a.H) {
-      s = 0.f;
-      for (int w = 0; w < kJoinWarps; ++w) s += sums[w][lane];
-      s *= a.scale;
-      Vec<T, 1> o;
-      from_floats(&s, o);
-      static_cast<Vec<T, 1>*>(a.grad_table)[static_cast<int64_t>(row) * a.H + c] = o;
+      float f[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) f[n] = 0.f;
+      for (int w = 0; w * each <= more; ++w) {
+        const Vec<float, N> v = sums[w][lane];
+#pragma unroll
+        for (int n = 0; n < N; ++n) f[n] += v.v[n];
+      }
+      T* out = static_cast<T*>(a.grad_table) + static_cast<int64_t>(row) * a.H + c;
+#pragma unroll
+      for (int n = 0; n < N; ++n) f[n] *= a.scale;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        Vec<T, 1> o;
+        from_floats(f + n, o);
+        reinterpret_cast<Vec<T, 1>*>(out)[n] = o;
+      }
     }
     __syncthreads();
   }
@@ -468,7 +487,7 @@ int sum_run(const EmbedArgs& a, cudaStream_t st) {
   int rc = launch(embed_sum_kernel<T, N>, dim3(static_cast<unsigned>((items + per - 1) / per)), dim3(lanes, per), 0, st,
                   a, static_cast<int>(slices));
   if (rc != MTP_OK || chunks == 1) return rc;
-  return launch(embed_join_kernel<T>, dim3(8 * kSms), dim3(kJoinWarps * 32), 0, st, a);
+  return launch(a.H % 4 ? embed_join_kernel<T, 1> : embed_join_kernel<T, 4>, dim3(4 * kSms), dim3(kJoinWarps * 32), 0, st, a);
 }
 
 template <typename T>
@@ -505,7 +524,7 @@ EmbedWs embed_workspace(int N, int H, int dtype) {
   EmbedWs w;
   // chunks so long that the items (a warp for 512 bytes of a row) fill the GPU once
   const int64_t slices = (static_cast<int64_t>(H) * (dtype == MTP_DTYPE_FP32 ? 4 : 2) + 511) / 512;
-  w.chunk = 32;
+  w.chunk = 32;  // at least embed_sum_kernel's kWhole
   while (w.chunk < 256 && static_cast<int64_t>(N) * slices > 32ll * kSms * w.chunk) w.chunk *= 2;
   const int64_t chunks = (static_cast<int64_t>(N) + w.chunk - 1) / w.chunk;
   int64_t at = 0;

@@ -30,29 +30,53 @@ constexpr int kOneCtaTokens = 16;  // up to here one CTA does all
 constexpr int kSms = 148;
 constexpr int kTogether = 19;  // parts of a column that a thread has in flight: all of 148
 
-int loss_threads(int E) { return E <= 256 ? 512 : 256; }
+// Warps of a CTA: a token each as far as the SMs go, then what registers allow.
+int loss_warps(int M, int E) {
+  return M <= kOneCtaTokens ? kOneCtaTokens : std::max(4, std::min((M - 1) / kSms + 1, E <= 256 ? 32 : 16));
+}
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <typename T, int VPT>
-__device__ __forceinline__ void load_row(const RouteLossArgs& a, int t, int lane, float (&v)[VPT]) {
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) v[i] = lane + 32 * i < a.E ? as_float(row[lane + 32 * i]) : -INFINITY;
+// Whether the lane's i-th expert is one; FULL: E is 32 VPT.
+template <bool FULL>
+__device__ __forceinline__ bool has(const RouteLossArgs& a, int lane, int i) {
+  return FULL || lane + 32 * i < a.E;
 }
 
-// v -> exp(v - max) (0 past the last expert); returns max and sum.
+template <bool FULL, typename T, int VPT>
+__device__ __forceinline__ void load_row(const RouteLossArgs& a, int t, int lane, float (&v)[VPT]) {
+  const T* row = static_cast<const T*>(a.logits) + t * a.stride + lane;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) v[i] = has<FULL>(a, lane, i) ? as_float(row[32 * i]) : -INFINITY;
+}
+
 template <int VPT>
-__device__ __forceinline__ float2 softmax_row(int E, int lane, float (&v)[VPT]) {
-  float mx = -INFINITY, s = 0.f;
+__device__ __forceinline__ float row_max(const float (&v)[VPT]) {
+  float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) mx = fmaxf(mx, v[i]);
-  mx = warp_max(mx);
+  return warp_max(mx);
+}
+
+// v -> exp(v - max) (0 past the last expert); returns max and sum. The forward
+// pass has the exponential of mtp_router_topk, so that both give the same bits.
+// FAST: by one instruction; its argument (v - max) log2(e) is rounded once, an
+// error of |v - max| 2^-24 of the result, and what max log2(e) loses all
+// values of the row share.
+template <bool FULL, bool FAST, int VPT>
+__device__ __forceinline__ float2 softmax_row(const RouteLossArgs& a, int lane, float (&v)[VPT], float mx) {
+  float s = 0.f;
+  const float shift = -mx * 1.44269504f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    v[i] = lane + 32 * i < E ? expf(v[i] - mx) : 0.f;
+    float e;
+    if (FAST)
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(v[i], 1.44269504f, shift)));
+    else
+      e = expf(v[i] - mx);
+    v[i] = has<FULL>(a, lane, i) ? e : 0.f;
     s += v[i];
   }
   return make_float2(mx, warp_sum(s));
@@ -86,33 +110,28 @@ __device__ __forceinline__ void write_choice(const RouteLossArgs& a, float p, in
   }
 }
 
-// The k largest, one after the other: a maximum over the warp each.
-template <typename T, int VPT>
-__device__ __noinline__ void choose_one_by_one(const RouteLossArgs& a, int t, float2 ms, int64_t o, int* hist) {
+// The k largest, one after the other: a maximum over the warp each. For the few
+// rows that choose() does not take: it keeps no registers and reads the row again.
+template <typename T>
+__device__ __forceinline__ void choose_one_by_one(const RouteLossArgs& a, int t, float2 ms, int64_t o, int* hist) {
   const int lane = threadIdx.x & 31;
-  float z[VPT];
-  load_row<T>(a, t, lane, z);
-  uint32_t key[VPT];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) key[i] = lane + 32 * i < a.E ? order_key(z[i]) : 0u;
+  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
+  uint32_t taken = 0;  // of this lane's experts
   float my_p = 0.f, wsum = 0.f;
   int my_id = 0;
+#pragma unroll 1
   for (int j = 0; j < a.k; ++j) {
     uint32_t best = 0;
     int at = 0;
-#pragma unroll
-    for (int i = VPT - 1; i >= 0; --i)
-      if (key[i] >= best) best = key[i], at = i;
+#pragma unroll 1
+    for (int i = 0; lane + 32 * i < a.E; ++i) {
+      const uint32_t key = taken >> i & 1 ? 0u : order_key(as_float(row[lane + 32 * i]));
+      if (key > best) best = key, at = i;
+    }
     const uint32_t top = __reduce_max_sync(kFullMask, best);
     const int id = __reduce_min_sync(kFullMask, best == top ? static_cast<unsigned>(lane + 32 * at) : 0xffffu);
-    float p = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (lane + 32 * i == id) {
-        key[i] = 0;
-        p = expf(z[i] - ms.x) / ms.y;
-      }
-    p = __shfl_sync(kFullMask, p, id & 31);
+    if (lane == (id & 31)) taken |= 1u << (id >> 5);
+    const float p = expf(as_float(row[id]) - ms.x) / ms.y;
     wsum += p;
     if (lane == j) {
       my_p = p;
@@ -123,68 +142,73 @@ __device__ __noinline__ void choose_one_by_one(const RouteLossArgs& a, int t, fl
 }
 
 struct Chosen {
-  float z[32];
-  int id[32];
+  struct alignas(8) {
+    float z;
+    int id;
+  } at[32];
 };
 
 // The same with less work: the k-th largest of the lanes' own maxima is no more
 // than the k-th largest of all, so that few values (the k, and those that share
-// a lane with one of them) are left to rank. Gives false, and does nothing,
-// where they are more than 32 or the row has a NaN.
-// 65536 tokens of 512 experts, top-8: one by one 192 us.
+// a lane with one of them) are left to rank. Gives their number, 0 where they
+// are more than 32 or there is no finite one.
+// 65536 tokens of 512 experts, top-8: one by one 195 us, so 106 us.
 template <int VPT>
-__device__ __forceinline__ bool choose(const RouteLossArgs& a, const float (&z)[VPT], float best, float2 ms, int64_t o,
-                                       Chosen& c, int* hist) {
+__device__ __forceinline__ int candidates(const RouteLossArgs& a, const float (&z)[VPT], float best, Chosen& c) {
   const int lane = threadIdx.x & 31;
-  if (!(ms.y < INFINITY)) return false;
   uint32_t mine = lane < a.E ? order_key(best) : 0u, least = 0;
   for (int j = 0; j < a.k; ++j) {
     least = __reduce_max_sync(kFullMask, mine);
     const unsigned at = __ballot_sync(kFullMask, mine == least);
     if (lane == __ffs(at) - 1) mine = 0;
   }
-  // the number of that order; -inf where there are fewer lanes than choices
-  const float bound = least == 0 ? -INFINITY : __uint_as_float(least >> 31 ? least & 0x7fffffffu : ~least);
+  // the number of that order
+  const float bound = __uint_as_float(least >> 31 ? least & 0x7fffffffu : ~least);
+  if (!(bound > -INFINITY)) return 0;
   int n = 0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const bool in = z[i] >= bound && lane + 32 * i < a.E;
+    const bool in = z[i] >= bound;  // -inf past the last expert
     const unsigned votes = __ballot_sync(kFullMask, in);
     if (votes == 0) continue;
     const int at = n + __popc(votes & ((1u << lane) - 1u));
     if (in && at < 32) {
-      c.z[at] = z[i];
-      c.id[at] = lane + 32 * i;
+      c.at[at].z = z[i];
+      c.at[at].id = lane + 32 * i;
     }
     n += __popc(votes);
   }
-  if (n > 32) return false;
+  return n <= 32 ? n : 0;
+}
+
+__device__ __forceinline__ void choose(const RouteLossArgs& a, int n, float2 ms, int64_t o, Chosen& c, int* hist) {
+  const int lane = threadIdx.x & 31;
   __syncwarp();
-  const float my_z = lane < n ? c.z[lane] : -INFINITY;
-  const int my_id = lane < n ? c.id[lane] : 0x7fffffff;
+  const auto mine = c.at[lane];  // of a lane below n
   int rank = 0;
+#pragma unroll 4
   for (int x = 0; x < n; ++x) {
-    const float other = c.z[x];
-    rank += other > my_z || (other == my_z && c.id[x] < my_id);
+    const auto other = c.at[x];
+    rank += other.z > mine.z || (other.z == mine.z && other.id < mine.id);
   }
   __syncwarp();
   if (lane < n && rank < a.k) {
-    c.z[rank] = expf(my_z - ms.x) / ms.y;
-    c.id[rank] = my_id;
+    c.at[rank].z = expf(mine.z - ms.x) / ms.y;
+    c.at[rank].id = mine.id;
   }
   __syncwarp();
   float wsum = 0.f;
-  for (int j = 0; j < a.k; ++j) wsum += c.z[j];
-  write_choice(a, c.z[lane], c.id[lane], wsum, o, hist);
+  for (int j = 0; j < a.k; ++j) wsum += c.at[j].z;
+  write_choice(a, c.at[lane].z, c.at[lane].id, wsum, o, hist);
   __syncwarp();
-  return true;
 }
 
-template <typename T, int VPT>
-__global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const RouteLossArgs a) {
+
+template <typename T, int VPT, bool FULL>
+__global__ void __launch_bounds__(VPT <= 8 ? 1024 : 512, 1) route_loss_kernel(const RouteLossArgs a) {
   extern __shared__ __align__(16) float sm[];  // [warps][E] loads, then [E] counts
-  __shared__ double red[16][2];
-  __shared__ Chosen chosen[16];
+  __shared__ double red[32][2];
+  __shared__ Chosen chosen[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   int* hist = reinterpret_cast<int*>(sm + warps * a.E);
   for (int e = tid; e < a.E; e += blockDim.x) hist[e] = 0;
@@ -192,11 +216,19 @@ __global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const 
   pdl_wait();
   __syncthreads();
   float load[VPT], squares = 0.f;
-  int n = 0;
+  int tokens = 0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) load[i] = 0.f;
-  for (int t = blockIdx.x * warps + warp; t < a.M; t += gridDim.x * warps) {
+  const int step = gridDim.x * warps;
+  float ahead[VPT];  // the next token's logits, on their way while this one's are ranked
+  int t = blockIdx.x * warps + warp;
+  if (t < a.M) load_row<FULL, T>(a, t, lane, ahead);
+  for (; t < a.M; t += step) {
     const int64_t o = static_cast<int64_t>(t) * a.k + lane;
+    float v[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) v[i] = ahead[i];
+    if (t + step < a.M) load_row<FULL, T>(a, t + step, lane, ahead);
     if (a.mask && !a.mask[t]) {
       if (lane < a.k) {
         a.weights[o] = 0.f;
@@ -204,29 +236,28 @@ __global__ void __launch_bounds__(VPT <= 8 ? 512 : 256) route_loss_kernel(const 
       }
       continue;
     }
-    float z[VPT], v[VPT];
-    load_row<T>(a, t, lane, z);
     float best = -INFINITY;  // of this lane
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      v[i] = z[i];
-      best = fmaxf(best, z[i]);
-    }
-    const float2 ms = softmax_row<VPT>(a.E, lane, v);
-    if (!choose<VPT>(a, z, best, ms, o, chosen[warp], hist)) choose_one_by_one<T, VPT>(a, t, ms, o, hist);
+    for (int i = 0; i < VPT; ++i) best = fmaxf(best, v[i]);
+    const int n = candidates<VPT>(a, v, best, chosen[warp]);
+    const float2 ms = softmax_row<FULL, false>(a, lane, v, warp_max(best));
+    if (n && ms.y < INFINITY)  // no NaN among them
+      choose(a, n, ms, o, chosen[warp], hist);
+    else
+      choose_one_by_one<T>(a, t, ms, o, hist);
     const float inv = 1.f / ms.y;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) load[i] = fmaf(v[i], inv, load[i]);
     const float lse = ms.x + logf(ms.y);
     squares = fmaf(lse, lse, squares);
-    ++n;
+    ++tokens;
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
     if (lane + 32 * i < a.E) sm[warp * a.E + lane + 32 * i] = load[i];
   if (lane == 0) {
     red[warp][0] = squares;
-    red[warp][1] = n;
+    red[warp][1] = tokens;
   }
   __syncthreads();
   double squares_all = 0, n_all = 0;
@@ -361,7 +392,7 @@ __device__ __forceinline__ T rounded(float v) {
   return o.v[0];
 }
 
-template <typename T, int VPT>
+template <typename T, int VPT, bool FULL>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   pdl_launch_dependents();
@@ -370,17 +401,17 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
   const float cz = a.grad_z_loss ? *a.grad_z_loss * a.pull[a.E] : 0.f;
   float pull[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) pull[i] = a.grad_balance && lane + 32 * i < a.E ? gb * a.pull[lane + 32 * i] : 0.f;
+  for (int i = 0; i < VPT; ++i) pull[i] = a.grad_balance && has<FULL>(a, lane, i) ? gb * a.pull[lane + 32 * i] : 0.f;
   for (int t = blockIdx.x * warps + warp; t < a.M; t += gridDim.x * warps) {
     T* out = static_cast<T*>(a.grad_logits) + static_cast<int64_t>(t) * a.E;
     if (a.mask && !a.mask[t]) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
-        if (lane + 32 * i < a.E) out[lane + 32 * i] = rounded<T>(0.f);
+        if (has<FULL>(a, lane, i)) out[lane + 32 * i] = rounded<T>(0.f);
       continue;
     }
     float v[VPT];
-    load_row<T>(a, t, lane, v);
+    load_row<FULL, T>(a, t, lane, v);
     int id = -1;
     float g = 0.f, zj = 0.f;
     if (a.grad_weights && lane < a.k) {
@@ -390,7 +421,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
       if (id < 0 || id >= a.E) id = -1;
       if (id >= 0) zj = as_float((static_cast<const T*>(a.logits) + t * a.stride)[id]);
     }
-    const float2 ms = softmax_row<VPT>(a.E, lane, v);
+    const float2 ms = softmax_row<FULL, true>(a, lane, v, row_max(v));
     const float inv = 1.f / ms.y;
     float mean = 0.f;  // sum_i a[i] p[i]
 #pragma unroll
@@ -400,7 +431,8 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
     }
     float direct = 0.f, pj = 0.f;
     if (a.grad_weights) {
-      pj = id >= 0 ? expf(zj - ms.x) * inv : 0.f;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(pj) : "f"(fmaf(zj, 1.44269504f, -ms.x * 1.44269504f)));
+      pj = id >= 0 ? pj * inv : 0.f;
       if (a.renorm) {
         const float w = pj / fmaxf(warp_sum(pj), 1e-20f);
         const float wg = id >= 0 ? w * g : 0.f;
@@ -414,7 +446,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
     const float shift = (a.grad_z_loss ? cz * (ms.x + logf(ms.y)) : 0.f) - mean;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if (lane + 32 * i < a.E) out[lane + 32 * i] = rounded<T>(v[i] * (pull[i] + shift));
+      if (has<FULL>(a, lane, i)) out[lane + 32 * i] = rounded<T>(v[i] * (pull[i] + shift));
     if (a.grad_weights) {
       __syncwarp();  // the chosen experts' entries once more, over the row's
       if (id >= 0) out[id] = rounded<T>(fmaf(pj, (a.grad_balance ? gb * a.pull[id] : 0.f) + shift, direct));
@@ -427,34 +459,39 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
 // CTAs of route_loss_kernel whose sums route_finish_kernel takes, 0: none.
 int64_t route_loss_parts(int M, int E) {
   if (M <= kOneCtaTokens) return 0;
-  const int warps = loss_threads(E) / 32;
-  return std::min<int64_t>((static_cast<int64_t>(M) + warps - 1) / warps, kSms * (16 / warps));
+  const int warps = loss_warps(M, E);
+  return std::min<int64_t>((static_cast<int64_t>(M) + warps - 1) / warps, kSms);
 }
 
 namespace {
 
-template <typename T, int VPT>
+template <typename T, int VPT, bool FULL>
 int forward_run(const RouteLossArgs& a, cudaStream_t st) {
-  const int threads = loss_threads(a.E), ctas = static_cast<int>(std::max<int64_t>(route_loss_parts(a.M, a.E), 1));
+  const int threads = 32 * loss_warps(a.M, a.E), ctas = static_cast<int>(std::max<int64_t>(route_loss_parts(a.M, a.E), 1));
   const size_t smem = static_cast<size_t>(threads / 32 + 1) * a.E * sizeof(float);
-  const int rc = launch(route_loss_kernel<T, VPT>, dim3(ctas), dim3(threads), smem, st, a);
+  static DeviceRecord record;
+  const int allowed = allow_shared(record, route_loss_kernel<T, VPT, FULL>, static_cast<size_t>(VPT <= 8 ? 33 : 17) * 32 * VPT * sizeof(float));
+  if (allowed != MTP_OK) return allowed;
+  const int rc = launch(route_loss_kernel<T, VPT, FULL>, dim3(ctas), dim3(threads), smem, st, a);
   if (rc != MTP_OK || ctas == 1) return rc;
   return launch(route_finish_kernel, dim3(kFinishCtas), dim3(kFinishThreads), 0, st, a, ctas);
 }
 
-template <typename T, int VPT>
+template <typename T, int VPT, bool FULL>
 int backward_run(const RouteLossArgs& a, cudaStream_t st) {
-  return launch(route_backward_kernel<T, VPT>, dim3(std::min((a.M + 7) / 8, 8 * kSms)), dim3(256), 0, st, a);
+  return launch(route_backward_kernel<T, VPT, FULL>, dim3(std::min((a.M + 7) / 8, 8 * kSms)), dim3(256), 0, st, a);
 }
 
 template <typename T>
 int run(const RouteLossArgs& a, bool backward, cudaStream_t st) {
   const int vpt = (a.E + 31) / 32;
-#define MTP_VPT(n)                                                                       \
-  if (vpt <= n) return backward ? backward_run<T, n>(a, st) : forward_run<T, n>(a, st);
+#define MTP_RUN(n, full) (backward ? backward_run<T, n, full>(a, st) : forward_run<T, n, full>(a, st))
+#define MTP_VPT(n) \
+  if (vpt <= n) return a.E == 32 * n ? MTP_RUN(n, true) : MTP_RUN(n, false);
   MTP_VPT(1) MTP_VPT(2) MTP_VPT(4) MTP_VPT(8) MTP_VPT(16)
 #undef MTP_VPT
-  return backward ? backward_run<T, 32>(a, st) : forward_run<T, 32>(a, st);
+  return a.E == 1024 ? MTP_RUN(32, true) : MTP_RUN(32, false);
+#undef MTP_RUN
 }
 
 int run(const RouteLossArgs& a, int dtype, bool backward, cudaStream_t st) {
