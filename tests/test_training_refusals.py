@@ -152,9 +152,9 @@ def test_the_tensors_device_is_current_at_the_launch(built_lib, monkeypatch, ind
         z = lambda *shape, dtype=F32: torch.empty(*shape, dtype=dtype, device=f"cuda:{index}")
         for name, call in [
             ("route", lambda: mtp_b200.route_tokens(z(4, 8), 2)),
-            ("route_backward", lambda: training._route_backward(z(4, 8), 2, True, None, z(4, 2, dtype=I32), z(9), z(4, 2), None, None)),
+            ("route_backward", lambda: training._route_backward(z(4, 8), 8, 2, True, None, z(4, 2, dtype=I32), z(9), z(4, 2), None, None)),
             ("norm", lambda: mtp_b200.layer_norm(z(4, 8), z(8), z(8))),
-            ("norm_backward", lambda: training._norm_backward(z(4, 8), z(4, 8), z(8), z(4, 2), F32, True, True, True)),
+            ("norm_backward", lambda: training._norm_backward(z(4, 8), z(4, 8), (4, 8), z(8), z(4, 2), F32, True, True, True)),
             ("embed", lambda: mtp_b200.embed_tokens(z(4, dtype=I32), z(5, 8))),
             ("embed_backward", lambda: training._embed_backward(z(4, dtype=I32), z(4, 8), 5, 1.0)),
         ]:
