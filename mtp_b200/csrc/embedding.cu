@@ -28,14 +28,19 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSliceRows = 1 << 17;   // rows that a CTA takes at once: bits in shared memory
 constexpr int kCounted = 512;         // tokens of a slice that are sorted by counting
 constexpr int kDigitBits = 6;         // of a round of the radix sort
-constexpr int kBatch = 8;             // ids that a lane has in flight
-constexpr int kKept = 128;            // tokens of a warp's range that it keeps while it counts them
-constexpr int kJoinWarps = 16;
+constexpr int kBatch = 4;             // times four ids that a lane has in flight
+constexpr int kKept = 256;            // tokens of a warp's range that it keeps while it counts them
+constexpr int kListed = 8192;         // tokens of a slice that are sorted in shared memory
+constexpr int kJoinThreads = 512;
 
 template <typename ID>
 __device__ __forceinline__ ID id_at(const EmbedArgs& a, int i) {
   return static_cast<const ID*>(a.ids)[i];
 }
+template <typename ID>
+struct alignas(16) Four {
+  ID id[4];
+};
 // An id as a number without sign: negative ones lie behind all rows.
 __device__ __forceinline__ uint32_t unsigned_id(int32_t id) { return static_cast<uint32_t>(id); }
 __device__ __forceinline__ uint64_t unsigned_id(int64_t id) { return static_cast<uint64_t>(id); }
@@ -90,8 +95,9 @@ struct SortShared {
   __align__(16) uint32_t key[kCounted];  // row << 9 | number in the slice
   int token[kCounted];
   int warp_in[kSortWarps], warp_below[kSortWarps];
-  int kept_row[kSortWarps][kKept], kept_token[kSortWarps][kKept];
+  int list[2][2][kListed];  // two lists of keys and tokens; the second keeps the warps' tokens before that
 };
+static_assert(kSortWarps * kKept <= kListed, "the second list holds what the warps keep");
 
 // One stable round of the radix sort: entries [0, n) of (key, token) by `bits`
 // bits of key - lo from `shift` on.
@@ -130,12 +136,17 @@ __device__ void radix_round(SortShared& s, const int32_t* key, const int32_t* to
     s.start[tid] = run;
   }
   __syncthreads();
-  if (tid == 0) {
+  if (warp == 0) {  // the digits' first places
     int run = 0;
-    for (int b = 0; b < bins; ++b) {
-      const int v = s.start[b];
-      s.start[b] = run;
-      run += v;
+    for (int b0 = 0; b0 < bins; b0 += 32) {
+      const int v = b0 + lane < bins ? s.start[b0 + lane] : 0;
+      int sum = v;
+      for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(kFullMask, sum, o);
+        if (lane >= o) sum += x;
+      }
+      if (b0 + lane < bins) s.start[b0 + lane] = run + sum - v;
+      run += __shfl_sync(kFullMask, sum, 31);
     }
   }
   __syncthreads();
@@ -164,7 +175,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
   pdl_wait();
   if (blockIdx.x == 0 && tid == 0) a.valid[1] = 0;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * rows, last = min(first + rows, static_cast<int64_t>(a.V));
-  const int span = ((a.N + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int span = ((a.N + kSortWarps - 1) / kSortWarps + 127) / 128 * 128;
+  const bool aligned_ids = (reinterpret_cast<uintptr_t>(a.ids) & 15) == 0;
   const int64_t begin64 = static_cast<int64_t>(warp) * span;
   const int begin = static_cast<int>(min(begin64, static_cast<int64_t>(a.N)));
   const int end = static_cast<int>(min(begin64 + span, static_cast<int64_t>(a.N)));
@@ -173,33 +185,60 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
     for (int x = tid; x < (have + 31) / 32; x += kSortThreads) s.present[x] = 0;
     __syncthreads();
     int in = 0, below = 0;
-    // fn(i, id, whether it is of this slice) for this lane's ids, 32 of the warp at a time in order
-    auto walk = [&](auto fn) {
-      for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
-        ID id[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) id[u] = i0 + 32 * u + lane < end ? id_at<ID>(a, i0 + 32 * u + lane) : ID(-1);
+    // A lane takes four ids that follow one another, the warp 128 in order. fn(position of
+    // the lane's first match among those so far, i, their rows, which of the four match)
+    // where the warp has any; most slices have none of most 128.
+    auto walk = [&](bool count, auto fn) {
+      int seen = 0;
+      for (int i0 = begin; i0 < end; i0 += 128 * kBatch) {
+        ID id[kBatch][4];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const auto x = unsigned_id(id[u]);
-          using U = decltype(unsigned_id(id[u]));
-          fn(i0 + 32 * u + lane, x, x - static_cast<U>(lo) < static_cast<U>(have));
+          const int i = i0 + 128 * u + 4 * lane;
+          if (aligned_ids && i + 4 <= end) {
+            const Four<ID> four = *reinterpret_cast<const Four<ID>*>(static_cast<const ID*>(a.ids) + i);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) id[u][x] = four.id[x];
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) id[u][x] = i + x < end ? id_at<ID>(a, i + x) : ID(-1);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          unsigned match = 0;
+          int row[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const auto v = unsigned_id(id[u][x]);
+            using U = decltype(unsigned_id(id[u][x]));
+            if (count) below += v < static_cast<U>(lo);
+            const U r = v - static_cast<U>(lo);
+            row[x] = static_cast<int>(r);
+            match |= (r < static_cast<U>(have) ? 1u : 0u) << x;
+          }
+          if (!__any_sync(kFullMask, match)) continue;
+          const int mine = __popc(match);
+          const unsigned under = (1u << lane) - 1u, b0 = __ballot_sync(kFullMask, mine & 1),
+                         b1 = __ballot_sync(kFullMask, mine & 2), b2 = __ballot_sync(kFullMask, mine & 4);
+          fn(seen + __popc(b0 & under) + 2 * __popc(b1 & under) + 4 * __popc(b2 & under), i0 + 128 * u + 4 * lane, row, match);
+          seen += __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
         }
       }
+      return seen;
     };
-    walk([&](int i, auto id, bool mine) {
-      below += id < static_cast<decltype(id)>(lo);
-      const unsigned votes = __ballot_sync(kFullMask, mine);
-      if (votes == 0) return;
-      if (mine) {
-        const int row = static_cast<int>(id - lo), p = in + __popc(votes & ((1u << lane) - 1u));
-        atomicOr(&s.present[row >> 5], 1u << (row & 31));
+    in = walk(true, [&](int p, int i, const int (&row)[4], unsigned match) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (!(match >> x & 1)) continue;
+        const uint32_t bit = 1u << (row[x] & 31);
+        if (!(*static_cast<volatile uint32_t*>(&s.present[row[x] >> 5]) & bit)) atomicOr(&s.present[row[x] >> 5], bit);
         if (p < kKept) {
-          s.kept_row[warp][p] = row;
-          s.kept_token[warp][p] = i;
+          s.list[1][0][warp * kKept + p] = row[x];
+          s.list[1][1][warp * kKept + p] = i + x;
         }
+        ++p;
       }
-      in += __popc(votes);
     });
     below = __reduce_add_sync(kFullMask, below);
     if (lane == 0) {
@@ -214,15 +253,19 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
       base += s.warp_below[w];
     }
     if (tid == 0 && lo64 + have == a.V) a.valid[0] = base + n;
-    // the rounds of the radix sort go between the halves of keys and order, the last into the first half
+    // Many tokens are sorted in shared memory, too many between the halves of keys and order;
+    // the last round writes the first half.
     const int bits = have > 1 ? 32 - __clz(have - 1) : 0;
     const int rounds = n <= kCounted ? 0 : (bits + kDigitBits - 1) / kDigitBits;
     int32_t* key = a.keys + base;
     int32_t* token = a.order + base;
     if (n > 0) {
-      const bool counted = n <= kCounted;
-      int32_t* key_to = rounds & 1 ? key + a.N : key;
-      int32_t* token_to = rounds & 1 ? token + a.N : token;
+      const bool counted = n <= kCounted, listed = n <= kListed;
+      // keys and tokens before round r
+      auto keys_of = [&](int r) { return r == rounds ? key : listed ? s.list[r & 1][0] : key + ((rounds - r) & 1 ? a.N : 0); };
+      auto tokens_of = [&](int r) { return r == rounds ? token : listed ? s.list[r & 1][1] : token + ((rounds - r) & 1 ? a.N : 0); };
+      int32_t* key_to = keys_of(0);
+      int32_t* token_to = tokens_of(0);
       auto put = [&](int p, int row, int t) {
         if (counted) {
           s.key[p] = static_cast<uint32_t>(row) << 9 | p;
@@ -233,12 +276,12 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
         }
       };
       if (in <= kKept) {
-        for (int x = lane; x < in; x += 32) put(at + x, s.kept_row[warp][x], s.kept_token[warp][x]);
+        for (int x = lane; x < in; x += 32) put(at + x, s.list[1][0][warp * kKept + x], s.list[1][1][warp * kKept + x]);
       } else {
-        walk([&](int i, auto id, bool mine) {
-          const unsigned votes = __ballot_sync(kFullMask, mine);
-          if (mine) put(at + __popc(votes & ((1u << lane) - 1u)), static_cast<int>(id - lo), i);
-          at += __popc(votes);
+        walk(false, [&](int p, int i, const int (&row)[4], unsigned match) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (match >> x & 1) put(at + p++, row[x], i + x);
         });
       }
       if (counted)
@@ -255,10 +298,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embed_sort_kernel(const Embed
         token[p] = s.token[tid];
       }
       const int each = rounds ? (bits + rounds - 1) / rounds : 0;
-      for (int r = 0; r < rounds; ++r) {
-        const int64_t from = (rounds - r) & 1 ? a.N : 0, to = a.N - from;
-        radix_round(s, key + from, token + from, key + to, token + to, n, lo, r * each, min(each, bits - r * each));
-      }
+      for (int r = 0; r < rounds; ++r)
+        radix_round(s, keys_of(r), tokens_of(r), keys_of(r + 1), tokens_of(r + 1), n, lo, r * each, min(each, bits - r * each));
     }
     // zeros to the rows without a token: a warp a row
     V zero;
@@ -285,7 +326,7 @@ constexpr int kWhole = 32;
 // blockDim (lanes of an item, items): an item is a chunk of the sorted tokens
 // and as many columns as its lanes hold.
 template <typename T, int N>
-__global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int slices) {
+__global__ void __launch_bounds__(256, 4) embed_sum_kernel(const EmbedArgs a, int slices) {
   using V = Vec<T, N>;
   pdl_launch_dependents();
   pdl_wait();
@@ -374,19 +415,19 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const EmbedArgs a, int s
   write();
 }
 
-// A CTA takes a row that reaches over chunks and 32 * N of its columns; its warps
-// share the chunks out evenly and in order.
+// A CTA takes a row that reaches over chunks and `lanes` * N of its columns; its
+// groups of `lanes` threads share the chunks out evenly and in order.
 template <typename T, int N>
-__global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const EmbedArgs a) {
-  __shared__ Vec<float, N> sums[kJoinWarps][32];
+__global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(const EmbedArgs a, int lanes) {
+  __shared__ Vec<float, N> sums[kJoinThreads];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, group = threadIdx.x / lanes, groups = kJoinThreads / lanes;
   const int valid = a.valid[0], owners = a.valid[1];
-  const int blocks = (a.H + 32 * N - 1) / (32 * N);
+  const int blocks = (a.H + lanes * N - 1) / (lanes * N);
   for (int64_t item = blockIdx.x; item < static_cast<int64_t>(owners) * blocks; item += gridDim.x) {
     const int chunk = a.owners[item / blocks];
-    const int64_t c = item % blocks * (32 * N) + lane * N;
+    const int64_t c = (item % blocks * lanes + threadIdx.x % lanes) * N;
     const int row = a.keys[(chunk + 1ll) * a.chunk];
     // chunks that the row reaches into: a search among the chunks' first keys, 32 at a time
     int more = 1;
@@ -402,8 +443,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const Embed
         more = static_cast<int>(min(more + stride * n, left));
       }
     }
-    const int each = (more + kJoinWarps) / kJoinWarps;  // of more + 1 parts
-    const int from = warp * each, to = min(from + each, more + 1);
+    const int each = (more + groups) / groups;  // of more + 1 parts
+    const int from = group * each, to = min(from + each, more + 1);
     Vec<float, N> s = {};
     if (c < a.H)
 #pragma unroll 8
@@ -412,14 +453,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) embed_join_kernel(const Embed
 #pragma unroll
         for (int n = 0; n < N; ++n) s.v[n] += v.v[n];
       }
-    sums[warp][lane] = s;
+    sums[threadIdx.x] = s;
     __syncthreads();
-    if (warp == 0 && c < a.H) {
+    if (group == 0 && c < a.H) {
       float f[N];
 #pragma unroll
       for (int n = 0; n < N; ++n) f[n] = 0.f;
-      for (int w = 0; w * each <= more; ++w) {
-        const Vec<float, N> v = sums[w][lane];
+#pragma unroll 8
+      for (int w = 0; w < (more + each) / each; ++w) {  // the groups that have parts
+        const Vec<float, N> v = sums[w * lanes + threadIdx.x];
 #pragma unroll
         for (int n = 0; n < N; ++n) f[n] += v.v[n];
       }
@@ -487,7 +529,11 @@ int sum_run(const EmbedArgs& a, cudaStream_t st) {
   int rc = launch(embed_sum_kernel<T, N>, dim3(static_cast<unsigned>((items + per - 1) / per)), dim3(lanes, per), 0, st,
                   a, static_cast<int>(slices));
   if (rc != MTP_OK || chunks == 1) return rc;
-  return launch(a.H % 4 ? embed_join_kernel<T, 1> : embed_join_kernel<T, 4>, dim3(4 * kSms), dim3(kJoinWarps * 32), 0, st, a);
+  const int columns = a.H % 4 ? 1 : 4;
+  int join_lanes = 4;
+  while (join_lanes * columns < a.H && join_lanes < 32) join_lanes *= 2;
+  return launch(columns == 1 ? embed_join_kernel<T, 1> : embed_join_kernel<T, 4>, dim3(4 * kSms), dim3(kJoinThreads), 0, st, a,
+                join_lanes);
 }
 
 template <typename T>
