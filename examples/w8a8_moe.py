@@ -8,8 +8,9 @@ shared expert whose two projections are ``int8_linear``. The result is compared
 with the same layer on the unquantised weights.
 
 Training: the router and the experts of such a layer learn to imitate a teacher;
-the tokens go to their experts and back through ``sort_tokens`` and
-``unsort_tokens``, whose gradients reach the rows and the routing weights.
+the tokens go to their experts and back through ``route_tokens``, ``sort_tokens``
+and ``unsort_tokens``, whose gradients reach the logits, the rows and the routing
+weights.
 """
 from __future__ import annotations
 
@@ -88,10 +89,8 @@ def train(args, g) -> tuple[float, float]:
     losses = []
     for _ in range(args.steps):
         logits = x @ router.T
-        ids = logits.detach().topk(k, -1).indices
-        weights = torch.softmax(logits, -1).gather(1, ids)
-        weights = weights / weights.sum(-1, keepdim=True)
-        rows, positions, offsets, _ = mtp_b200.sort_tokens(x, ids.to(torch.int32), e)
+        weights, ids, *_ = mtp_b200.route_tokens(logits, k)
+        rows, positions, offsets, _ = mtp_b200.sort_tokens(x, ids, e)
         ends = offsets.tolist()
         y = torch.cat([rows[ends[n]:ends[n + 1]] @ experts[n].T for n in range(e)])
         loss = (mtp_b200.unsort_tokens(y, positions, weights) - target).square().mean()

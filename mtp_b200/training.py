@@ -20,7 +20,6 @@ depend on timing: equal inputs give equal bits.
 """
 from __future__ import annotations
 
-import math
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -29,6 +28,8 @@ import torch
 from . import _lib
 from .w8a8 import (DTYPES, MAX_EXTENT, _F32, _FLOATS, _current_device, _differentiated, _row_stride, _stream, _tensor,
                    _too_large)
+
+_MOST = torch.finfo(torch.float32).max
 
 _route_entry = _lib.Entry("mtp_route_tokens")
 _route_backward_entry = _lib.Entry("mtp_route_tokens_backward")
@@ -254,8 +255,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                 raise ValueError(f"{name} must have {h} entries, got {t.numel()}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    if not 0 <= eps < math.inf:
-        raise ValueError(f"eps must be a number from 0 on, got {eps}")
+    if not 0 <= eps <= _MOST:
+        raise ValueError(f"eps must be a number of fp32 from 0 on, got {eps}")
     if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, rows, weight, bias, eps)
     return _norm(x, rows, weight, bias, eps, False)[0]
@@ -320,8 +321,8 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> 
     for what, n in (("ids", ids.numel()), ("rows of table", v), ("columns", h)):
         if n > MAX_EXTENT:
             _too_large(what, n)
-    if not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise ValueError(f"scale must be a finite number, got {scale!r}")
+    if not isinstance(scale, (int, float)) or not abs(scale) <= _MOST:
+        raise ValueError(f"scale must be a finite number of fp32, got {scale!r}")
     if _differentiated(table):
         return _EmbedTokens.apply(ids, table, scale)
     return _embed(ids, table, scale)

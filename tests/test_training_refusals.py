@@ -258,3 +258,11 @@ class TestOnTheGpu:
         ids.add_(1)
         with pytest.raises(RuntimeError, match="modified"):
             out.sum().backward()
+
+    @pytest.mark.parametrize("value", [1e39, -1e39, 10 ** 400])
+    def test_numbers_that_fp32_does_not_hold(self, cuda_device, value):
+        x, ids = torch.zeros(4, 8, device=cuda_device), torch.zeros(3, dtype=I32, device=cuda_device)
+        with pytest.raises(ValueError, match="fp32"):
+            mtp_b200.embed_tokens(ids, x, value)
+        with pytest.raises(ValueError, match="fp32"):
+            mtp_b200.layer_norm(x, eps=abs(value))
