@@ -23,7 +23,7 @@ constexpr int kRowThreads = 1024;    // most threads of a row in norm_row_kernel
 constexpr int kGroupThreads = 512;   // of a CTA of the ring kernels: 128 registers each
 constexpr int kGroupWarps = kGroupThreads / 32;
 constexpr int kRing = 224 * 1024;    // bytes of rows in flight and parameters of such a CTA
-constexpr int kStages = 8;
+constexpr int kStages = 4;
 constexpr uint64_t kTimeoutNs = 2000000000ull;
 
 // The sums of two values over the CTA, for all threads.
@@ -256,21 +256,26 @@ __device__ __forceinline__ int rows_of(const NormArgs& a, const NormPlan& p, int
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return reinterpret_cast<float2&>(d);
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return reinterpret_cast<float2&>(d);
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return reinterpret_cast<float2&>(d);
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
@@ -763,11 +768,12 @@ bool make_plan(const NormArgs& a, int e, int together, bool backward, NormPlan& 
   p.groups = std::min(kGroupThreads / p.lanes, p.lanes == 32 ? kGroupWarps : 15);  // a named barrier each
   p.columns = static_cast<uint32_t>(p.lanes * e);  // the threads' columns, those past H too
   const int64_t kept = 4ll * p.columns * (backward ? 1 : 2);
-  // blocks of about 2 KB and at least `together` rows, fewer where that leaves groups without one
-  p.batch = static_cast<int>(std::max<int64_t>(std::min<int64_t>(std::max<int64_t>(2048 / row, together), a.M / (kSms * p.groups)), 1));
   p.row_pitch = a.stride == a.H || a.M == 1 ? 0 : static_cast<uint32_t>(round_up(row + 15, 16));
+  // blocks of about 2 KB and at least `together` rows, fewer where that leaves groups without one
+  const int64_t in_ring = p.row_pitch ? p.row_pitch : row;
+  p.batch = static_cast<int>(std::max<int64_t>(std::min<int64_t>(std::max<int64_t>(2048 / in_ring, together), a.M / (kSms * p.groups)), 1));
   // a lead of up to 15 bytes, and the last unit to its end
-  p.stage_bytes = static_cast<uint32_t>(round_up(p.row_pitch ? p.batch * static_cast<int64_t>(p.row_pitch) : p.batch * row + (N * sizeof(T) == 16 ? 0 : 30), 128));
+  p.stage_bytes = static_cast<uint32_t>(round_up(p.batch * in_ring + (p.row_pitch || N * sizeof(T) == 16 ? 0 : 30), 128));
   p.stages = static_cast<int>(std::min<int64_t>((kRing - kept) / p.groups / (static_cast<int64_t>(parts) * p.stage_bytes), kStages));
   if (p.stages < 2) return false;
   p.ring_bytes = static_cast<uint32_t>(p.stage_bytes * p.stages * p.groups * parts);
@@ -800,7 +806,8 @@ int forward_run(const NormArgs& a, cudaStream_t st) {
   const int64_t vectors = (static_cast<int64_t>(a.H) + N - 1) / N;
   NormPlan p;
   if (a.M > 2 * kSms) {
-    const int e = a.H > (N == 1 ? 512 : 16 * kGroupThreads) ? 32 : a.H > 256 ? 16 : 8;
+    // columns of a thread: few where rows are narrow, and of fp32, whose rows are twice as long
+    const int e = a.H > (N == 1 ? 512 : 16 * kGroupThreads) ? 32 : a.H > (sizeof(T) == 4 ? 8 * kGroupThreads : 256) ? 16 : 8;
     if (make_plan<T, N>(a, e, 2, false, p) && p.batch > 1)
       return e == 32 ? forward_ring<T, N, 32, 2>(a, p, st) : e == 16 ? forward_ring<T, N, 16, 2>(a, p, st) : forward_ring<T, N, 8, 2>(a, p, st);
     if (make_plan<T, N>(a, e, 1, false, p))
@@ -818,7 +825,7 @@ int forward_run(const NormArgs& a, cudaStream_t st) {
 template <typename T, int N>
 bool backward_run(const NormArgs& a, cudaStream_t st, int& rc, int& parts) {
   NormPlan p;
-  const int e = a.H <= 256 ? 8 : a.H <= 16 * kGroupThreads ? 16 : 32;
+  const int e = a.H <= 8 * kGroupThreads ? 8 : a.H <= 16 * kGroupThreads ? 16 : 32;
   if (!make_plan<T, N>(a, e, 1, true, p)) return false;
   parts = p.ctas;
   rc = e == 8 ? backward_ring<T, N, 8>(a, p, st) : e == 16 ? backward_ring<T, N, 16>(a, p, st) : backward_ring<T, N, 32>(a, p, st);

@@ -223,3 +223,17 @@ def test_same_bits_again(cuda_device):
     for _ in range(3):
         for p, q in zip(torch.autograd.grad(mtp_b200.layer_norm(*leaves), leaves, g), first):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,h,wide", [(6000, 1, 3), (5000, 8, 24), (4000, 24, 25), (3000, 40, 64), (700, 5000, 5001), (500, 8200, 8208)])
+def test_many_rows_of_a_wider_tensor(cuda_device, dtype, m, h, wide):
+    x, _, _ = inputs(m, wide, dtype, F32)
+    _, w, b = inputs(1, h, dtype, F32)
+    check(x[:, wide - h:], w, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF, F32])
+@pytest.mark.parametrize("m,h", [(400, 16384), (400, 9000), (310, 12345), (400, 8193), (303, 4097), (1000, 1026), (2500, 129)])
+def test_many_wide_rows(cuda_device, dtype, m, h):
+    check(*inputs(m, h, dtype, F32))
