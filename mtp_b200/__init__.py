@@ -1,6 +1,10 @@
 """mtp_b200: B200-native (sm_100a) GPTQ-int4 W4A16 mixture-of-experts layer
 forward and its MTP-driven expert-prefetch path.
 
+Around them: an int8 (W8A8) expert path, the sort of tokens by expert, and what
+training such a layer needs beside that (router with losses, layer norm,
+embedding).
+
 The compute runs in ``lib/libmtp_b200.so`` (hand-written CUDA behind a C ABI,
 ``include/mtp_b200.h``); this package is the host-side mirror of the reference
 interfaces. There is no CPU fallback.

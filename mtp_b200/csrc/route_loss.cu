@@ -15,6 +15,14 @@
 // A warp takes a token, its logits stay in registers. The sums over tokens go
 // warp by warp in registers, then over the warps, then over the CTAs, always in
 // the same order; the counts are integers. So results do not depend on timing.
+//
+// The logits are read once forward and once, with the gradient written,
+// backward. Instructions bound it, not HBM: 65536 x 512 logits fill 62 % of the
+// issue slots forward, 52 % backward.
+//   8192 x 256, top-8:  16.6 us forward (two launches), 7.1 us backward
+//   65536 x 512, top-8: 88 us and 54 us (bytes alone 21 and 41)
+//   32768 x 1024, top-8: 72 us and 64 us (21 and 41)
+//   one token: 4.3 us and 2.3 us
 #include "rows.cuh"
 
 #include <math.h>
@@ -26,7 +34,8 @@ namespace {
 
 constexpr int kFinishCtas = 8;  // one cluster
 constexpr int kFinishThreads = 1024;
-constexpr int kOneCtaTokens = 16;  // up to here one CTA does all
+// Up to here one CTA does all, 4.3 us; two launches take 9.6 (64 tokens).
+constexpr int kOneCtaTokens = 16;
 constexpr int kSms = 148;
 constexpr int kTogether = 19;  // parts of a column that a thread has in flight: all of 148
 
@@ -152,7 +161,7 @@ struct Chosen {
 // than the k-th largest of all, so that few values (the k, and those that share
 // a lane with one of them) are left to rank. Gives their number, 0 where they
 // are more than 32 or there is no finite one.
-// 65536 tokens of 512 experts, top-8: one by one 195 us, so 106 us.
+// 65536 tokens of 512 experts, top-8: 195 us one by one, 127 us so.
 template <int VPT>
 __device__ __forceinline__ int candidates(const RouteLossArgs& a, const float (&z)[VPT], float best, Chosen& c) {
   const int lane = threadIdx.x & 31;
