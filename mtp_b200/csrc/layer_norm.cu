@@ -7,16 +7,16 @@
 //           dx = rstd (wg - mean(wg) - xhat mean(wg xhat)),
 //           dw = sum over the rows of g xhat, db = sum of g.
 //
-// All sums in fp32 in a fixed order; results are rounded once. The 1 / sqrt is
-// rsqrtf, within 2 units in the last place.
+// All sums in fp32 in a fixed order; results are rounded once. In the ring
+// 1 / sqrt is rsqrtf, within 2 units in the last place.
 //
 // The bytes are x in and y out; for the gradients x and grad in and dx out. What
 // keeps the kernels from HBM's rate is the work per row between its two sums
 // (16384 x 8192 bf16: 14 and 24 instructions a value, one barrier a row):
-//   8192 x 2048 bf16:  21 us forward, 36 backward (bytes alone 10 and 15)
-//   16384 x 8192 bf16: 113 us and 181 us (82 and 123: 4.8 and 4.5 TB/s)
-//   16384 x 4096 fp32: 94 us and 127 us (82 and 123: 5.7 and 6.4 TB/s)
-//   one row of 2048: 2.2 us, 6.1 us
+//   8192 x 2048 bf16:  22 us forward, 37 backward (bytes alone 10 and 15)
+//   16384 x 8192 bf16: 111 us and 181 us (82 and 123: 4.8 and 4.5 TB/s)
+//   16384 x 4096 fp32: 95 us and 127 us (82 and 123: 5.6 and 6.3 TB/s)
+//   one row of 2048: 2.3 us, 6.1 us
 // Taken one after the other, 16384 x 8192 bf16 there and back: rows read three
 // times and columns by a kernel of their own 197 + 681 us; one pass, rows in
 // registers 176 + 463; a ring of bulk copies with one value a load 188 + 307, with
@@ -295,6 +295,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// s / n with n's reciprocal at hand: one correction makes a quotient that is a
+// number of fp32 exact, so that constant rows have no variance.
+__device__ __forceinline__ float quotient(float s, float n, float inv) {
+  const float q = s * inv;
+  return fmaf(fmaf(-q, n, s), inv, q);
+}
+
 // The sums of two values over the warp at once, the first in the lower half of
 // the lanes, the second in the upper.
 __device__ __forceinline__ float half_sums(float p, float q) {
@@ -449,7 +456,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
       const float my_sum = R == 2 ? half_sums(sum[0], sum[R - 1]) : warp_sum(sum[0]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        centre[r] = (R == 2 ? __shfl_sync(kFullMask, my_sum, 16 * r) : my_sum) * inv_columns;
+        centre[r] = quotient(R == 2 ? __shfl_sync(kFullMask, my_sum, 16 * r) : my_sum, columns, inv_columns);
         if (mine < E) cols.fill(v[r], centre[r]);  // no square
         float2 s = {0.f, 0.f};
 #pragma unroll
@@ -462,7 +469,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
         squares[r] = s.x + s.y;
       }
       float my_squares = R == 2 ? half_sums(squares[0], squares[R - 1]) : warp_sum(squares[0]);
-      float my_mean = my_sum * inv_columns;
+      float my_mean = quotient(my_sum, a.H, inv);
       if (warps > 1) {
         if ((lane & 15) == 0 && half == lane >> 4) {
           red[parity][half][0][warp] = my_sum;
@@ -475,9 +482,9 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
         my_mean = s;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) my_mean += __shfl_xor_sync(kFullMask, my_mean, o);
-        my_mean *= inv;
+        my_mean = quotient(my_mean, a.H, inv);
         // squares around the row's mean: those around a warp's, and its distance
-        const float d = s * inv_others - my_mean;
+        const float d = quotient(s, others, inv_others) - my_mean;
         my_squares = fmaf(others * d, d, my_squares);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) my_squares += __shfl_xor_sync(kFullMask, my_squares, o);
@@ -490,14 +497,14 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
         if (g.at == 0 && ahead < plan.blocks) issue(ahead, g.s);
         g.advance(plan);
       }
-      const float my_rstd = rsqrtf(fmaf(my_squares, inv, a.eps)) + g.poison, my_shift = -my_mean * my_rstd;
+      const float my_rstd = rsqrtf(fmaf(my_squares, inv, a.eps)) + g.poison;
       if (a.stats && (g.at & ~16) == 0 && half == g.at >> 4 && r0 + half < rows)
         *reinterpret_cast<float2*>(a.stats + 2 * (t0 + r0 + half)) = make_float2(my_mean, my_rstd);
-      float rstd[R], shift[R];
+      float rstd[R], mean[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         rstd[r] = R == 2 ? __shfl_sync(kFullMask, my_rstd, 16 * r) : my_rstd;
-        shift[r] = R == 2 ? __shfl_sync(kFullMask, my_shift, 16 * r) : my_shift;
+        mean[r] = R == 2 ? __shfl_sync(kFullMask, my_mean, 16 * r) : my_mean;
       }
       T* out = static_cast<T*>(a.y) + (t0 + r0) * a.H;
 #pragma unroll
@@ -510,7 +517,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
         for (int r = 0; r < R; ++r) {
 #pragma unroll
           for (int e = 0; e < C::kPairs; ++e)
-            v[r][i][e] = fma2(fma2(v[r][i][e], both(rstd[r]), both(shift[r])), w[kKeep ? i : 0][e], b[kKeep ? i : 0][e]);
+            v[r][i][e] = fma2(mul2(add2(v[r][i][e], both(-mean[r])), both(rstd[r])), w[kKeep ? i : 0][e], b[kKeep ? i : 0][e]);
           if (r0 + r < rows) cols.write(out + r * static_cast<int64_t>(a.H), i, v[r][i]);
         }
       }
@@ -569,7 +576,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_backward_kernel(const N
     const int64_t t0 = static_cast<int64_t>(block) * plan.batch;
     const uint8_t* stage = g.ring + static_cast<size_t>(g.s) * 2 * plan.stage_bytes;
     for (int r = 0; r < rows; ++r) {
-      const float rstd = st.y + g.poison, shift = -st.x * rstd;
+      const float rstd = st.y + g.poison, mean = st.x;
       const int64_t next = r + 1 < rows ? t0 + r + 1 : static_cast<int64_t>(block + g.step) * plan.batch;
       if (next < a.M) st = stat(next);
       const uint8_t* xs = stage + x.offset(t0, r);
@@ -580,7 +587,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_backward_kernel(const N
         cols.read(gs, i, gr);
         if (!kKeep) cols.kept(weight, i, w[0]);
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) xh[e] = fma2(xh[e], both(rstd), both(shift));
+        for (int e = 0; e < kPairs; ++e) xh[e] = mul2(add2(xh[e], both(-mean)), both(rstd));
       };
       float2 s1 = {0.f, 0.f}, s2 = {0.f, 0.f};
 #pragma unroll

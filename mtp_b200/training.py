@@ -15,8 +15,9 @@ errors raise ``ValueError`` before any launch; a non-zero C status raises
 :class:`mtp_b200.MtpError`. Every call is asynchronous on the current torch
 stream of its tensors' GPU, which need not be the current one. There is no CPU
 path. Gradients are first derivatives, backward; forward mode raises
-``RuntimeError``. All sums are in fp32 or more and in an order that does not
-depend on timing: equal inputs give equal bits.
+``RuntimeError``. All sums are in fp32 or more and in an order that sizes and
+memory layout fix, not timing: the same call gives the same bits. (Should a
+bounded wait of a layer norm kernel run out, the rows that it was for are NaN.)
 """
 from __future__ import annotations
 

@@ -166,3 +166,46 @@ def test_same_bits_again(cuda_device, n, v):
     first = run()
     for _ in range(3):
         assert torch.equal(run(), first)
+
+
+def test_more_rows_than_a_slice_holds(cuda_device):
+    """A table so long that a CTA takes its rows in two turns."""
+    table, g = table_of(19_500_003, 1, F32)
+    ids = torch.randint(0, 19_500_003, (3000,), generator=g, device="cuda", dtype=I32)
+    ids[:600] = torch.arange(131_000, 131_600, device="cuda")  # over the turns' border
+    ids[600:1300] = 131_100
+    ids[1300] = 19_500_002
+    check(ids, table, 0.5)
+
+
+@pytest.mark.parametrize("n,v,h", [(1_300_000, 1000, 8), (600_000, 70, 40), (1_300_000, 300_000, 2)])
+def test_very_many_tokens(cuda_device, n, v, h):
+    table, g = table_of(v, h, F32)
+    check(torch.randint(0, v, (n,), generator=g, device="cuda", dtype=I32), table)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("kind", [I32, I64])
+def test_ids_off_16_bytes(cuda_device, kind, offset):
+    table, g = table_of(500, 32, F32)
+    ids = torch.randint(-3, 503, (2000 + offset,), generator=g, device="cuda", dtype=kind)[offset:]
+    check(ids, table)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 values in the table, in the rows and in the gradient."""
+    import mtp_b200
+    v = n = 1_050_000
+    h = 2048
+    table = torch.zeros(v, h, dtype=BF, device="cuda")
+    table[-500:] = torch.randn(500, h, device="cuda").to(BF)
+    ids = torch.zeros(n, dtype=I32, device="cuda")
+    ids[-400:] = torch.arange(v - 400, v, device="cuda", dtype=I32)
+    table.requires_grad_()
+    out = mtp_b200.embed_tokens(ids, table)
+    assert torch.equal(out[-400:].detach(), table[-400:].detach()) and not out[:-400].any()
+    grad = torch.zeros_like(out)
+    grad[-400:] = torch.randn(400, h, device="cuda").to(BF)
+    grad[5] = 1
+    (got,) = torch.autograd.grad(out, table, grad)
+    assert torch.equal(got[-400:], grad[-400:]) and (got[0] == 1).all() and not got[1:-400].any()

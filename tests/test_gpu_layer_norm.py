@@ -237,3 +237,72 @@ def test_many_rows_of_a_wider_tensor(cuda_device, dtype, m, h, wide):
 @pytest.mark.parametrize("m,h", [(400, 16384), (400, 9000), (310, 12345), (400, 8193), (303, 4097), (1000, 1026), (2500, 129)])
 def test_many_wide_rows(cuda_device, dtype, m, h):
     check(*inputs(m, h, dtype, F32))
+
+
+MANY = 500  # rows that go through the ring
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("h", [32, 96, 600, 2048, 3001, 9000])
+def test_many_constant_rows(cuda_device, dtype, h):
+    import mtp_b200
+    x, w, b = inputs(MANY, h, dtype, F32)
+    x[1::3], x[2::3] = 2.0, 0.0
+    y = mtp_b200.layer_norm(x, w, b)
+    want = b.to(dtype)
+    # the sum of h twos is a number of fp32, and so is its quotient by h
+    assert torch.equal(y[1::3], want.expand_as(y[1::3])) and torch.equal(y[2::3], want.expand_as(y[2::3]))
+    check(x, w, b)
+    with torch.no_grad():
+        assert torch.isnan(mtp_b200.layer_norm(x, w, b, 0.0)[1::3]).all()  # 0 / 0, as the formula has it
+
+
+@pytest.mark.parametrize("h", [64, 1024, 2048, 3000, 10000])
+def test_offsets_of_many_rows_cost_no_digits(cuda_device, h):
+    import mtp_b200
+    x = (4096 + torch.arange(h, device="cuda") % 2).float()[None].repeat(MANY, 1)
+    y = mtp_b200.layer_norm(x, eps=0.0)
+    d = (h / 32 + 40) * U * 4096.5
+    assert ((y.abs() - 1).abs() <= 4 * d + 16 * U).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("h", [48, 2048, 1001])
+def test_bad_values_stay_in_their_row_of_many(cuda_device, bad, h):
+    import mtp_b200
+    x, w, b = inputs(MANY, h, F32, F32)
+    clean = mtp_b200.layer_norm(x, w, b)
+    x[77, 7] = bad
+    x[401] = bad
+    keep = torch.ones(MANY, dtype=torch.bool, device="cuda")
+    keep[[77, 401]] = False
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = mtp_b200.layer_norm(*leaves)
+    assert torch.isnan(y[~keep]).all() and torch.equal(y[keep], clean[keep])
+    dx, dw, db = torch.autograd.grad(y, leaves, torch.ones_like(x))
+    assert torch.isnan(dx[~keep]).all() and torch.isfinite(dx[keep]).all()
+    assert torch.isnan(dw).all() and torch.isfinite(db).all()
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 values: the last rows are as in a call of their own."""
+    import mtp_b200
+    m, h = 1_050_000, 2048
+    x = torch.zeros(m, h, dtype=BF, device="cuda")
+    tail, w, b = inputs(600, h, BF, F32)
+    x[-600:] = tail
+    g = torch.zeros_like(x)
+    g[-600:] = torch.randn(600, h, device="cuda").to(BF)
+    results = []
+    for rows, grad in ((x, g), (tail, g[-600:].clone())):
+        leaves = [t.detach().requires_grad_() for t in (rows, w, b)]
+        y = mtp_b200.layer_norm(*leaves)
+        dx, dw, db = torch.autograd.grad(y, leaves, grad)
+        results.append((y[-600:].detach().clone(), dx[-600:].clone(), dw, db))
+        assert rows is tail or (torch.equal(y[0], b.to(BF)) and not dx[:-600].any())
+        del y, dx
+    for i in (0, 1):
+        assert torch.equal(results[0][i], results[1][i])
+    for i in (2, 3):  # 600 terms in another order
+        size = g[-600:].abs().double().sum(0) * 8
+        assert ((results[0][i].double() - results[1][i].double()).abs() <= 600 * U * size + 1e-6).all()

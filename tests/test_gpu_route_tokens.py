@@ -246,3 +246,24 @@ def test_same_bits_again(cuda_device):
     for _ in range(3):
         for x, y in zip(results(), first):
             assert torch.equal(x, y)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 logits: the last tokens are as in a call of their own."""
+    import mtp_b200
+    m, e = 2_150_000, 1000
+    z = torch.zeros(m, e, dtype=BF, device="cuda")
+    tail, _ = logits(300, e, BF)
+    z[-300:] = tail
+    mask = torch.zeros(m, dtype=torch.bool, device="cuda")
+    mask[-300:] = True
+    results = []
+    for rows, counted in ((z, mask), (tail, None)):
+        rows.requires_grad_()
+        r = mtp_b200.route_tokens(rows, 6, token_mask=counted)
+        (grad,) = torch.autograd.grad(r.weights.square().sum() + r.balance_loss + r.z_loss, rows)
+        results.append((r.weights[-300:], r.ids[-300:], r.counts, grad[-300:].clone()))
+        assert rows is tail or not grad[:-300].any()
+        del grad
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert torch.equal(results[0][2], results[1][2]) and torch.equal(results[0][3], results[1][3])
