@@ -31,6 +31,7 @@ from .w8a8 import (DTYPES, MAX_EXTENT, _F32, _FLOATS, _current_device, _differen
                    _too_large)
 
 _MOST = torch.finfo(torch.float32).max
+_PARAMS = {t: _F32 if t == torch.float32 else (t, torch.float32) for t in _FLOATS}  # types of a layer norm's parameters
 
 _route_entry = _lib.Entry("mtp_route_tokens")
 _route_backward_entry = _lib.Entry("mtp_route_tokens_backward")
@@ -49,6 +50,17 @@ def _workspace(name: str, *shape) -> int:
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _like(x):
+    """A contiguous tensor as x; empty_like is the cheapest of torch's calls, and keeps the strides of a slice's rows."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+def _is_row(t, index, dtypes, n) -> bool:
+    """What _tensor and a check of the size ask of a contiguous t [n], in the order of a call that is right."""
+    return (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype in dtypes and t.ndim == 1
+            and t.shape[0] == n and t.is_contiguous())
 
 
 def _first_derivative(backward):
@@ -184,7 +196,7 @@ def _norm(x, rows, weight, bias, eps, need_stats):
         with torch.cuda.device(device):
             return _norm(x, rows, weight, bias, eps, need_stats)
     (m, stride), h = rows, x.shape[-1]
-    y = x.new_empty(x.shape)
+    y = _like(x)
     stats = x.new_empty(m, 2, dtype=torch.float32) if need_stats else None
     param = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
     _norm_entry(x.data_ptr(), stride, DTYPES[x.dtype], m, h, _ptr(weight), _ptr(bias), DTYPES[param], eps,
@@ -198,8 +210,8 @@ def _norm_backward(grad, x, rows, weight, stats, param, need_x, need_weight, nee
         with torch.cuda.device(device):
             return _norm_backward(grad, x, rows, weight, stats, param, need_x, need_weight, need_bias)
     (m, stride), h = rows, x.shape[-1]
-    grad_x = x.new_empty(x.shape) if need_x else None
-    grad_weight = x.new_empty(h, dtype=param) if need_weight else None
+    grad_x = _like(x) if need_x else None
+    grad_weight = torch.empty_like(weight) if need_weight else None
     grad_bias = x.new_empty(h, dtype=param) if need_bias else None
     size = _workspace("mtp_layer_norm_backward_workspace_size", m, h) if need_weight or need_bias else 0
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
@@ -248,12 +260,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if x.numel() // h > MAX_EXTENT:
         _too_large("rows", x.numel() // h)
     rows = _rows_of(x)
-    types = _FLOATS if x.dtype == torch.float32 else (x.dtype, torch.float32)
+    types, index = _PARAMS[x.dtype], x.get_device()
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _tensor(name, t, 1, types if types is not _FLOATS else _F32, x.device)
-            if t.numel() != h:
-                raise ValueError(f"{name} must have {h} entries, got {t.numel()}")
+        if t is not None and not _is_row(t, index, types, h):
+            _tensor(name, t, 1, types, x.device)
+            raise ValueError(f"{name} must have {h} entries, got {t.numel()}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     if not 0 <= eps <= _MOST:

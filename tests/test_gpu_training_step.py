@@ -174,3 +174,40 @@ def test_gradients_add_up_over_two_calls(cuda_device):
     first = block.table.grad.clone()
     mtp_b200.embed_tokens(block.ids, block.table).sum().backward()
     assert torch.equal(block.table.grad, 2 * first)
+
+
+def test_backward_into_grads_captured(cuda_device):
+    """loss.backward() in a graph, with no eager graph of the same leaves alive: the gradients it leaves in .grad."""
+    import gc
+    want = Block(seed=5, m=400).grads()
+    block = Block(seed=5, m=400)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block.loss().backward()  # loads the kernels
+    torch.cuda.current_stream().wait_stream(side)
+    for t in block.leaves:
+        t.grad = None
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = block.loss()
+        loss.backward()
+    for t in block.leaves:
+        t.grad.fill_(float("nan"))
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip((loss.detach(), *(t.grad for t in block.leaves)), want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_calls_of_other_sizes_between(cuda_device, order):
+    """Nothing of one call is left for the next: a small step between two large ones, and the other way round."""
+    sizes = [(3000, 5000), (7, 20)] if order else [(7, 20), (3000, 5000)]
+    blocks = [Block(m=m, v=v, seed=m) for m, v in sizes]
+    first = [b.grads() for b in blocks]
+    for _ in range(2):
+        for b, w in zip(blocks, first):
+            for x, y in zip(b.grads(), w):
+                assert torch.equal(x, y)
