@@ -27,8 +27,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .w8a8 import (DTYPES, MAX_EXTENT, _F32, _FLOATS, _current_device, _differentiated, _row_stride, _stream, _tensor,
-                   _too_large)
+from .w8a8 import (DTYPES, MAX_EXTENT, _F32, _FLOATS, _current_device, _differentiated, _given_back, _row_stride, _stream,
+                   _tensor, _too_large)
 
 _MOST = torch.finfo(torch.float32).max
 _PARAMS = {t: _F32 if t == torch.float32 else (t, torch.float32) for t in _FLOATS}  # types of a layer norm's parameters
@@ -131,7 +131,8 @@ class _RouteTokens(torch.autograd.Function):
         # ids and counts are not differentiable: they go around autograd, in `rest`
         weights, ids, counts, balance, z, pull = _route(logits, stride, top_k, renormalize, token_mask, True)
         ctx.save_for_backward(logits, ids, pull, token_mask)
-        ctx.stride, ctx.top_k, ctx.renormalize = stride, top_k, renormalize
+        ctx.saved = logits.shape, logits.dtype, logits.device
+        ctx.top_k, ctx.renormalize = top_k, renormalize
         ctx.set_materialize_grads(False)
         rest.extend((ids, counts))
         return weights, balance, z
@@ -139,10 +140,17 @@ class _RouteTokens(torch.autograd.Function):
     @_first_derivative
     def backward(ctx, grad_weights, grad_balance, grad_z):
         logits, ids, pull, token_mask = ctx.saved_tensors
+        shape, dtype, device = ctx.saved
+        (m, e), k = shape, ctx.top_k
+        logits = _given_back("router_logits", logits, shape, dtype, device, rows=True)
+        ids = _given_back("ids", ids, (m, k), torch.int32, device)
+        pull = _given_back("counts' terms", pull, (e + 1,), torch.float32, device)
+        if token_mask is not None:
+            token_mask = _given_back("token_mask", token_mask, (m,), torch.bool, device)
         if grad_weights is not None:
             grad_weights = grad_weights.contiguous()
-        return (_route_backward(logits, ctx.stride, ctx.top_k, ctx.renormalize, token_mask, ids, pull, grad_weights,
-                                grad_balance, grad_z), None, None, None, None, None)
+        return (_route_backward(logits, _row_stride("router_logits", logits), k, ctx.renormalize, token_mask, ids, pull,
+                                grad_weights, grad_balance, grad_z), None, None, None, None, None)
 
 
 def route_tokens(router_logits: torch.Tensor, top_k: int, renormalize: bool = True, *,
@@ -226,7 +234,6 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, rows, weight, bias, eps):
         y, stats = _norm(x, rows, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.rows = rows
         ctx.param = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
         return y
 
@@ -234,7 +241,13 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, stats = ctx.saved_tensors
         need_x, _, need_weight, need_bias, _ = ctx.needs_input_grad
-        grad_x, grad_weight, grad_bias = _norm_backward(grad.contiguous(), x, ctx.rows, weight, stats, ctx.param, need_x,
+        device, h = grad.device, grad.shape[-1]
+        x = _given_back("x", x, grad.shape, grad.dtype, device, rows=True)
+        rows = _rows_of(x)
+        stats = _given_back("rows' statistics", stats, (rows[0], 2), torch.float32, device)
+        if weight is not None:
+            weight = _given_back("weight", weight, (h,), ctx.param, device)
+        grad_x, grad_weight, grad_bias = _norm_backward(grad.contiguous(), x, rows, weight, stats, ctx.param, need_x,
                                                         need_weight, need_bias)
         return grad_x, None, grad_weight, grad_bias, None
 
@@ -307,12 +320,13 @@ class _EmbedTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale):
         ctx.save_for_backward(ids)
-        ctx.v, ctx.scale = table.shape[0], scale
+        ctx.v, ctx.scale, ctx.id_type = table.shape[0], scale, ids.dtype
         return _embed(ids, table, scale)
 
     @_first_derivative
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
+        ids = _given_back("ids", ids, grad.shape[:-1], ctx.id_type, grad.device)
         return None, _embed_backward(ids, grad.contiguous(), ctx.v, ctx.scale), None
 
 

@@ -124,6 +124,18 @@ def _row_stride(name: str, t: torch.Tensor) -> int:
     return t.stride(0)
 
 
+def _given_back(name: str, t: torch.Tensor, shape, dtype, device: torch.device, rows: bool = False) -> torch.Tensor:
+    """A saved tensor in the backward pass. Saved-tensor hooks (offloading, recomputation, compression) put another one
+    in its place, in any memory order: it is made contiguous unless ``rows`` of it may be a slice of wider ones. One that
+    has not the saved one's shape, type and device is an error, since a kernel would read past its end."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise RuntimeError(f"the saved {name} was {dtype} {tuple(shape)} on {device}; a saved-tensor hook gave back "
+                           f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.is_contiguous() or (rows and t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
 # ---------------------------------------------------------------------------
 # sort and unsort
 # ---------------------------------------------------------------------------
