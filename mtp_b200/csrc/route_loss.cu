@@ -69,22 +69,25 @@ __device__ __forceinline__ float row_max(const float (&v)[VPT]) {
   return warp_max(mx);
 }
 
+// exp(v) by one instruction, for v = z - max of a row. Subtracted before it is
+// scaled: max log2(e) rounded by itself is a factor that the row's values share,
+// but from |max| of 2e9 on one that no number of fp32 holds. v is 0 at the
+// maximum. The argument is rounded twice, an error of |v| 2^-23 of the result.
+__device__ __forceinline__ float fast_exp(float v) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * 1.44269504f));
+  return e;
+}
+
 // v -> exp(v - max) (0 past the last expert); returns max and sum. The forward
 // pass has the exponential of mtp_router_topk, so that both give the same bits.
-// FAST: by one instruction; its argument (v - max) log2(e) is rounded once, an
-// error of |v - max| 2^-24 of the result, and what max log2(e) loses all
-// values of the row share.
+// FAST: fast_exp.
 template <bool FULL, bool FAST, int VPT>
 __device__ __forceinline__ float2 softmax_row(const RouteLossArgs& a, int lane, float (&v)[VPT], float mx) {
   float s = 0.f;
-  const float shift = -mx * 1.44269504f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    float e;
-    if (FAST)
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(v[i], 1.44269504f, shift)));
-    else
-      e = expf(v[i] - mx);
+    const float e = FAST ? fast_exp(v[i] - mx) : expf(v[i] - mx);
     v[i] = has<FULL>(a, lane, i) ? e : 0.f;
     s += v[i];
   }
@@ -440,8 +443,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteLossArgs
     }
     float direct = 0.f, pj = 0.f;
     if (a.grad_weights) {
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(pj) : "f"(fmaf(zj, 1.44269504f, -ms.x * 1.44269504f)));
-      pj = id >= 0 ? pj * inv : 0.f;
+      pj = id >= 0 ? fast_exp(zj - ms.x) * inv : 0.f;
       if (a.renorm) {
         const float w = pj / fmaxf(warp_sum(pj), 1e-20f);
         const float wg = id >= 0 ? w * g : 0.f;
