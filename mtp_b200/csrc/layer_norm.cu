@@ -227,7 +227,10 @@ struct Walk {
   uint8_t* ring;
   int group, at, first, step, s;
   uint32_t phase;
-  float poison;  // NaN once a wait ran out: the results from there on say so
+  // NaN once a wait of this thread ran out. It joins the thread's part of a row's sums, so that all of the row is NaN
+  // whichever thread it was, and the rows behind it. The thread that issues copies then issues no more: a barrier whose
+  // phase may not be over takes no arrival, and what the others wait for runs out too.
+  float poison;
 
   __device__ __forceinline__ uint32_t bar(int q) const { return smem_u32(&full[group][q]); }
   __device__ __forceinline__ void begin(const NormPlan& p, uint64_t (*bars)[kStages], uint8_t* smem, int parts) {
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
         for (int i = 0; i < C::kVectors; ++i)
 #pragma unroll
           for (int e = 0; e < C::kPairs; ++e) s = add2(s, v[r][i][e]);
-        sum[r] = s.x + s.y;
+        sum[r] = s.x + s.y + g.poison;
       }
       // this lane's row (half): the warp's sum
       const float my_sum = R == 2 ? half_sums(sum[0], sum[R - 1]) : warp_sum(sum[0]);
@@ -494,10 +497,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_ring_kernel(const NormA
       }
       if (r0 + R >= rows) {  // every thread has its values of the last row
         const int ahead = block + plan.stages * g.step;
-        if (g.at == 0 && ahead < plan.blocks) issue(ahead, g.s);
+        if (g.at == 0 && ahead < plan.blocks && g.poison == 0.f) issue(ahead, g.s);
         g.advance(plan);
       }
-      const float my_rstd = rsqrtf(fmaf(my_squares, inv, a.eps)) + g.poison;
+      const float my_rstd = rsqrtf(fmaf(my_squares, inv, a.eps));
       if (a.stats && (g.at & ~16) == 0 && half == g.at >> 4 && r0 + half < rows)
         *reinterpret_cast<float2*>(a.stats + 2 * (t0 + r0 + half)) = make_float2(my_mean, my_rstd);
       float rstd[R], mean[R];
@@ -616,7 +619,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) norm_backward_kernel(const N
       const float m1 = __shfl_sync(kFullMask, p, 0) * inv, m2 = __shfl_sync(kFullMask, p, 16) * inv;
       auto refill = [&] {
         const int ahead = block + plan.stages * g.step;
-        if (g.at == 0 && ahead < plan.blocks) issue(ahead, g.s);
+        if (g.at == 0 && ahead < plan.blocks && g.poison == 0.f) issue(ahead, g.s);
         g.advance(plan);
       };
       if (kKeep && r == rows - 1) refill();  // every thread has its values of the last row

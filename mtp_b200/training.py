@@ -17,7 +17,8 @@ stream of its tensors' GPU, which need not be the current one. There is no CPU
 path. Gradients are first derivatives, backward; forward mode raises
 ``RuntimeError``. All sums are in fp32 or more and in an order that sizes and
 memory layout fix, not timing: the same call gives the same bits. (Should a
-bounded wait of a layer norm kernel run out, the rows that it was for are NaN.)
+bounded wait of a layer norm kernel run out, the rows that it was for are NaN,
+rows behind them may be, and so may columns of the sums over them.)
 """
 from __future__ import annotations
 
