@@ -32,6 +32,7 @@ namespace mtp {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPlainCtas = 32768;    // most of the plain kernels, whose 32-bit row index steps past the last row by as many
 constexpr int kSms = 148;
 constexpr int kRowThreads = 1024;    // most threads of a row in norm_row_kernel
 constexpr int kGroupThreads = 512;   // of a CTA of the ring kernels: 128 registers each
@@ -840,7 +841,7 @@ int forward_run(const NormArgs& a, cudaStream_t st) {
       return e == 32 ? forward_ring<T, N, 32, 1>(a, p, st) : e == 16 ? forward_ring<T, N, 16, 1>(a, p, st) : forward_ring<T, N, 8, 1>(a, p, st);
   }
   if (vectors > 8 * kRowThreads)
-    return launch(a.param_fp32 ? norm_kernel<T, float> : norm_kernel<T, T>, dim3(std::min(a.M, 1 << 20)), dim3(kThreads), 0, st, a);
+    return launch(a.param_fp32 ? norm_kernel<T, float> : norm_kernel<T, T>, dim3(std::min(a.M, kPlainCtas)), dim3(kThreads), 0, st, a);
   const int lanes = static_cast<int>(std::min<int64_t>((vectors + 31) / 32 * 32, kRowThreads));
   const int nv = static_cast<int>((vectors + lanes - 1) / lanes);
   auto* kernel = nv == 1 ? norm_row_kernel<T, N, 1> : nv <= 4 ? norm_row_kernel<T, N, 4> : norm_row_kernel<T, N, 8>;
@@ -879,7 +880,7 @@ int run(const NormArgs& a, bool backward, cudaStream_t st) {
     if (!fused) {
       if (a.grad_x)
         rc = launch(a.param_fp32 ? norm_rows_backward_kernel<T, float> : norm_rows_backward_kernel<T, T>,
-                    dim3(std::min(a.M, 1 << 20)), dim3(kThreads), 0, st, a);
+                    dim3(std::min(a.M, kPlainCtas)), dim3(kThreads), 0, st, a);
       parts = std::min(a.M, 64);
       if (rc == MTP_OK && (a.grad_weight || a.grad_bias))
         rc = launch(norm_columns_kernel<T>, dim3((a.H + kThreads - 1) / kThreads, parts), dim3(kThreads), 0, st, a);
