@@ -206,6 +206,7 @@ class _SortTokens(torch.autograd.Function):
         # positions, offsets and scales are not differentiable: they go around autograd, in `rest`
         rows, *others = _sort(x, ids, num_experts, expert_map, row_scales)
         ctx.save_for_backward(others[0])
+        ctx.pairs = ids.shape
         rest.extend(others)
         return rows
 
@@ -213,6 +214,7 @@ class _SortTokens(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_rows):
         (positions,) = ctx.saved_tensors
+        positions = _given_back("positions", positions, ctx.pairs, torch.int32, grad_rows.device)
         return _unsort(grad_rows.contiguous(), positions, None), None, None, None, None, None
 
 
@@ -220,13 +222,19 @@ class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, positions, weights):
         ctx.save_for_backward(rows if weights is not None and weights.requires_grad else None, positions, weights)
-        ctx.num_rows = rows.shape[0]
+        ctx.num_rows, ctx.pairs = rows.shape[0], positions.shape
         return _unsort(rows, positions, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         rows, positions, weights = ctx.saved_tensors
+        device = grad.device
+        positions = _given_back("positions", positions, ctx.pairs, torch.int32, device)
+        if weights is not None:
+            weights = _given_back("topk_weights", weights, ctx.pairs, torch.float32, device)
+        if rows is not None:
+            rows = _given_back("rows", rows, (ctx.num_rows, grad.shape[1]), grad.dtype, device)
         need_rows, _, need_weights = ctx.needs_input_grad
         grad_rows, grad_weights = _unsort_backward(grad.contiguous(), rows, ctx.num_rows, positions, weights, need_rows,
                                                    need_weights)

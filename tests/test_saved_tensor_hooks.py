@@ -155,6 +155,56 @@ def test_a_tensor_left_on_another_device_is_refused(entries, monkeypatch):
     assert "norm_backward" not in entries and "route_backward" not in entries
 
 
+def _pairs():
+    rows, weights = torch.randn(6, 5, requires_grad=True), torch.rand(3, 2, requires_grad=True)
+    return rows, torch.tensor([[0, 3], [4, 1], [2, 5]], dtype=I32), weights
+
+
+def test_unsort_takes_tensors_in_row_order(entries):
+    rows, positions, weights = _pairs()
+    hooks = Hooks(columns_first)
+    with hooks:
+        mtp_b200.unsort_tokens(rows, positions, weights).sum().backward()
+    _, at_rows, num_rows, _, at_positions, at_weights = entries["unsort_backward"][:6]
+    assert num_rows == 6 and len(hooks.given) == 3
+    assert not any(hooks.at(p) is not None for p in (at_rows, at_positions, at_weights))  # copies in row order
+
+
+def test_sort_takes_positions_in_row_order(entries):
+    x, hooks = torch.randn(3, 5, requires_grad=True), Hooks(columns_first)
+    with hooks:
+        mtp_b200.sort_tokens(x, torch.zeros(3, 2, dtype=I32), 4).rows.sum().backward()
+    assert len(hooks.given) == 1 and hooks.at(entries["unsort"][3]) is None
+
+
+def test_sort_and_unsort_without_hooks_make_no_copies(entries):
+    rows, positions, weights = _pairs()
+    mtp_b200.unsort_tokens(rows, positions, weights).sum().backward()
+    args = entries["unsort_backward"]
+    assert (args[1], args[4], args[5]) == (rows.data_ptr(), positions.data_ptr(), weights.data_ptr())
+
+
+@pytest.mark.parametrize("wrong", WRONG.values(), ids=WRONG)
+@pytest.mark.parametrize("which", range(3))
+def test_unsort_refuses_other_tensors(entries, wrong, which):
+    (rows, positions, weights), seen = _pairs(), []
+    with Hooks(lambda t: (seen.append(t), wrong(t) if len(seen) == which + 1 else t)[1]):
+        y = mtp_b200.unsort_tokens(rows, positions, weights)
+        with pytest.raises(RuntimeError, match="saved"):
+            y.sum().backward()
+    assert len(seen) == 3 and "unsort_backward" not in entries
+
+
+@pytest.mark.parametrize("wrong", WRONG.values(), ids=WRONG)
+def test_sort_refuses_other_positions(entries, wrong):
+    x = torch.randn(3, 5, requires_grad=True)
+    with Hooks(wrong):
+        r = mtp_b200.sort_tokens(x, torch.zeros(3, 2, dtype=I32), 4)
+        with pytest.raises(RuntimeError, match="saved"):
+            r.rows.sum().backward()
+    assert "unsort" not in entries
+
+
 @pytest.mark.gpu
 class TestOnTheGpu:
     @pytest.fixture(params=["on the host", "pinned", "dense", "wider", "columns first", "checkpoint"])
@@ -219,3 +269,18 @@ class TestOnTheGpu:
         (want,) = torch.autograd.grad(mtp_b200.embed_tokens(ids, table), table, gy)
         (got,) = torch.autograd.grad(around(lambda t: mtp_b200.embed_tokens(ids, t), table), table, gy)
         assert torch.equal(got, want)
+
+    def test_sort_and_unsort(self, around):
+        g = torch.Generator(device="cuda").manual_seed(2)
+        x = torch.randn(90, 40, generator=g, device="cuda", requires_grad=True)
+        w = torch.rand(90, 3, generator=g, device="cuda", requires_grad=True)
+        ids = torch.randint(-1, 7, (90, 3), generator=g, device="cuda", dtype=I32)
+        gy = torch.randn(90, 40, generator=g, device="cuda")
+
+        def there_and_back(x, w):
+            r = mtp_b200.sort_tokens(x, ids, 7)
+            return mtp_b200.unsort_tokens(r.rows * 2, r.positions, w)
+
+        want = torch.autograd.grad(there_and_back(x, w), (x, w), gy)
+        got = torch.autograd.grad(around(there_and_back, x, w), (x, w), gy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
