@@ -337,7 +337,8 @@ MTP_API int mtp_route_tokens_backward(const void* logits, int64_t logits_stride,
  * fp16 or fp32, rows x_stride elements apart), the variance over H, in fp32,
  * rounded once. weight, bias [H] (NULL: 1 and 0): param_dtype, the type of x or
  * fp32. stats [M, 2] (or NULL): mean and 1 / sqrt(var + eps) of each row, for
- * the gradient.                                                             */
+ * the gradient. Should a bounded wait run out, the rows that it was for are NaN,
+ * and rows behind them may be; the same holds for the gradients below.      */
 MTP_API int mtp_layer_norm(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t H, const void* weight,
                            const void* bias, int32_t param_dtype, float eps, void* y, float* stats, void* stream);
 /* Its gradients for grad [M, H] (contiguous): grad_x [M, H] in the type of x,

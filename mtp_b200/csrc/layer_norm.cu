@@ -7,16 +7,27 @@
 //           dx = rstd (wg - mean(wg) - xhat mean(wg xhat)),
 //           dw = sum over the rows of g xhat, db = sum of g.
 //
-// All sums in fp32 in a fixed order; results are rounded once. In the ring
-// 1 / sqrt is rsqrtf, within 2 units in the last place.
+// All sums in fp32, in an order that sizes and memory layout fix; results are
+// rounded once. In the ring 1 / sqrt is rsqrtf, within 2 units in the last place,
+// and sums go warp by warp: the bits of a row may differ between calls of up to 296
+// rows, which norm_row_kernel takes, and of more.
 //
 // The bytes are x in and y out; for the gradients x and grad in and dx out. What
 // keeps the kernels from HBM's rate is the work per row between its two sums
 // (16384 x 8192 bf16: 14 and 24 instructions a value, one barrier a row):
-//   8192 x 2048 bf16:  22 us forward, 37 backward (bytes alone 10 and 15)
-//   16384 x 8192 bf16: 111 us and 181 us (82 and 123: 4.8 and 4.5 TB/s)
-//   16384 x 4096 fp32: 95 us and 127 us (82 and 123: 5.6 and 6.3 TB/s)
-//   one row of 2048: 2.3 us, 6.1 us
+//   8192 x 2048 bf16:  19 us forward, 36 backward (bytes alone 10 and 15)
+//   16384 x 8192 bf16: 113 us and 182 us (82 and 123: 4.7 and 4.4 TB/s)
+//   16384 x 4096 fp32: 96 us and 129 us (82 and 123: 5.6 and 6.2 TB/s)
+//   20000 x 5001 bf16: 147 us and 371 us (61 and 92: values one by one)
+//   one row of 2048: 2.5 us, 6.4 us
+// Rows that the ring has no room for (two stages of whole rows and the parameters:
+// forward up to 16384 values of 16 bits and 14336 of fp32, the gradients, with x
+// and grad in it, 16384 and 11264) take norm_row_kernel forward, up to its 8192
+// vectors, and otherwise plain kernels that read a row three times, a value a load:
+//   4096 x 12288 fp32: 92 us (ring) and 305 us (62 and 92)
+//   4096 x 16384 fp32: 146 us and 475 us (82 and 123)
+//   8192 x 20480 bf16: 314 us and 818 us (103 and 154)
+//   8192 x 32769 bf16: 790 us and 1634 us (164 and 246)
 // Taken one after the other, 16384 x 8192 bf16 there and back: rows read three
 // times and columns by a kernel of their own 197 + 681 us; one pass, rows in
 // registers 176 + 463; a ring of bulk copies with one value a load 188 + 307, with
@@ -96,8 +107,9 @@ __device__ __forceinline__ void params(const void* p, bool fp32, int c, float ot
 // ---------------------------------------------------------------------------
 // forward of a few rows: a row in the registers of blockDim.x threads
 // ---------------------------------------------------------------------------
-// (and of rows wider than the ring's 16384). One row of 2048 bf16: 2.2 us; for
-// 8192 of them it takes 39 us, the ring 21.
+// (and of rows wider than the ring's 16384 values of 16 bits or 14336 of fp32, up
+// to 8192 vectors). One row of 2048 bf16: 2.5 us; for 8192 of them it takes 39 us,
+// the ring 19.
 template <typename T, int N, int NV>
 __global__ void __launch_bounds__(kRowThreads, 1) norm_row_kernel(const NormArgs a) {
   using V = Vec<T, N>;

@@ -17,12 +17,18 @@
 // the same order; the counts are integers. So results do not depend on timing.
 //
 // The logits are read once forward and once, with the gradient written,
-// backward. Instructions bound it, not HBM: 65536 x 512 logits fill 62 % of the
-// issue slots forward, 52 % backward.
-//   8192 x 256, top-8:  16.6 us forward (two launches), 7.1 us backward
-//   65536 x 512, top-8: 88 us and 54 us (bytes alone 21 and 41)
-//   32768 x 1024, top-8: 72 us and 64 us (21 and 41)
-//   one token: 4.3 us and 2.3 us
+// backward. Forward the dependent steps of a token bound it (k rounds of maximum
+// and vote, ranking in shared memory, exponentials), with 16 warps a SM to hide
+// them from 257 experts on: 65536 x 512 logits fill 62 % of the issue slots and a
+// quarter of HBM's rate. The gradient is near HBM's (5 TB/s there).
+//   8192 x 256, top-8:  16.5 us forward (two launches), 6.3 us backward
+//   65536 x 512, top-8: 89 us and 55 us (bytes alone 21 and 41)
+//   32768 x 1024, top-8: 71 us and 63 us (21 and 41)
+//   one token: 4.1 us and 2.3 us
+// More choices, and rows whose logits are all equal, go one by one (see there):
+//   8192 x 256, top-16, 20, 24 and 32: 31, 64, 97 and 124 us forward
+//   8192 x 1024, top-8, 20 and 32:     28, 318 and 558 us
+//   equal logits, 8192 x 256 and 65536 x 512, top-8: 42 us and 540 us
 #include "rows.cuh"
 
 #include <math.h>
@@ -122,8 +128,12 @@ __device__ __forceinline__ void write_choice(const RouteLossArgs& a, float p, in
   }
 }
 
-// The k largest, one after the other: a maximum over the warp each. For the few
-// rows that choose() does not take: it keeps no registers and reads the row again.
+// The k largest, one after the other: a maximum over the warp each. For the rows
+// that choose() does not take: those with a NaN, without k finite logits, or with
+// more than 32 candidates. Of normal logits of 256 experts the last are none for
+// k = 8, 0.1 % for 16, 15 % for 20, 92 % for 24 and all for 32 (1024 experts and
+// k = 20: 26 %); rows of more than 32 equal logits are too. It keeps no registers
+// and reads the row again k times.
 template <typename T>
 __device__ __forceinline__ void choose_one_by_one(const RouteLossArgs& a, int t, float2 ms, int64_t o, int* hist) {
   const int lane = threadIdx.x & 31;
